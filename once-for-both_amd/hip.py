@@ -280,13 +280,12 @@ _side_streams, _side_keep, _side_dirty = {}, [], [False]
 
 def ensure_side_stream(device, priority=None):
     """Creates the side stream of `device` (idempotent; `priority` given: replaces it, after joining the old one).
-    HIP maps streams onto its hardware queues (GPU_MAX_HW_QUEUES, default 4) in creation order: with RCCL's own streams created first a
-    normal-priority side stream lands on the main stream's hardware queue - the two then run one after the other and the
-    weight-gradient overlap is lost (one rank, DeiT-S bs 128: 27.0 instead of 25.0 ms per step).  A HIGH-priority stream has a queue
-    of its own whatever was created before it (25.4 ms with RCCL, 25.0 without), so that is the default for eager steps.  Inside a
-    captured hipGraph the placement of parallel branches is a lottery (a high-priority branch, GPU_MAX_HW_QUEUES = 8 or merely other
-    streams in the process make the replay of the bs-128 step 37 instead of 26 ms): engine.GraphedStep captures single-stream
-    (scripts/lab/queue_matrix.sh has the table: queues x priority x eager / graph x plain / one-rank RCCL)."""
+    It has the default priority unless the caller (or OFB_SIDE_PRIORITY) asks for another: work on streams of different priorities has
+    hung these GPUs.  HIP maps streams onto its hardware queues (GPU_MAX_HW_QUEUES, default 4) in creation order, so create it before
+    RCCL's own streams exist: created after them it can land on the main stream's hardware queue - the two then run one after the other
+    and the weight-gradient overlap is lost (one rank, DeiT-S bs 128: 27.0 instead of 25.0 ms per step).  Inside a captured hipGraph the
+    placement of parallel branches is a lottery (merely other streams in the process make the replay of the bs-128 step 37 instead of
+    26 ms): engine.GraphedStep captures single-stream (scripts/lab/queue_matrix.sh has the table)."""
     device = torch.device(device)
     if device.index is None:
         device = torch.device('cuda', torch.cuda.current_device())
@@ -295,7 +294,7 @@ def ensure_side_stream(device, priority=None):
         if side is not None:
             join_side()
             torch.cuda.current_stream(device).wait_stream(side)
-        pr = int(os.environ.get('OFB_SIDE_PRIORITY', '-1')) if priority is None else int(priority)
+        pr = int(os.environ.get('OFB_SIDE_PRIORITY', '0')) if priority is None else int(priority)
         side = _side_streams[device] = torch.cuda.Stream(device=device, priority=pr)
     return side
 
