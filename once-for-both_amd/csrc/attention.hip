@@ -845,7 +845,7 @@ int check_shape(int B, int N, int H, int dh) {
   return OFB_OK;
 }
 
-// out[0] = max |x[i]| (out zeroed by a memset node ahead of the launch)
+// out[0] = max |x[i]| (out zeroed by a fill kernel ahead of the launch)
 __global__ __launch_bounds__(256) void amax_kernel(const float* __restrict__ x, size_t n, float* __restrict__ out) {
   __shared__ float red[4];
   float am = 0.f;
@@ -862,7 +862,7 @@ __global__ __launch_bounds__(256) void amax_kernel(const float* __restrict__ x, 
 extern "C" int ofb_amax(const float* x, int64_t n, float* out, void* stream) {
   if (!x || !out || n <= 0) return OFB_EINVAL;
   hipStream_t s = (hipStream_t)stream;
-  if (hipMemsetAsync(out, 0, 4, s) != hipSuccess) return (int)hipGetLastError();
+  ofb_zero_words(out, 1, s);
   const int64_t nb = (n + 255) / 256;
   hipLaunchKernelGGL(amax_kernel, dim3((unsigned)(nb < 1024 ? nb : 1024)), dim3(256), 0, s, x, (size_t)n, out);
   return ofb_launch_status();
@@ -918,7 +918,7 @@ int attention_bwd_launch(const float* qkv, const float* out, const float* lse, c
   if (hipFuncSetAttribute(lng ? (const void*)attn_bwd_kernel<true> : (const void*)attn_bwd_kernel<false>,
                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)BWD_LDS) != hipSuccess)
     return (int)hipGetLastError();
-  if (dqkv_amax && !amax_per_wg && hipMemsetAsync(dqkv_amax, 0, 4, s) != hipSuccess) return (int)hipGetLastError();
+  if (dqkv_amax && !amax_per_wg) ofb_zero_words(dqkv_amax, 1, s);
   ofb_prof_pre(4, s, 10.0 * B * H * (double)N * N * dh);
   if (!lng)
     hipLaunchKernelGGL(attn_bwd_kernel<false>, dim3(B * H), dim3(AB_THREADS), BWD_LDS, s, qkv, out, lse, dout, dqkv, B, N, H, dh, scale,

@@ -101,7 +101,7 @@ __device__ __forceinline__ void store_h4(char* slot, float v0, float v1, float v
 
 // ---- statistics + conversion f32 <-> H-format ---------------------------------------------------------------------
 // value = X * rowscale[r / rs_div] (optional).  Stage 1: hdr.amax = max|value|, hdr.rn2sq = max_r sum_c value^2 by atomic max
-// (header zeroed by a memset node ahead of the launch); one wave per row, grid-stride.
+// (header zeroed by a fill kernel ahead of the launch); one wave per row, grid-stride.
 // One wave's rows r_first, r_first + r_stride, ...: FOUR rows at a time - their loads are in flight together and their row sums are
 // reduced side by side (one row at a time every row cost a memory round trip and a reduction chain of its own: the bound passes ran
 // at 9 % of the HBM rate).  Per row the same sum in the same order; rows past the end take part with factor 0.
@@ -1582,10 +1582,10 @@ extern "C" int64_t ofb_hformat_bytes(int32_t R, int32_t C) {
 }
 
 namespace {
-// header.amax for the conversion kernels: measured (memset + statistics pass) or the caller's bound
+// header.amax for the conversion kernels: measured (fill + statistics pass) or the caller's bound
 int h_prepare_header(const float* X, int R, int C, int ld, void* P, const float* rowscale, int rs_div, const float* bound, hipStream_t s) {
   if (bound) return 0;                                 // the conversion kernel reads the caller's scalar itself
-  if (hipMemsetAsync(P, 0, 16, s) != hipSuccess) return (int)hipGetLastError();
+  ofb_zero_words(P, 4, s);
   const int nb = ofb_cdiv(R, 4) < 512 ? ofb_cdiv(R, 4) : 512;
   hipLaunchKernelGGL(hstat_kernel, dim3(nb), dim3(256), 0, s, X, R, C, ld, (ofb_hhdr*)P, rowscale, rs_div);
   return 0;
@@ -1610,7 +1610,7 @@ extern "C" int ofb_patchify_hformat(const float* img, int32_t B, int32_t Cin, in
   if (R > 0x7fffffff / 4 || Cc > 65536) return OFB_ELIMIT;
   hipStream_t s = (hipStream_t)stream;
   const int ncb = (int)((Cc + 15) / 16), rgs = (int)(((R + 15) / 16) * 4);
-  if (hipMemsetAsync(P, 0, 16, s) != hipSuccess) return (int)hipGetLastError();
+  ofb_zero_words(P, 4, s);
   hipLaunchKernelGGL(hstat_flat_kernel, dim3(2048), dim3(256), 0, s, img, (size_t)B * Cin * H * W, (ofb_hhdr*)P);
   hipLaunchKernelGGL(patchify_hformat_kernel, dim3((ncb * 16 + 255) / 256, rgs), dim3(256), 0, s, img, B, Cin, H, W, patch, (char*)P, ncb);
   return ofb_launch_status();

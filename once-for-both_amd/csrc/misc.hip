@@ -520,7 +520,7 @@ extern "C" int ofb_ls_cross_entropy(const float* logits, const int64_t* labels, 
 
 // The two readers of the final token stream [B][T = L + 1][D] (vision_transformer.py:735-744): block r < B copies image r's cls row,
 // block B + i the token row of masked patch ids[i] (global patch id p = b L + l -> token row p + p / L + 1).  One launch for what was
-// three index launches, a strided copy and a gather; the backward zero-fills the stream gradient (a memset node) and scatters both
+// three index launches, a strided copy and a gather; the backward zero-fills the stream gradient (a fill kernel) and scatters both
 // kinds of rows (disjoint, unique: plain stores) in one launch.
 __global__ __launch_bounds__(128) void token_taps_kernel(const float* __restrict__ src_stream, const float* __restrict__ rows_cls,
                                                          const float* __restrict__ rows_z, const int32_t* __restrict__ ids, int B, int T,
@@ -553,7 +553,7 @@ extern "C" int ofb_token_taps_bwd(const float* dcls, const float* dz, const int3
                                   int32_t D, float* dstream, void* stream) {
   if (!dstream || B <= 0 || T < 2 || D <= 0 || n_ids < 0 || (dz && n_ids > 0 && !patch_ids)) return OFB_EINVAL;
   hipStream_t s = (hipStream_t)stream;
-  if (hipMemsetAsync(dstream, 0, (size_t)B * T * D * sizeof(float), s) != hipSuccess) return OFB_EINVAL;
+  ofb_zero_words(dstream, (int64_t)B * T * D, s);
   const int n = dz ? n_ids : 0;
   if (!dcls && n == 0) return ofb_launch_status();
   hipLaunchKernelGGL(token_taps_kernel, dim3(B + n), dim3(128), 0, s, (const float*)nullptr, dcls, dz, patch_ids, B, T, D, (float*)nullptr,
@@ -614,10 +614,11 @@ extern "C" int ofb_scale_by_scalar(const float* x, const float* scalar_dev, floa
 
 __global__ __launch_bounds__(256) void ema_kernel(const ofb_ema_tensor* __restrict__ tab, float decay, float omd,
                                                   const int32_t* __restrict__ skip) {
+#pragma clang fp contract(off)          // torch rounds the two products and the sum separately (HIP's __fmul_rn would contract)
   if (skip && *skip) return;
   const ofb_ema_tensor tt = tab[blockIdx.y];
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < tt.n; i += (int64_t)gridDim.x * 256)
-    tt.ema[i] = __fadd_rn(__fmul_rn(tt.ema[i], decay), __fmul_rn(omd, tt.src[i]));
+    tt.ema[i] = tt.ema[i] * decay + omd * tt.src[i];
 }
 
 extern "C" int ofb_ema_update(const ofb_ema_tensor* table_dev, int32_t n_tensors, int64_t max_numel, float decay,

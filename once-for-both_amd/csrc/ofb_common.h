@@ -14,6 +14,17 @@ static inline bool ofb_aligned16(const void* p) { return (((uintptr_t)p) & 15u) 
 static inline int ofb_cdiv(int a, int b) { return (a + b - 1) / b; }
 __device__ __forceinline__ bool ofb_aligned16_dev(const void* p) { return (((uintptr_t)p) & 15u) == 0; }
 
+// Clears n 32-bit words with a kernel: a memset recorded into a captured graph has given wrong results on replays after the first, so no
+// entry point that a caller may capture clears memory with hipMemsetAsync.
+static __global__ __launch_bounds__(256) void ofb_zero_words_kernel(uint32_t* __restrict__ p, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0u;
+}
+static inline void ofb_zero_words(void* p, int64_t n, hipStream_t s) {
+  if (n <= 0) return;
+  const int64_t g = (n + 255) / 256;
+  hipLaunchKernelGGL(ofb_zero_words_kernel, dim3((unsigned)(g < 2048 ? g : 2048)), dim3(256), 0, s, (uint32_t*)p, n);
+}
+
 // profiling hook (prof.hip): brackets a launch with events when enabled
 void ofb_prof_pre(int tag, hipStream_t s, double work);
 void ofb_prof_post(int tag, hipStream_t s);

@@ -474,7 +474,7 @@ __global__ __launch_bounds__(256) void ln_bwd_p_kernel(const float* __restrict__
 // Bound of LayerNorm backward's scaled output BEFORE it is computed (the exponent of its H-format planes): dx = rstd P(gamma * dy)
 // with P an orthogonal projection (it removes the components along 1 and xhat), so per row
 //   |dx|_inf <= |dx|_2 <= rstd |gamma * dy|_2   (+ the residual gradient's own max / norm), times the row's DropPath factor.
-// header.amax / header.rn2sq (zeroed by a memset node) take the maxima over the rows.  NJ > 0: even D, one wave per 4-row group, the
+// header.amax / header.rn2sq (zeroed by a fill kernel) take the maxima over the rows.  NJ > 0: even D, one wave per 4-row group, the
 // four rows' float2 loads in flight together (an HBM-bound pass over dy: 8-10 us for [25216][384]); NJ == 0: any D, a wave per row.
 template <int NJ>
 __global__ __launch_bounds__(256) void ln_bwd_stat_kernel(const float* __restrict__ dy, const float* __restrict__ gamma,
