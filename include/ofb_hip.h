@@ -533,6 +533,61 @@ int ofb_jpeg_decode_batch(const uint8_t* const* files, const int64_t* nbytes, in
 int ofb_jpeg_decode_pixels(const ofb_jpeg_job* jobs_dev, int32_t n_images, int32_t max_blocks, int32_t max_w, int32_t max_h,
                            const int16_t* coef_dev, uint8_t* planes_dev, uint8_t* out_dev, void* stream);
 
+/* ---- attention with a learned relative position bias by buckets (csrc/relpos.hip) -----------------------------------------------
+ * S = scale q k^T + table[bucket(pos_k[j] - pos_q[i])][h], softmax over the keys j < key_lens[b] (and j <= i + q_offset if causal), times v;
+ * a query that sees no key has output and gradients 0.  q, k, v, out, dout, dq, dk, dv: elements of `dtype` (0 f32, 1 bf16, 2 f16) at
+ * b * sb + token * st + head * sh + channel, strides in elements (read tensors: multiples of 16 bytes and 16-byte aligned; written ones:
+ * strides multiples of 4 elements).  d: a multiple of 8, at most 128.  lut[width]: bucket of each difference lo .. lo + width - 1 (differences are clamped; width <= 4096);
+ * bucket_start[n_buckets + 1] / bucket_order[width]: the lut inverted (dtable only).  pos_q / pos_k: positions of the queries and keys, or
+ * both NULL: i + q_offset and j.  Only index ranges are checked: lut entries must be < n_buckets.
+ * f32 (forward and backward) and f16 (backward) read upper bounds of the tensors from bound_*: n_bound (n_bound_do) partial maxima each
+ * (1 .. 256; ofb_relpos_amax writes 256). */
+typedef struct {
+  const void *q, *k, *v;
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+  void* out;
+  int64_t o_sb, o_st, o_sh;
+  float* out32;                 /* [B][Nq][H][d] unrounded output: read by the backward (f32: out itself if contiguous); may be NULL forward */
+  float* stats;                 /* [B][H][Nq][2] row maximum (log2 units) and 1 / row sum; may be NULL forward */
+  const float* table;           /* [n_buckets][H] */
+  const int32_t *lut, *bucket_start, *bucket_order, *pos_q, *pos_k, *key_lens;
+  int32_t lo, width, n_buckets, q_offset, causal, dtype;
+  int32_t B, H, Nq, Nk, d;
+  float scale;
+  const float *bound_q, *bound_k, *bound_v, *bound_do;
+  int32_t n_bound, n_bound_do;
+  float *split_o, *split_ml;    /* workspaces of ofb_relpos_sizes floats */
+  const void* dout;
+  int64_t do_sb, do_st, do_sh;
+  void *dq, *dk, *dv;
+  int64_t dq_sb, dq_st, dq_sh, dk_sb, dk_st, dk_sh, dv_sb, dv_st, dv_sh;
+  float* dtable;                /* [n_buckets][H], or NULL */
+  float *delta, *partial, *sat; /* delta: [B][H][Nq]; the others of ofb_relpos_sizes floats */
+} ofb_relpos_args;
+/* out4[0..3]: floats of split_o, split_ml, partial, sat (0: not needed) */
+int ofb_relpos_sizes(const ofb_relpos_args* a, int64_t* out4);
+/* 256 partial maxima of |x| for `count` of q, k, v, dout (0 .. 3) from `first` on, into bound_*; tokens nobody sees are left out */
+int ofb_relpos_amax(const ofb_relpos_args* a, int32_t first, int32_t count, void* stream);
+int ofb_relpos_fwd(const ofb_relpos_args* a, void* stream);
+int ofb_relpos_bwd(const ofb_relpos_args* a, void* stream);
+
+/* ---- distillation from a teacher's top logits (csrc/distill.hip) ----------------------------------------------------------------
+ * z, values, dz: elements of `dtype` (0 f32, 1 bf16, 2 f16), contiguous [R][V] and [R][K], z and dz 16-byte aligned; indices: int32, or int64 if idx64.
+ * An entry whose class is outside 0 .. V - 1 or whose value is -inf is no entry.  rest [R] (or NULL): log-sum-exp of the teacher's other
+ * logits / tau (ignored where every class is stored).  A row without an entry has loss and gradient 0.  K <= 1024, K <= V.
+ * stats: [R][8], kept for the backward; part: [R][ofb_distill_segments][2] if that is over 1; row_loss [R]; loss (or NULL) = loss_scale times their sum.
+ * up: the upstream gradient, one value or (up_rows) one per row; dz = up * grad_scale * (d row_loss / d z / tau). */
+int ofb_distill_segments(int64_t R, int32_t V);
+int ofb_distill_fwd(const void* z, const void* values, const void* indices, int32_t idx64, const float* rest, int64_t R, int32_t V, int32_t K,
+                    float tau, int32_t dtype, float* stats, float* part, float* row_loss, double loss_scale, float* loss, void* stream);
+int ofb_distill_bwd(const void* z, const void* values, const void* indices, int32_t idx64, int64_t R, int32_t V, int32_t K, float tau,
+                    int32_t dtype, const float* stats, const float* up, int32_t up_rows, float grad_scale, void* dz, void* stream);
+/* the K largest logits of each row in descending order (NaN first; ties: the lowest class first) and rest = log-sum-exp of the others / tau (-inf if
+ * there are none).  cand: [R][ofb_top_logits_segments][K] 64-bit words, part: [R][segments][2], if that is over 1. */
+int ofb_top_logits_segments(int64_t R, int32_t V, int32_t K);
+int ofb_top_logits(const void* z, int64_t R, int32_t V, int32_t K, float tau, int32_t dtype, void* values, int32_t* indices, float* rest,
+                   void* cand, float* part, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

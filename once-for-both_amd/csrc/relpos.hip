@@ -1,0 +1,1188 @@
+// Attention with a learned relative position bias by buckets, forward and backward, for f32, bf16 and f16 tensors:
+//
+//   S_ij = scale q_i . k_j + T[bucket(pos_k[j] - pos_q[i])][h],   P = softmax_j S over the keys that query i sees,   O = P V
+//   D_i = dO_i . O_i,  dP = dO V^T,  dS = P (dP - D),  dV = P^T dO,  dQ = scale dS K,  dK = scale dS^T Q,
+//   dT[c][h] = sum over the batch and over the pairs of bucket c of dS.
+//
+// The bias never exists as a matrix: a pair's bucket goes by the clamped difference of two integer positions, so each head's bias is a
+// vector w[difference - lo] (a few hundred floats, already times log2 e) that every workgroup gathers from the table into LDS.  Positions
+// are j and i + q_offset, or come from two int32 arrays (a patch grid: y (2 w - 1) + x makes one number of two coordinates).
+//
+// Matrix products: v_mfma_f32_32x32x16.  bf16 and f16 operands as they are; f32 operands as two f16 planes of a power-of-two scaled copy and
+// three products (hformat.h), with the exponents from device-side maxima.  Scores, softmax statistics, dS and all sums are f32 (the
+// table's gradient sums in 64 bits); P and dS are rounded to the operand type for the second product - bf16, or f16 times 2^14 and a power
+// of two that keeps |dS| < 2^15, in two planes again for f32.
+//
+// Operand conventions (lane l, hh = l >> 5): A[row = l & 31][k = 8 hh + j], B[k = 8 hh + j][col = l & 31], accumulator register r holds
+// row 8 (r >> 2) + 4 hh + (r & 3) of column l & 31.  A reduction may run over its index in any order that both operands share, so an
+// accumulator feeds the next product as its B operand without leaving its registers: registers 8 s .. 8 s + 7 are the k-slots of step s,
+// and the A operand is read with rows 16 s + 8 (j >> 2) + 4 hh + (j & 3) - two transposing LDS reads of four rows each.
+#include "hformat.h"
+
+#define RP_F32 0
+#define RP_BF16 1
+#define RP_F16 2
+#define RP_THREADS 256
+#define RP_TILE 128              /* queries (forward, dQ) or keys (dK dV, table gradient) of a workgroup: four waves of 32 */
+#define RP_PAD 4                 /* entries of w on either side, so that four consecutive differences need one clamp */
+#define RP_WMAX 4096
+#define RP_PE 14                 /* f16 planes hold P 2^14 */
+#define RP_NBOUND 256            /* partial maxima of a tensor */
+
+namespace {
+
+typedef __bf16 rp_bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 rp_bf16x2 __attribute__((ext_vector_type(2)));
+typedef short rp_s16x4 __attribute__((ext_vector_type(4)));
+typedef short rp_s16x8 __attribute__((ext_vector_type(8)));
+typedef rp_s16x8 rp_frag;
+
+template <int DT> struct rp_type { static constexpr int NP = 1, ES = 2; };
+template <> struct rp_type<RP_F32> { static constexpr int NP = 2, ES = 4; };
+
+// rows of a streamed tile: 64, or 32 where two planes or wide heads would take the LDS of a second workgroup
+template <int DT, int DP> struct rp_geo {
+  static constexpr int NP = rp_type<DT>::NP;
+  static constexpr int KB = (NP == 1 && DP <= 64) ? 64 : 32;
+  static constexpr int PITCH = DP * 2 + 16;                  // bytes of a row of one plane: 8 rows' 16-byte chunks fall into different banks
+  static constexpr int PLANE = KB * PITCH;
+  static constexpr int TENSOR = NP * PLANE;
+  static constexpr int STAGE = 2 * TENSOR;                   // two tensors (K and V, or Q and dO)
+  static constexpr int CHUNKS = KB * DP / 8;
+  static constexpr int PER = (CHUNKS + RP_THREADS - 1) / RP_THREADS;
+};
+
+template <int DT>
+__device__ __forceinline__ f32x16 rp_mm1(rp_frag a, rp_frag b, f32x16 c) {
+  if constexpr (DT == RP_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(rp_bf16x8, a), __builtin_bit_cast(rp_bf16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(ofb_f16x8, a), __builtin_bit_cast(ofb_f16x8, b), c, 0, 0, 0);
+}
+template <int DT, int NP>
+__device__ __forceinline__ f32x16 rp_mm(const rp_frag (&a)[NP], const rp_frag (&b)[NP], f32x16 c) {
+  if constexpr (NP == 2) {                                   // smallest terms first; the dropped one is below 2^-22 of the product
+    c = rp_mm1<DT>(a[1], b[0], c);
+    c = rp_mm1<DT>(a[0], b[1], c);
+  }
+  return rp_mm1<DT>(a[0], b[0], c);
+}
+__device__ __forceinline__ f32x16 rp_zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+// eight consecutive elements of a row as the type keeps them
+template <int DT> struct rp_chunk { uint4 v; };
+template <> struct rp_chunk<RP_F32> { f32x4 v[2]; };
+template <int DT>
+__device__ __forceinline__ rp_chunk<DT> rp_zero_chunk() {
+  rp_chunk<DT> c;
+  if constexpr (DT == RP_F32) c.v[0] = c.v[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  else c.v = make_uint4(0, 0, 0, 0);
+  return c;
+}
+template <int DT>
+__device__ __forceinline__ rp_chunk<DT> rp_load_chunk(const char* p) {
+  rp_chunk<DT> c;
+  if constexpr (DT == RP_F32) { c.v[0] = reinterpret_cast<const f32x4*>(p)[0]; c.v[1] = reinterpret_cast<const f32x4*>(p)[1]; }
+  else c.v = *reinterpret_cast<const uint4*>(p);
+  return c;
+}
+template <int DT>
+__device__ __forceinline__ void rp_planes(const rp_chunk<DT>& c, float hs, rp_frag (&out)[rp_type<DT>::NP]) {
+  if constexpr (DT == RP_F32) {
+    unsigned h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ofb_hsplit_pair(c.v[i >> 1][2 * (i & 1)] * hs, c.v[i >> 1][2 * (i & 1) + 1] * hs, h[i], l[i]);
+    out[0] = __builtin_bit_cast(rp_frag, make_uint4(h[0], h[1], h[2], h[3]));
+    out[1] = __builtin_bit_cast(rp_frag, make_uint4(l[0], l[1], l[2], l[3]));
+  } else {
+    out[0] = __builtin_bit_cast(rp_frag, c.v);
+  }
+}
+template <int DT>
+__device__ __forceinline__ float rp_chunk_at(const rp_chunk<DT>& c, int i) {
+  if constexpr (DT == RP_F32) return c.v[i >> 2][i & 3];
+  else if constexpr (DT == RP_BF16) return (float)__builtin_bit_cast(rp_bf16x8, c.v)[i];
+  else return (float)__builtin_bit_cast(ofb_f16x8, c.v)[i];
+}
+__device__ __forceinline__ unsigned rp_pk_bf16(float a, float b) {
+  ofb_f32x2 v = {a, b};
+  return __builtin_bit_cast(unsigned, __builtin_convertvector(v, rp_bf16x2));
+}
+// eight ALREADY SCALED floats as the operand of the second product
+template <int DT>
+__device__ __forceinline__ void rp_pack8(const float (&x)[8], rp_frag (&out)[rp_type<DT>::NP]) {
+  unsigned h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == RP_F32) ofb_hsplit_pair(x[2 * i], x[2 * i + 1], h[i], l[i]);
+    else if constexpr (DT == RP_BF16) h[i] = rp_pk_bf16(x[2 * i], x[2 * i + 1]);
+    else h[i] = ofb_pk_f16(x[2 * i], x[2 * i + 1]);
+  }
+  out[0] = __builtin_bit_cast(rp_frag, make_uint4(h[0], h[1], h[2], h[3]));
+  if constexpr (DT == RP_F32) out[1] = __builtin_bit_cast(rp_frag, make_uint4(l[0], l[1], l[2], l[3]));
+}
+// four consecutive elements of an output row
+template <int DT>
+__device__ __forceinline__ void rp_store4(char* p, float a, float b, float c, float d) {
+  if constexpr (DT == RP_F32) *reinterpret_cast<f32x4*>(p) = f32x4{a, b, c, d};
+  else if constexpr (DT == RP_BF16) *reinterpret_cast<uint2*>(p) = make_uint2(rp_pk_bf16(a, b), rp_pk_bf16(c, d));
+  else *reinterpret_cast<uint2*>(p) = make_uint2(ofb_pk_f16(a, b), ofb_pk_f16(c, d));
+}
+
+// a [rows][DP] tile on its way from memory to LDS: one register image per thread, loaded a tile ahead
+template <int DT, int DP>
+struct rp_stage {
+  using G = rp_geo<DT, DP>;
+  rp_chunk<DT> c[G::PER];
+  __device__ __forceinline__ void load(const char* base, int64_t row_bytes, int row0, int row_end, int d) {
+#pragma unroll
+    for (int i = 0; i < G::PER; ++i) {
+      const int id = threadIdx.x + RP_THREADS * i, row = row0 + id / (DP / 8), ch = (id % (DP / 8)) * 8;
+      c[i] = rp_zero_chunk<DT>();
+      if (row < row_end && ch < d && (G::CHUNKS % RP_THREADS == 0 || id < G::CHUNKS)) c[i] = rp_load_chunk<DT>(base + (int64_t)row * row_bytes + ch * rp_type<DT>::ES);
+    }
+  }
+  __device__ __forceinline__ void store(char* lds, float hs) const {
+#pragma unroll
+    for (int i = 0; i < G::PER; ++i) {
+      const int id = threadIdx.x + RP_THREADS * i;
+      if (G::CHUNKS % RP_THREADS != 0 && id >= G::CHUNKS) continue;
+      rp_frag f[G::NP];
+      rp_planes<DT>(c[i], hs, f);
+#pragma unroll
+      for (int p = 0; p < G::NP; ++p) *reinterpret_cast<rp_frag*>(lds + p * G::PLANE + (id / (DP / 8)) * G::PITCH + (id % (DP / 8)) * 16) = f[p];
+    }
+  }
+};
+
+// A operand from an LDS tile, rows along the tile's rows: k-step ks of row0 + (l & 31)
+template <int DT, int DP>
+__device__ __forceinline__ void rp_rows(const char* lds, int row0, int ks, int lane, rp_frag (&out)[rp_type<DT>::NP]) {
+  using G = rp_geo<DT, DP>;
+#pragma unroll
+  for (int p = 0; p < G::NP; ++p) out[p] = *reinterpret_cast<const rp_frag*>(lds + p * G::PLANE + (row0 + (lane & 31)) * G::PITCH + (2 * ks + (lane >> 5)) * 16);
+}
+// A operand from an LDS tile, rows along the tile's columns (channels 32 ct ..), k-slots = tile rows row0 + 8 (j >> 2) + 4 hh + (j & 3).
+// ds_read_b64_tr_b16: in each group of 16 lanes, lane 4 e + q addresses four channels of row e, lane i receives four rows of channel i.
+template <int DT, int DP>
+__device__ __forceinline__ void rp_cols(const char* lds, int row0, int ct, int lane, rp_frag (&out)[rp_type<DT>::NP]) {
+  using G = rp_geo<DT, DP>;
+  const int off = (row0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * G::PITCH + (32 * ct + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+#pragma unroll
+  for (int p = 0; p < G::NP; ++p) {
+    const char* q = lds + p * G::PLANE + off;
+    const rp_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) rp_s16x4*)(q));
+    const rp_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) rp_s16x4*)(q + 8 * G::PITCH));
+    out[p] = rp_s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  }
+}
+
+struct rp_scales { int eq, ek, ev, ed, es; };
+
+// max of a tensor's partial maxima, by every thread of the workgroup (n <= RP_NBOUND; an absent vector counts as 0)
+__device__ __forceinline__ float rp_bound(const float* part, int n, float* red) {
+  float v = 0.f;
+  if (part && (int)threadIdx.x < n) v = part[threadIdx.x];
+  v = ofb_wave_max(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// the head's bias by difference, times log2 e, padded by RP_PAD copies of its ends
+__device__ __forceinline__ void rp_bias_vector(const ofb_relpos_args& a, int head, float* w) {
+  for (int i = threadIdx.x; i < a.width + 2 * RP_PAD; i += RP_THREADS) {
+    const int c = min(max(i - RP_PAD, 0), a.width - 1);
+    const float t = a.table[(int64_t)a.lut[c] * a.H + head], x = t * 1.44269504088896340736f;
+    w[i] = fabsf(t) < INFINITY ? fminf(fmaxf(x, -3.402823466e38f), 3.402823466e38f) : x;      // (a finite bias stays one: the type's lowest value as a mask)
+  }
+}
+__device__ __forceinline__ int rp_keys_of(const ofb_relpos_args& a, int b) {
+  const int n = a.key_lens ? a.key_lens[b] : a.Nk;
+  return min(max(n, 0), a.Nk);
+}
+
+__device__ __forceinline__ int rp_idx(int diff, int width) { return min(max(diff, 0), width - 1) + RP_PAD; }
+
+// register r of an accumulator <-> row of the 32 x 32 tile
+__device__ __forceinline__ int rp_row(int r, int hh) { return 8 * (r >> 2) + 4 * hh + (r & 3); }
+
+// the biases of the four pairs whose differences are d0, d0 + step, ... (step +1 or -1): one clamp, one 16-byte read
+template <int STEP>
+__device__ __forceinline__ void rp_bias4(const float* w, int d0, int width, float (&out)[4]) {
+  if constexpr (STEP > 0) {
+    const float* p = w + RP_PAD + min(max(d0, -RP_PAD), width);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = p[j];
+  } else {
+    const float* p = w + RP_PAD + min(max(d0 - 3, -RP_PAD), width);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = p[3 - j];
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// forward
+// ------------------------------------------------------------------------------------------------------------------
+// A workgroup owns 128 queries of one head (a wave 32 of them, query on the lane), keys stream through two LDS stages.  S^T = K Q^T has
+// keys along the registers, so the softmax of a row is register-local but for one exchange between lane halves, and P^T is the B operand of
+// O^T = V^T P^T as it stands.
+template <int DT, int DP, bool SPLIT>
+__global__ __launch_bounds__(RP_THREADS) void relpos_fwd_kernel(ofb_relpos_args a) {
+  using G = rp_geo<DT, DP>;
+  constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ float red[4];
+  float* w = reinterpret_cast<float*>(smem);
+  int* pk = reinterpret_cast<int*>(smem + ((a.width + 2 * RP_PAD + 3) & ~3) * 4);
+  char* tiles = reinterpret_cast<char*>(pk + 2 * KB);
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, hh = lane >> 5;
+  const int nqt = (a.Nq + RP_TILE - 1) / RP_TILE;
+  const int id = ofb_xcd_remap(blockIdx.x, gridDim.x);
+  const int qt = id % nqt, bh = id / nqt, head = bh % a.H, b = bh / a.H;
+  const char* qp = (const char*)a.q + (b * a.q_sb + head * a.q_sh) * ES;
+  const char* kp = (const char*)a.k + (b * a.k_sb + head * a.k_sh) * ES;
+  const char* vp = (const char*)a.v + (b * a.v_sb + head * a.v_sh) * ES;
+
+  int kend = rp_keys_of(a, b);
+  const int q_last = min(a.Nq, (qt + 1) * RP_TILE) - 1;
+  if (a.causal) kend = min(kend, max(0, q_last + a.q_offset + 1));
+  int kb0 = 0, kb1 = (kend + KB - 1) / KB;
+  if constexpr (SPLIT) {
+    const int per = ((a.Nk + KB - 1) / KB + (int)gridDim.y - 1) / (int)gridDim.y;
+    kb0 = min(kb1, per * (int)blockIdx.y);
+    kb1 = min(kb1, kb0 + per);
+  }
+
+  rp_stage<DT, DP> ks_, vs_;
+  int pk_next = 0;
+  auto fetch = [&](int kb) {
+    ks_.load(kp, a.k_st * ES, kb * KB, kend, a.d);
+    vs_.load(vp, a.v_st * ES, kb * KB, kend, a.d);
+    if (a.pos_k && threadIdx.x < KB) { const int j = kb * KB + threadIdx.x; pk_next = j < kend ? a.pos_k[j] : 0; }
+  };
+  if (kb0 < kb1) fetch(kb0);
+  rp_bias_vector(a, head, w);
+  float hq = 1.f, hk = 1.f, hv = 1.f, c_s = a.scale * 1.44269504088896340736f, c_o = 1.f;
+  if constexpr (DT == RP_F32) {
+    const int eq = ofb_h_exp(rp_bound(a.bound_q, a.n_bound, red)), ek = ofb_h_exp(rp_bound(a.bound_k, a.n_bound, red)),
+              ev = ofb_h_exp(rp_bound(a.bound_v, a.n_bound, red));
+    hq = ofb_h_pow2(eq); hk = ofb_h_pow2(ek); hv = ofb_h_pow2(ev);
+    c_s = c_s * ofb_h_pow2(-eq) * ofb_h_pow2(-ek);
+    c_o = ofb_h_pow2(-ev);
+  }
+  if constexpr (DT != RP_BF16) c_o *= ofb_h_pow2(-RP_PE);
+  const float p_sc = DT == RP_BF16 ? 1.f : ofb_h_pow2(RP_PE);
+
+  const int q0 = qt * RP_TILE + wv * 32, qi = q0 + (lane & 31);
+  const bool active = q0 < a.Nq, qok = qi < a.Nq;
+  const int pq = a.pos_q ? (qok ? a.pos_q[qi] : 0) : qi + a.q_offset;
+  const int seen = a.causal ? min(kend, max(0, qi + a.q_offset + 1)) : kend;      // this query sees keys 0 .. seen - 1
+  rp_frag qf[DP / 16][NP];
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const int ch = 16 * s + 8 * hh;
+    rp_chunk<DT> c = rp_zero_chunk<DT>();
+    if (qok && ch < a.d) c = rp_load_chunk<DT>(qp + (int64_t)qi * a.q_st * ES + ch * ES);
+    rp_planes<DT>(c, hq, qf[s]);
+  }
+  f32x16 O[DP / 32];
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t) O[t] = rp_zero16();
+  float m = -INFINITY, l = 0.f;
+
+  auto commit = [&](int buf) {
+    ks_.store(tiles + buf * G::STAGE, hk);
+    vs_.store(tiles + buf * G::STAGE + G::TENSOR, hv);
+    if (a.pos_k && threadIdx.x < KB) pk[buf * KB + threadIdx.x] = pk_next;
+  };
+  if (kb0 < kb1) commit(0);
+  __syncthreads();
+  const int lo = a.lo, width = a.width, hi = lo + width - 1;
+  for (int kb = kb0; kb < kb1; ++kb) {
+    const int buf = (kb - kb0) & 1;
+    const char* kt_ = tiles + buf * G::STAGE;
+    const char* vt_ = kt_ + G::TENSOR;
+    if (kb + 1 < kb1) fetch(kb + 1);
+    const int j0 = kb * KB;
+    if (active && (!a.causal || j0 <= q0 + 31 + a.q_offset)) {
+      f32x16 S[KB / 32];
+#pragma unroll
+      for (int t = 0; t < KB / 32; ++t) {
+        S[t] = rp_zero16();
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+          rp_frag kf[NP];
+          rp_rows<DT, DP>(kt_, 32 * t, s, lane, kf);
+          S[t] = rp_mm<DT, NP>(kf, qf[s], S[t]);
+        }
+      }
+      // scores in log2 units, with the bias
+      if (a.pos_k) {
+#pragma unroll
+        for (int t = 0; t < KB / 32; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; r += 4) {
+            const int4 pj = *reinterpret_cast<const int4*>(&pk[buf * KB + 32 * t + rp_row(r, hh)]);
+            S[t][r] = fmaf(S[t][r], c_s, w[rp_idx(pj.x - pq - lo, width)]);
+            S[t][r + 1] = fmaf(S[t][r + 1], c_s, w[rp_idx(pj.y - pq - lo, width)]);
+            S[t][r + 2] = fmaf(S[t][r + 2], c_s, w[rp_idx(pj.z - pq - lo, width)]);
+            S[t][r + 3] = fmaf(S[t][r + 3], c_s, w[rp_idx(pj.w - pq - lo, width)]);
+          }
+      } else {
+        const int dmax = j0 + KB - 1 - q0 - a.q_offset, dmin = j0 - (q0 + 31) - a.q_offset;
+        if (dmax <= lo || dmin >= hi) {                        // the whole tile lies beyond the first or the last difference
+          const float wc = w[RP_PAD + (dmax <= lo ? 0 : width - 1)];
+#pragma unroll
+          for (int t = 0; t < KB / 32; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[t][r] = fmaf(S[t][r], c_s, wc);
+        } else {
+#pragma unroll
+          for (int t = 0; t < KB / 32; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+              float w4[4];
+              rp_bias4<1>(w, j0 + 32 * t + rp_row(r, hh) - pq - lo, width, w4);
+#pragma unroll
+              for (int u = 0; u < 4; ++u) S[t][r + u] = fmaf(S[t][r + u], c_s, w4[u]);
+            }
+        }
+      }
+      const bool whole = j0 + KB <= kend && (!a.causal || j0 + KB - 1 <= q0 + a.q_offset);
+      if (!whole) {
+#pragma unroll
+        for (int t = 0; t < KB / 32; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (j0 + 32 * t + rp_row(r, hh) >= seen) S[t][r] = -INFINITY;
+      }
+      float mb = S[0][0];
+#pragma unroll
+      for (int t = 0; t < KB / 32; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mb = fmaxf(mb, S[t][r]);
+      OFB_XOR_STEP(mb, fmaxf, 32)
+      const float m_new = fmaxf(m, mb);
+      if (__any(m_new > m)) {                                  // the running maximum moves rarely after the first tiles
+        const float alpha = m_new > -INFINITY ? __builtin_amdgcn_exp2f(m - m_new) : 1.f;
+        l *= alpha;
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t) O[t] *= alpha;
+        m = m_new;
+      }
+      const float mu = m > -INFINITY ? m : 0.f;                // a row that has seen nothing yet: exp2(-inf - 0) = 0
+#pragma unroll
+      for (int t = 0; t < KB / 32; ++t) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          float p8[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float p = __builtin_amdgcn_exp2f(S[t][8 * s + j] - mu);
+            l += p;
+            p8[j] = p * p_sc;
+          }
+          rp_frag pf[NP];
+          rp_pack8<DT>(p8, pf);
+#pragma unroll
+          for (int ct = 0; ct < DP / 32; ++ct) {
+            rp_frag vf[NP];
+            rp_cols<DT, DP>(vt_, 32 * t + 16 * s, ct, lane, vf);
+            O[ct] = rp_mm<DT, NP>(vf, pf, O[ct]);
+          }
+        }
+      }
+    }
+    if (kb + 1 < kb1) commit(buf ^ 1);
+    __syncthreads();
+  }
+  OFB_XOR_STEP(l, ofb_add_, 32)
+  if (!qok) return;
+  if constexpr (SPLIT) {                                       // partial sums in units of exp2(m), joined by relpos_join_kernel
+    const int64_t row = ((int64_t)blockIdx.y * a.B * a.H + bh) * a.Nq + qi;
+    if (hh == 0) { a.split_ml[2 * row] = m; a.split_ml[2 * row + 1] = l; }
+#pragma unroll
+    for (int ct = 0; ct < DP / 32; ++ct)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int ch = 32 * ct + rp_row(r, hh);
+        if (ch < a.d) *reinterpret_cast<f32x4*>(a.split_o + row * a.d + ch) = f32x4{O[ct][r] * c_o, O[ct][r + 1] * c_o, O[ct][r + 2] * c_o, O[ct][r + 3] * c_o};
+      }
+  } else {
+    const float linv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);           // (a NaN stays one)
+    if (a.stats && hh == 0) {
+      float* st = a.stats + 2 * ((int64_t)bh * a.Nq + qi);
+      st[0] = m > -INFINITY ? m : 0.f;
+      st[1] = linv;
+    }
+    const float f = linv * c_o;
+    char* op = (char*)a.out + (b * a.o_sb + qi * a.o_st + head * a.o_sh) * ES;
+    float* o32 = a.out32 ? a.out32 + (((int64_t)b * a.Nq + qi) * a.H + head) * a.d : nullptr;
+#pragma unroll
+    for (int ct = 0; ct < DP / 32; ++ct)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int ch = 32 * ct + rp_row(r, hh);
+        if (ch < a.d) {
+          const float x0 = O[ct][r] * f, x1 = O[ct][r + 1] * f, x2 = O[ct][r + 2] * f, x3 = O[ct][r + 3] * f;
+          rp_store4<DT>(op + ch * ES, x0, x1, x2, x3);
+          if (o32) *reinterpret_cast<f32x4*>(o32 + ch) = f32x4{x0, x1, x2, x3};
+        }
+      }
+  }
+}
+
+// joins the key ranges of a split forward: one wave per row, lanes along the channels
+template <int DT>
+__global__ __launch_bounds__(RP_THREADS) void relpos_join_kernel(ofb_relpos_args a, int splits) {
+  constexpr int ES = rp_type<DT>::ES;
+  const int lane = threadIdx.x & 63;
+  const int64_t rows = (int64_t)a.B * a.H * a.Nq, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int qi = (int)(row % a.Nq);
+  const int64_t bh = row / a.Nq;
+  const int head = (int)(bh % a.H);
+  const int64_t b = bh / a.H;
+  float m = -INFINITY, l = 0.f;
+  for (int s = 0; s < splits; ++s) m = fmaxf(m, a.split_ml[2 * (s * rows + row)]);
+  const float mu = m > -INFINITY ? m : 0.f;
+  for (int s = 0; s < splits; ++s) l += a.split_ml[2 * (s * rows + row) + 1] * __builtin_amdgcn_exp2f(a.split_ml[2 * (s * rows + row)] - mu);
+  const float linv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  if (a.stats && lane == 0) { a.stats[2 * row] = mu; a.stats[2 * row + 1] = linv; }
+  for (int ch = lane * 4; ch < a.d; ch += 256) {
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s)
+      o += *reinterpret_cast<const f32x4*>(a.split_o + (s * rows + row) * a.d + ch) * __builtin_amdgcn_exp2f(a.split_ml[2 * (s * rows + row)] - mu);
+    o *= linv;
+    rp_store4<DT>((char*)a.out + (b * a.o_sb + qi * a.o_st + head * a.o_sh + ch) * ES, o[0], o[1], o[2], o[3]);
+    if (a.out32) *reinterpret_cast<f32x4*>(a.out32 + ((b * a.Nq + qi) * a.H + head) * a.d + ch) = o;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// backward
+// ------------------------------------------------------------------------------------------------------------------
+template <int DT>
+__device__ __forceinline__ rp_scales rp_all_scales(const ofb_relpos_args& a, float* red) {
+  rp_scales e = {0, 0, 0, 0, 0};
+  if constexpr (DT != RP_BF16) {
+    const float bv = rp_bound(a.bound_v, a.n_bound, red), bd = rp_bound(a.bound_do, a.n_bound_do, red);
+    e.es = ofb_h_exp(2.f * a.d * bv * bd);                     // |dS| <= P (|dP| + |D|) <= 2 d max|dO| max|V|
+    if constexpr (DT == RP_F32) {
+      e.eq = ofb_h_exp(rp_bound(a.bound_q, a.n_bound, red));
+      e.ek = ofb_h_exp(rp_bound(a.bound_k, a.n_bound, red));
+      e.ev = ofb_h_exp(bv);
+      e.ed = ofb_h_exp(bd);
+    }
+  }
+  return e;
+}
+
+// dQ, D, and the part of the table's gradient that lies beyond the last differences.  The forward's layout: 128 queries a workgroup, the
+// query on the lane; dS^T is the B operand of dQ^T = K^T dS^T from its registers.
+template <int DT, int DP>
+__global__ __launch_bounds__(RP_THREADS) void relpos_dq_kernel(ofb_relpos_args a) {
+  using G = rp_geo<DT, DP>;
+  constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ float red[4];
+  float* w = reinterpret_cast<float*>(smem);
+  int* pk = reinterpret_cast<int*>(smem + ((a.width + 2 * RP_PAD + 3) & ~3) * 4);
+  char* tiles = reinterpret_cast<char*>(pk + 2 * KB);
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, hh = lane >> 5;
+  const int nqt = (a.Nq + RP_TILE - 1) / RP_TILE;
+  const int id = ofb_xcd_remap(blockIdx.x, gridDim.x);
+  const int qt = id % nqt, bh = id / nqt, head = bh % a.H, b = bh / a.H;
+  const char* qp = (const char*)a.q + (b * a.q_sb + head * a.q_sh) * ES;
+  const char* kp = (const char*)a.k + (b * a.k_sb + head * a.k_sh) * ES;
+  const char* vp = (const char*)a.v + (b * a.v_sb + head * a.v_sh) * ES;
+  const char* dp = (const char*)a.dout + (b * a.do_sb + head * a.do_sh) * ES;
+  int kend = rp_keys_of(a, b);
+  const int q_last = min(a.Nq, (qt + 1) * RP_TILE) - 1;
+  if (a.causal) kend = min(kend, max(0, q_last + a.q_offset + 1));
+  const int kb1 = (kend + KB - 1) / KB;
+  rp_stage<DT, DP> ks_, vs_;
+  int pk_next = 0;
+  auto fetch = [&](int kb) {
+    ks_.load(kp, a.k_st * ES, kb * KB, kend, a.d);
+    vs_.load(vp, a.v_st * ES, kb * KB, kend, a.d);
+    if (a.pos_k && threadIdx.x < KB) { const int j = kb * KB + threadIdx.x; pk_next = j < kend ? a.pos_k[j] : 0; }
+  };
+  if (kb1 > 0) fetch(0);
+  rp_bias_vector(a, head, w);
+  const rp_scales e = rp_all_scales<DT>(a, red);
+  const float hq = ofb_h_pow2(e.eq), hk = ofb_h_pow2(e.ek), hv = ofb_h_pow2(e.ev), hd = ofb_h_pow2(e.ed), hs = ofb_h_pow2(e.es);
+  const float c_s = a.scale * 1.44269504088896340736f * ofb_h_pow2(-e.eq) * ofb_h_pow2(-e.ek);
+  const float c_dp = ofb_h_pow2(-e.ed) * ofb_h_pow2(-e.ev);
+  const float c_dq = a.scale * ofb_h_pow2(-e.es) * ofb_h_pow2(-e.ek);
+
+  const int q0 = qt * RP_TILE + wv * 32, qi = q0 + (lane & 31);
+  const bool active = q0 < a.Nq, qok = qi < a.Nq;
+  const int pq = a.pos_q ? (qok ? a.pos_q[qi] : 0) : qi + a.q_offset;
+  const int seen = a.causal ? min(kend, max(0, qi + a.q_offset + 1)) : kend;
+  rp_frag qf[DP / 16][NP], df[DP / 16][NP];
+  float D = 0.f, m = 0.f, linv = 0.f;
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const int ch = 16 * s + 8 * hh;
+    rp_chunk<DT> c = rp_zero_chunk<DT>(), g = rp_zero_chunk<DT>();
+    if (qok && ch < a.d) {
+      c = rp_load_chunk<DT>(qp + (int64_t)qi * a.q_st * ES + ch * ES);
+      g = rp_load_chunk<DT>(dp + (int64_t)qi * a.do_st * ES + ch * ES);
+      const float* o32 = a.out32 + (((int64_t)b * a.Nq + qi) * a.H + head) * a.d + ch;
+      const f32x4 oa = *reinterpret_cast<const f32x4*>(o32), ob = *reinterpret_cast<const f32x4*>(o32 + 4);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) D = fmaf(rp_chunk_at<DT>(g, j), j < 4 ? oa[j & 3] : ob[j & 3], D);
+    }
+    rp_planes<DT>(c, hq, qf[s]);
+    rp_planes<DT>(g, hd, df[s]);
+  }
+  OFB_XOR_STEP(D, ofb_add_, 32)
+  if (qok) {
+    const int64_t row = (int64_t)bh * a.Nq + qi;
+    m = a.stats[2 * row];
+    linv = a.stats[2 * row + 1];
+  }
+  f32x16 dQ[DP / 32];
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t) dQ[t] = rp_zero16();
+  float sat_lo = 0.f, sat_hi = 0.f, pat_lo = 0.f, pat_hi = 0.f, left = 0.f;
+  auto commit = [&](int buf) {
+    ks_.store(tiles + buf * G::STAGE, hk);
+    vs_.store(tiles + buf * G::STAGE + G::TENSOR, hv);
+    if (a.pos_k && threadIdx.x < KB) pk[buf * KB + threadIdx.x] = pk_next;
+  };
+  if (kb1 > 0) commit(0);
+  __syncthreads();
+  const int lo = a.lo, width = a.width, hi = lo + width - 1;
+  for (int kb = 0; kb < kb1; ++kb) {
+    const int buf = kb & 1;
+    const char* kt_ = tiles + buf * G::STAGE;
+    const char* vt_ = kt_ + G::TENSOR;
+    if (kb + 1 < kb1) fetch(kb + 1);
+#pragma unroll
+    for (int t = 0; t < KB / 32; ++t) {
+      const int j0 = kb * KB + 32 * t;
+      if (!active || j0 >= kend || (a.causal && j0 > q0 + 31 + a.q_offset)) continue;
+      f32x16 S = rp_zero16(), dP = rp_zero16();
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) {
+        rp_frag kf[NP], vf[NP];
+        rp_rows<DT, DP>(kt_, 32 * t, s, lane, kf);
+        rp_rows<DT, DP>(vt_, 32 * t, s, lane, vf);
+        S = rp_mm<DT, NP>(kf, qf[s], S);
+        dP = rp_mm<DT, NP>(vf, df[s], dP);
+      }
+      const bool whole = j0 + 32 <= kend && (!a.causal || j0 + 31 <= q0 + a.q_offset);
+      const int dmax = j0 + 31 - q0 - a.q_offset, dmin = j0 - (q0 + 31) - a.q_offset;
+      const bool far = !a.pos_k && (dmax <= lo || dmin >= hi);
+      const float wc = far ? w[RP_PAD + (dmax <= lo ? 0 : width - 1)] : 0.f;
+      float ds[16], ps[16];
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int jr = j0 + rp_row(r, hh);
+        float w4[4];
+        if (far) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) w4[u] = wc;
+        } else if (a.pos_k) {
+          const int4 pj = *reinterpret_cast<const int4*>(&pk[buf * KB + 32 * t + rp_row(r, hh)]);
+          w4[0] = w[rp_idx(pj.x - pq - lo, width)];
+          w4[1] = w[rp_idx(pj.y - pq - lo, width)];
+          w4[2] = w[rp_idx(pj.z - pq - lo, width)];
+          w4[3] = w[rp_idx(pj.w - pq - lo, width)];
+        } else {
+          rp_bias4<1>(w, jr - pq - lo, width, w4);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          float p = __builtin_amdgcn_exp2f(fmaf(S[r + u], c_s, w4[u]) - m) * linv;
+          if (!whole && jr + u >= seen) p = 0.f;
+          float x = p * (fmaf(dP[r + u], c_dp, -D));
+          if (!whole && jr + u >= seen) x = 0.f;               // (0 times a non-finite dP)
+          ds[r + u] = x;
+          ps[r + u] = p;
+        }
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum += ds[r];
+      left += sum;
+      if (!a.pos_k && a.sat) {
+        if (far) {
+          float psum = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) psum += ps[r];
+          if (dmax <= lo) { sat_lo += sum; pat_lo += psum; } else { sat_hi += sum; pat_hi += psum; }
+        } else if (dmin <= lo || dmax >= hi) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int diff = j0 + rp_row(r, hh) - pq;
+            const bool below = diff <= lo, above = diff >= hi && diff > lo;
+            sat_lo += below ? ds[r] : 0.f;
+            pat_lo += below ? ps[r] : 0.f;
+            sat_hi += above ? ds[r] : 0.f;
+            pat_hi += above ? ps[r] : 0.f;
+          }
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        float x8[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x8[j] = ds[8 * s + j] * hs;
+        rp_frag xf[NP];
+        rp_pack8<DT>(x8, xf);
+#pragma unroll
+        for (int ct = 0; ct < DP / 32; ++ct) {
+          rp_frag kf[NP];
+          rp_cols<DT, DP>(kt_, 32 * t + 16 * s, ct, lane, kf);
+          dQ[ct] = rp_mm<DT, NP>(kf, xf, dQ[ct]);
+        }
+      }
+    }
+    if (kb + 1 < kb1) commit(buf ^ 1);
+    __syncthreads();
+  }
+  // D came from an output whose P was rounded for the product.  A row of dS sums to zero, so what this row's sum is off by is D's error: the
+  // kernels that follow read D without it, and the sums above lose it times their share of P.  (The table's gradient is f32 and sums whole rows'
+  // parts, where an error that a row's terms share does not average out: without this it was 1e-3 off for bf16.)
+  OFB_XOR_STEP(left, ofb_add_, 32)
+  if (qok && hh == 0) a.delta[(int64_t)bh * a.Nq + qi] = D + left;
+  sat_lo -= left * pat_lo;
+  sat_hi -= left * pat_hi;
+  if (a.sat) {
+    if (!qok) sat_lo = sat_hi = 0.f;                           // (P of a row behind the last query is 0 anyway)
+    sat_lo = ofb_wave_sum(sat_lo);
+    sat_hi = ofb_wave_sum(sat_hi);
+    if (lane == 0) {
+      const int64_t n = (int64_t)a.B * nqt * 4, at = ((int64_t)b * nqt + qt) * 4 + wv;
+      a.sat[(2 * (int64_t)head) * n + at] = sat_lo;
+      a.sat[(2 * (int64_t)head + 1) * n + at] = sat_hi;
+    }
+  }
+  if (!qok) return;
+  char* op = (char*)a.dq + (b * a.dq_sb + qi * a.dq_st + head * a.dq_sh) * ES;
+#pragma unroll
+  for (int ct = 0; ct < DP / 32; ++ct)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int ch = 32 * ct + rp_row(r, hh);
+      if (ch < a.d) rp_store4<DT>(op + ch * ES, dQ[ct][r] * c_dq, dQ[ct][r + 1] * c_dq, dQ[ct][r + 2] * c_dq, dQ[ct][r + 3] * c_dq);
+    }
+}
+
+// a query tile's row statistics in LDS: max, 1 / sum, D, position - each a vector of KB
+template <int KB>
+__device__ __forceinline__ void rp_row_stats(const ofb_relpos_args& a, int64_t bh, int row0, f32x4& v, int& pos) {
+  const int i = row0 + threadIdx.x;
+  v = f32x4{0.f, 0.f, 0.f, 0.f};
+  pos = 0;
+  if (threadIdx.x < KB && i < a.Nq) {
+    const int64_t row = bh * a.Nq + i;
+    v[0] = a.stats[2 * row];
+    v[1] = a.stats[2 * row + 1];
+    v[2] = a.delta[row];
+    pos = a.pos_q ? a.pos_q[i] : i + a.q_offset;
+  }
+}
+
+// P and dS of a 32 x 32 tile, rows = queries i0 .. (LDS tiles qt_ and dt_ at row tr), the wave's key on the lane
+template <int DT, int DP>
+__device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char* qt_, const char* dt_, int tr, const rp_frag (&kf)[DP / 16][rp_type<DT>::NP],
+                                           const rp_frag (&vf)[DP / 16][rp_type<DT>::NP], const float* st, const int* ps, const float* w, int i0, int j0,
+                                           int kj, int pkj, bool kok, float c_s, float c_dp, float (&P)[16], float (&dS)[16]) {
+  using G = rp_geo<DT, DP>;
+  constexpr int NP = G::NP, KB = G::KB;
+  const int lane = threadIdx.x & 63, hh = lane >> 5, lo = a.lo, width = a.width, hi = lo + width - 1;
+  f32x16 S = rp_zero16(), dP = rp_zero16();
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    rp_frag qa[NP], da[NP];
+    rp_rows<DT, DP>(qt_, tr, s, lane, qa);
+    rp_rows<DT, DP>(dt_, tr, s, lane, da);
+    S = rp_mm<DT, NP>(qa, kf[s], S);
+    dP = rp_mm<DT, NP>(da, vf[s], dP);
+  }
+  const int dmax = j0 + 31 - i0 - a.q_offset, dmin = j0 - (i0 + 31) - a.q_offset;
+  const bool far = !a.pos_q && (dmax <= lo || dmin >= hi);
+  const float wc = far ? w[RP_PAD + (dmax <= lo ? 0 : width - 1)] : 0.f;
+  const bool cut = a.causal && j0 + 31 > i0 + a.q_offset;
+#pragma unroll
+  for (int r = 0; r < 16; r += 4) {
+    const int rr = rp_row(r, hh);
+    const f32x4 m4 = *reinterpret_cast<const f32x4*>(&st[tr + rr]), l4 = *reinterpret_cast<const f32x4*>(&st[KB + tr + rr]),
+                d4 = *reinterpret_cast<const f32x4*>(&st[2 * KB + tr + rr]);
+    float w4[4];
+    if (far) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) w4[u] = wc;
+    } else if (a.pos_q) {
+      const int4 pi = *reinterpret_cast<const int4*>(&ps[tr + rr]);
+      w4[0] = w[rp_idx(pkj - pi.x - lo, width)];
+      w4[1] = w[rp_idx(pkj - pi.y - lo, width)];
+      w4[2] = w[rp_idx(pkj - pi.z - lo, width)];
+      w4[3] = w[rp_idx(pkj - pi.w - lo, width)];
+    } else {
+      rp_bias4<-1>(w, kj - (i0 + rr + a.q_offset) - lo, width, w4);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float p = __builtin_amdgcn_exp2f(fmaf(S[r + u], c_s, w4[u]) - m4[u]) * l4[u];
+      float x = p * fmaf(dP[r + u], c_dp, -d4[u]);
+      if (!kok || (cut && kj > i0 + rr + u + a.q_offset)) p = x = 0.f;
+      P[r + u] = p;
+      dS[r + u] = x;
+    }
+  }
+}
+
+// dK and dV: a workgroup owns 128 keys of one head (a wave 32, key on the lane, K and V in registers), queries stream through LDS.
+// S = Q K^T and dP = dO V^T have queries along the registers: P and dS are the B operands of dV^T = dO^T P and dK^T = Q^T dS.
+template <int DT, int DP>
+__global__ __launch_bounds__(RP_THREADS) void relpos_dkv_kernel(ofb_relpos_args a) {
+  using G = rp_geo<DT, DP>;
+  constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ float red[4];
+  float* w = reinterpret_cast<float*>(smem);
+  float* st = reinterpret_cast<float*>(smem + ((a.width + 2 * RP_PAD + 3) & ~3) * 4);      // [2][3][KB]
+  int* ps = reinterpret_cast<int*>(st + 6 * KB);                                            // [2][KB]
+  char* tiles = reinterpret_cast<char*>(ps + 2 * KB);
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, hh = lane >> 5;
+  const int nkt = (a.Nk + RP_TILE - 1) / RP_TILE;
+  const int id = ofb_xcd_remap(blockIdx.x, gridDim.x);
+  const int kt = id % nkt, bh = id / nkt, head = bh % a.H, b = bh / a.H;
+  const char* qp = (const char*)a.q + (b * a.q_sb + head * a.q_sh) * ES;
+  const char* kp = (const char*)a.k + (b * a.k_sb + head * a.k_sh) * ES;
+  const char* vp = (const char*)a.v + (b * a.v_sb + head * a.v_sh) * ES;
+  const char* dp = (const char*)a.dout + (b * a.do_sb + head * a.do_sh) * ES;
+  const int kend = rp_keys_of(a, b), j_first = kt * RP_TILE;
+  int qb0 = 0, qb1 = (a.Nq + KB - 1) / KB;
+  if (a.causal) qb0 = min(qb1, max(0, j_first - a.q_offset) / KB);
+  if (j_first >= kend) qb0 = qb1;                              // nobody sees these keys: their gradients are zeros
+  rp_stage<DT, DP> qs_, ds_;
+  f32x4 st_next;
+  int ps_next;
+  auto fetch = [&](int qb) {
+    qs_.load(qp, a.q_st * ES, qb * KB, a.Nq, a.d);
+    ds_.load(dp, a.do_st * ES, qb * KB, a.Nq, a.d);
+    rp_row_stats<KB>(a, bh, qb * KB, st_next, ps_next);
+  };
+  if (qb0 < qb1) fetch(qb0);
+  rp_bias_vector(a, head, w);
+  const rp_scales e = rp_all_scales<DT>(a, red);
+  const float hq = ofb_h_pow2(e.eq), hk = ofb_h_pow2(e.ek), hv = ofb_h_pow2(e.ev), hd = ofb_h_pow2(e.ed), hs = ofb_h_pow2(e.es);
+  const float c_s = a.scale * 1.44269504088896340736f * ofb_h_pow2(-e.eq) * ofb_h_pow2(-e.ek);
+  const float c_dp = ofb_h_pow2(-e.ed) * ofb_h_pow2(-e.ev);
+  const float c_dk = a.scale * ofb_h_pow2(-e.es) * ofb_h_pow2(-e.eq);
+  const float p_sc = DT == RP_BF16 ? 1.f : ofb_h_pow2(RP_PE);
+  const float c_dv = DT == RP_BF16 ? 1.f : ofb_h_pow2(-RP_PE) * ofb_h_pow2(-e.ed);
+
+  const int j0 = j_first + wv * 32, kj = j0 + (lane & 31);
+  const bool active = j0 < kend, kok = kj < kend;
+  const int pkj = a.pos_k ? (kok ? a.pos_k[kj] : 0) : kj;
+  rp_frag kf[DP / 16][NP], vf[DP / 16][NP];
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const int ch = 16 * s + 8 * hh;
+    rp_chunk<DT> c = rp_zero_chunk<DT>(), g = rp_zero_chunk<DT>();
+    if (kok && ch < a.d) {
+      c = rp_load_chunk<DT>(kp + (int64_t)kj * a.k_st * ES + ch * ES);
+      g = rp_load_chunk<DT>(vp + (int64_t)kj * a.v_st * ES + ch * ES);
+    }
+    rp_planes<DT>(c, hk, kf[s]);
+    rp_planes<DT>(g, hv, vf[s]);
+  }
+  f32x16 dK[DP / 32], dV[DP / 32];
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t) dK[t] = dV[t] = rp_zero16();
+  auto commit = [&](int buf) {
+    qs_.store(tiles + buf * G::STAGE, hq);
+    ds_.store(tiles + buf * G::STAGE + G::TENSOR, hd);
+    if (threadIdx.x < KB) {
+#pragma unroll
+      for (int u = 0; u < 3; ++u) st[(buf * 3 + u) * KB + threadIdx.x] = st_next[u];
+      ps[buf * KB + threadIdx.x] = ps_next;
+    }
+  };
+  if (qb0 < qb1) commit(0);
+  __syncthreads();
+  for (int qb = qb0; qb < qb1; ++qb) {
+    const int buf = (qb - qb0) & 1;
+    const char* qt_ = tiles + buf * G::STAGE;
+    const char* dt_ = qt_ + G::TENSOR;
+    if (qb + 1 < qb1) fetch(qb + 1);
+#pragma unroll
+    for (int t = 0; t < KB / 32; ++t) {
+      const int i0 = qb * KB + 32 * t;
+      if (!active || i0 >= a.Nq || (a.causal && j0 > i0 + 31 + a.q_offset)) continue;
+      float P[16], dS[16];
+      rp_tile_ds<DT, DP>(a, qt_, dt_, 32 * t, kf, vf, st + buf * 3 * KB, ps + buf * KB, w, i0, j0, kj, pkj, kok, c_s, c_dp, P, dS);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        float p8[8], x8[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { p8[j] = P[8 * s + j] * p_sc; x8[j] = dS[8 * s + j] * hs; }
+        rp_frag pf[NP], xf[NP];
+        rp_pack8<DT>(p8, pf);
+        rp_pack8<DT>(x8, xf);
+#pragma unroll
+        for (int ct = 0; ct < DP / 32; ++ct) {
+          rp_frag df[NP], qf[NP];
+          rp_cols<DT, DP>(dt_, 32 * t + 16 * s, ct, lane, df);
+          rp_cols<DT, DP>(qt_, 32 * t + 16 * s, ct, lane, qf);
+          dV[ct] = rp_mm<DT, NP>(df, pf, dV[ct]);
+          dK[ct] = rp_mm<DT, NP>(qf, xf, dK[ct]);
+        }
+      }
+    }
+    if (qb + 1 < qb1) commit(buf ^ 1);
+    __syncthreads();
+  }
+  if (kj >= a.Nk) return;
+  char* okp = (char*)a.dk + (b * a.dk_sb + kj * a.dk_st + head * a.dk_sh) * ES;
+  char* ovp = (char*)a.dv + (b * a.dv_sb + kj * a.dv_st + head * a.dv_sh) * ES;
+#pragma unroll
+  for (int ct = 0; ct < DP / 32; ++ct)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int ch = 32 * ct + rp_row(r, hh);
+      if (ch < a.d) {
+        rp_store4<DT>(okp + ch * ES, dK[ct][r] * c_dk, dK[ct][r + 1] * c_dk, dK[ct][r + 2] * c_dk, dK[ct][r + 3] * c_dk);
+        rp_store4<DT>(ovp + ch * ES, dV[ct][r] * c_dv, dV[ct][r + 1] * c_dv, dV[ct][r + 2] * c_dv, dV[ct][r + 3] * c_dv);
+      }
+    }
+}
+
+// The table's gradient by difference.  A workgroup owns one head, one query tile and one part of the batch; for every key tile of 128 it sums
+// dS over its part of the batch in registers (so a pair's bucket is looked up once, not once per sample), then adds the tile to a histogram by
+// difference in LDS: whole numbers of 2^-40 of the tile's largest |dS|, so that the order of the additions does not matter.  Without
+// position arrays only the tiles with differences strictly between the first and the last are visited (relpos_dq_kernel sums the rest).
+template <int DT, int DP>
+__global__ __launch_bounds__(RP_THREADS) void relpos_dbias_kernel(ofb_relpos_args a, int chunks) {
+  using G = rp_geo<DT, DP>;
+  constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ float red[4];
+  const int wpad = (a.width + 2 * RP_PAD + 3) & ~3;
+  float* w = reinterpret_cast<float*>(smem);
+  float* st = w + wpad;                                                                     // [3][KB]
+  int* ps = reinterpret_cast<int*>(st + 3 * KB);                                            // [KB]
+  unsigned long long* hist = reinterpret_cast<unsigned long long*>(ps + KB);                // [wpad]
+  double* acc = reinterpret_cast<double*>(hist + wpad);                                     // [wpad]
+  char* tiles = reinterpret_cast<char*>(acc + wpad);
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, hh = lane >> 5;
+  const int nqt = (a.Nq + KB - 1) / KB;
+  const int chunk = blockIdx.x % chunks, qt = (blockIdx.x / chunks) % nqt, head = blockIdx.x / (chunks * nqt);
+  const int b0 = (int)((int64_t)a.B * chunk / chunks), b1 = (int)((int64_t)a.B * (chunk + 1) / chunks);
+  rp_bias_vector(a, head, w);
+  for (int i = threadIdx.x; i < wpad; i += RP_THREADS) { hist[i] = 0ull; acc[i] = 0.0; }
+  const rp_scales e = rp_all_scales<DT>(a, red);
+  const float hq = ofb_h_pow2(e.eq), hk = ofb_h_pow2(e.ek), hv = ofb_h_pow2(e.ev), hd = ofb_h_pow2(e.ed);
+  const float c_s = a.scale * 1.44269504088896340736f * ofb_h_pow2(-e.eq) * ofb_h_pow2(-e.ek);
+  const float c_dp = ofb_h_pow2(-e.ed) * ofb_h_pow2(-e.ev);
+  const int i_first = qt * KB, i_last = min(a.Nq, i_first + KB) - 1, lo = a.lo, width = a.width, hi = lo + width - 1;
+  int kt0 = 0, kt1 = (a.Nk + RP_TILE - 1) / RP_TILE;
+  if (!a.pos_k) {                                              // keys with lo < j - (i + q_offset) < hi for some query of the tile
+    const int64_t jmin = max((int64_t)0, (int64_t)i_first + a.q_offset + lo + 1), jmax = min((int64_t)a.Nk - 1, (int64_t)i_last + a.q_offset + hi - 1);
+    kt0 = (int)min((int64_t)kt1, jmin / RP_TILE);
+    kt1 = jmax < jmin ? kt0 : (int)(jmax / RP_TILE) + 1;
+  }
+  bool poison = false;
+  for (int kt = kt0; kt < kt1; ++kt) {
+    const int j0 = kt * RP_TILE + wv * 32, kj = j0 + (lane & 31);
+    if (a.causal && kt * RP_TILE > i_last + a.q_offset) break;
+    const int pkj = a.pos_k ? (kj < a.Nk ? a.pos_k[kj] : 0) : kj;
+    float sum[KB / 32][16];
+#pragma unroll
+    for (int t = 0; t < KB / 32; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum[t][r] = 0.f;
+    for (int b = b0; b < b1; ++b) {
+      const int kend = rp_keys_of(a, b);
+      if (kt * RP_TILE >= kend) continue;
+      rp_stage<DT, DP> qs_, ds_;
+      f32x4 st_next;
+      int ps_next;
+      qs_.load((const char*)a.q + (b * a.q_sb + head * a.q_sh) * ES, a.q_st * ES, i_first, a.Nq, a.d);
+      ds_.load((const char*)a.dout + (b * a.do_sb + head * a.do_sh) * ES, a.do_st * ES, i_first, a.Nq, a.d);
+      rp_row_stats<KB>(a, (int64_t)b * a.H + head, i_first, st_next, ps_next);
+      const char* kp = (const char*)a.k + (b * a.k_sb + head * a.k_sh) * ES;
+      const char* vp = (const char*)a.v + (b * a.v_sb + head * a.v_sh) * ES;
+      const bool kok = kj < kend;
+      rp_frag kf[DP / 16][NP], vf[DP / 16][NP];
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) {
+        const int ch = 16 * s + 8 * hh;
+        rp_chunk<DT> c = rp_zero_chunk<DT>(), g = rp_zero_chunk<DT>();
+        if (kok && ch < a.d) {
+          c = rp_load_chunk<DT>(kp + (int64_t)kj * a.k_st * ES + ch * ES);
+          g = rp_load_chunk<DT>(vp + (int64_t)kj * a.v_st * ES + ch * ES);
+        }
+        rp_planes<DT>(c, hk, kf[s]);
+        rp_planes<DT>(g, hv, vf[s]);
+      }
+      __syncthreads();                                         // the tile before has been read
+      qs_.store(tiles, hq);
+      ds_.store(tiles + G::TENSOR, hd);
+      if (threadIdx.x < KB) {
+#pragma unroll
+        for (int u = 0; u < 3; ++u) st[u * KB + threadIdx.x] = st_next[u];
+        ps[threadIdx.x] = ps_next;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < KB / 32; ++t) {
+        const int i0 = i_first + 32 * t;
+        if (j0 >= kend || i0 >= a.Nq || (a.causal && j0 > i0 + 31 + a.q_offset)) continue;
+        float P[16], dS[16];
+        rp_tile_ds<DT, DP>(a, tiles, tiles + G::TENSOR, 32 * t, kf, vf, st, ps, w, i0, j0, kj, pkj, kok, c_s, c_dp, P, dS);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[t][r] += dS[r];
+      }
+    }
+    float mx = 0.f;
+#pragma unroll
+    for (int t = 0; t < KB / 32; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        mx = fmaxf(mx, fabsf(sum[t][r]));
+        poison |= !(fabsf(sum[t][r]) < 3.0e38f);
+      }
+    mx = ofb_wave_max(mx);
+    __syncthreads();
+    if (lane == 0) red[wv] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    if (mx > 0.f && mx < 3.0e38f) {                            // (the same in every thread)
+      int ex;
+      frexpf(mx, &ex);
+      const double up = __builtin_ldexp(1.0, 40 - ex), down = __builtin_ldexp(1.0, ex - 40);
+#pragma unroll
+      for (int t = 0; t < KB / 32; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int i = i_first + 32 * t + rp_row(r, hh);
+          const int diff = pkj - (a.pos_q ? ps[32 * t + rp_row(r, hh)] : i + a.q_offset);
+          const float x = sum[t][r];
+          if (x != 0.f && fabsf(x) < 3.0e38f && (a.pos_k || (diff > lo && diff < hi)))
+            atomicAdd(&hist[min(max(diff - lo, 0), width - 1)], (unsigned long long)__double2ll_rn((double)x * up));
+        }
+      __syncthreads();
+      for (int i = threadIdx.x; i < width; i += RP_THREADS) {
+        acc[i] += (double)(long long)hist[i] * down;
+        hist[i] = 0ull;
+      }
+    }
+  }
+  const bool bad = __syncthreads_or(poison);
+  const int64_t rows = (int64_t)nqt * chunks, at = (int64_t)qt * chunks + chunk;
+  for (int i = threadIdx.x; i < width; i += RP_THREADS) a.partial[((int64_t)head * width + i) * rows + at] = bad ? __builtin_nanf("") : (float)acc[i];
+}
+
+// table gradient: one wave per (bucket, head) adds up the differences of its bucket over all workgroups, in a fixed order and in 64 bits
+__global__ __launch_bounds__(RP_THREADS) void relpos_table_kernel(ofb_relpos_args a, int64_t rows, int64_t nsat) {
+  const int lane = threadIdx.x & 63, id = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (id >= a.n_buckets * a.H) return;
+  const int c = id / a.H, head = id % a.H;
+  double sum = 0.0;
+  for (int e = a.bucket_start[c]; e < a.bucket_start[c + 1]; ++e) {
+    const int i = a.bucket_order[e];
+    if (nsat > 0 && (i == 0 || i == a.width - 1)) {            // (a single difference takes both)
+      for (int side = i == 0 ? 0 : 1; side < (i == a.width - 1 ? 2 : 1); ++side) {
+        const float* p = a.sat + (2 * (int64_t)head + side) * nsat;
+        for (int64_t r = lane; r < nsat; r += 64) sum += (double)p[r];
+      }
+    } else {
+      const float* p = a.partial + ((int64_t)head * a.width + i) * rows;
+      for (int64_t r = lane; r < rows; r += 64) sum += (double)p[r];
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if (lane == 0) a.dtable[(int64_t)c * a.H + head] = (float)sum;
+}
+
+// partial maxima of |x| of up to three tensors (blockIdx.y), over the tokens that can be seen: what lies behind them may hold anything
+template <int DT>
+__global__ __launch_bounds__(RP_THREADS) void relpos_amax_kernel(ofb_relpos_args a, int first) {
+  constexpr int ES = rp_type<DT>::ES;
+  __shared__ float red[4];
+  const int which = first + blockIdx.y;                        // 0 q, 1 k, 2 v, 3 dout
+  const char* x = (const char*)(which == 0 ? a.q : which == 1 ? a.k : which == 2 ? a.v : a.dout);
+  const int64_t sb = which == 0 ? a.q_sb : which == 1 ? a.k_sb : which == 2 ? a.v_sb : a.do_sb;
+  const int64_t st = which == 0 ? a.q_st : which == 1 ? a.k_st : which == 2 ? a.v_st : a.do_st;
+  const int64_t sh = which == 0 ? a.q_sh : which == 1 ? a.k_sh : which == 2 ? a.v_sh : a.do_sh;
+  const bool key = which == 1 || which == 2;
+  const int per = a.H * (a.d / 8);                             // chunks of a token
+  const int tokens = key ? a.Nk : a.Nq;
+  float v = 0.f;
+  const int64_t rows = (int64_t)a.B * tokens;
+  // one token after the other per group of threads: `per` chunks each
+  const int group = min(per, RP_THREADS), groups = RP_THREADS / group, g = threadIdx.x / group, t0 = threadIdx.x % group;
+  if (g < groups) {
+    for (int64_t row = (int64_t)blockIdx.x * groups + g; row < rows; row += (int64_t)gridDim.x * groups) {
+      const int b = (int)(row / tokens), i = (int)(row - (int64_t)b * tokens);
+      int end = rp_keys_of(a, b);
+      if (key) { if (i >= (a.causal ? min(end, max(0, a.Nq + a.q_offset)) : end)) continue; }
+      else if (end == 0 || (a.causal && i + a.q_offset < 0)) continue;       // a query that sees nothing
+      for (int c = t0; c < per; c += group) {
+        const int head = c / (a.d / 8), ch = (c % (a.d / 8)) * 8;
+        const rp_chunk<DT> q = rp_load_chunk<DT>(x + (b * sb + (int64_t)i * st + head * sh + ch) * ES);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v = fmaxf(v, fabsf(rp_chunk_at<DT>(q, j)));
+      }
+    }
+  }
+  v = ofb_wave_max(v);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float* out = (float*)(which == 0 ? a.bound_q : which == 1 ? a.bound_k : which == 2 ? a.bound_v : a.bound_do);
+  if (threadIdx.x == 0) out[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+template <int DT, int DP> int rp_lds(const ofb_relpos_args& a, int kind) {       // 0 forward / dQ, 1 dK dV, 2 table gradient
+  using G = rp_geo<DT, DP>;
+  const int w = ((a.width + 2 * RP_PAD + 3) & ~3) * 4;
+  if (kind == 0) return w + 2 * G::KB * 4 + 2 * G::STAGE;
+  if (kind == 1) return w + 8 * G::KB * 4 + 2 * G::STAGE;
+  return w * 5 + 4 * G::KB * 4 + G::STAGE;
+}
+
+template <typename F> int rp_allow(F* f, int bytes) {
+  return bytes <= 65536 ? 0 : (int)hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+#define RP_LAUNCH(kernel, grid, lds, stream, ...)                                                                    \
+  do {                                                                                                               \
+    if (const int rc_ = rp_allow(kernel, lds)) return rc_;                                                           \
+    hipLaunchKernelGGL(kernel, grid, dim3(RP_THREADS), lds, stream, __VA_ARGS__);                                    \
+  } while (0)
+
+// queries per workgroup and the batch parts of the table gradient: enough workgroups for the chip, no more partial rows than that takes
+int rp_table_chunks(const ofb_relpos_args& a, int kb) {
+  const int64_t tiles = (int64_t)a.H * ((a.Nq + kb - 1) / kb);
+  const int64_t want = (768 + tiles - 1) / tiles;
+  return (int)(want < a.B ? (want < 1 ? 1 : want) : a.B);
+}
+int rp_kb(const ofb_relpos_args& a) { return a.dtype != RP_F32 && a.d <= 64 ? 64 : 32; }
+
+// key ranges of the forward: where the query tiles leave most of the chip idle, ranges of at least four tiles
+int rp_splits(const ofb_relpos_args& a) {
+  const int64_t wgs = (int64_t)a.B * a.H * ((a.Nq + RP_TILE - 1) / RP_TILE), nkb = (a.Nk + rp_kb(a) - 1) / rp_kb(a);
+  if (wgs >= 512 || nkb < 8) return 1;
+  const int64_t want = (1024 + wgs - 1) / wgs, most = nkb / 4;
+  const int64_t s = want < most ? want : most;
+  return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+int rp_check(const ofb_relpos_args* a) {
+  if (!a || !a->q || !a->k || !a->v || !a->table || !a->lut) return OFB_EINVAL;
+  if (a->B < 1 || a->H < 1 || a->Nq < 1 || a->Nk < 1 || a->d < 8 || a->d % 8 || a->dtype < 0 || a->dtype > 2) return OFB_EINVAL;
+  if (a->width < 1 || a->n_buckets < 1 || (!a->pos_q) != (!a->pos_k) || (a->pos_q && a->causal)) return OFB_EINVAL;
+  if (a->d > 128 || a->width > RP_WMAX || a->Nq > (1 << 29) || a->Nk > (1 << 29)) return OFB_ELIMIT;
+  if (a->q_offset > (1 << 29) || a->q_offset < -(1 << 29) || a->lo > (1 << 29) || a->lo < -(1 << 29)) return OFB_ELIMIT;
+  const int64_t tiles = (int64_t)a->B * a->H * (((int64_t)(a->Nq > a->Nk ? a->Nq : a->Nk) + 31) / 32);
+  if (tiles > 0x3fffffff) return OFB_ELIMIT;
+  const int64_t unit = a->dtype == RP_F32 ? 4 : 8;             // 16-byte loads
+  if (!ofb_aligned16(a->q) || !ofb_aligned16(a->k) || !ofb_aligned16(a->v)) return OFB_EINVAL;
+  for (int64_t s : {a->q_sb, a->q_st, a->q_sh, a->k_sb, a->k_st, a->k_sh, a->v_sb, a->v_st, a->v_sh})
+    if (s % unit || s < 0) return OFB_EINVAL;
+  if (a->dtype == RP_F32 && (!a->bound_q || !a->bound_k || !a->bound_v || a->n_bound < 1 || a->n_bound > RP_NBOUND)) return OFB_EINVAL;
+  return OFB_OK;
+}
+
+template <int DT, int DP> int rp_forward(const ofb_relpos_args& a, hipStream_t s) {
+  const int64_t wgs = (int64_t)a.B * a.H * ((a.Nq + RP_TILE - 1) / RP_TILE);
+  const int lds = rp_lds<DT, DP>(a, 0), splits = rp_splits(a);
+  if (splits > 1) {
+    if (!a.split_o || !a.split_ml) return OFB_EINVAL;
+    RP_LAUNCH((relpos_fwd_kernel<DT, DP, true>), dim3((unsigned)wgs, splits), lds, s, a);
+    const int64_t rows = (int64_t)a.B * a.H * a.Nq;
+    hipLaunchKernelGGL((relpos_join_kernel<DT>), dim3((unsigned)((rows + 3) / 4)), dim3(RP_THREADS), 0, s, a, splits);
+  } else {
+    RP_LAUNCH((relpos_fwd_kernel<DT, DP, false>), dim3((unsigned)wgs), lds, s, a);
+  }
+  return ofb_launch_status();
+}
+
+template <int DT, int DP> int rp_backward(const ofb_relpos_args& a, hipStream_t s) {
+  const int kb = rp_geo<DT, DP>::KB, nqt = (a.Nq + RP_TILE - 1) / RP_TILE, nkt = (a.Nk + RP_TILE - 1) / RP_TILE;
+  RP_LAUNCH((relpos_dq_kernel<DT, DP>), dim3((unsigned)((int64_t)a.B * a.H * nqt)), (rp_lds<DT, DP>(a, 0)), s, a);
+  RP_LAUNCH((relpos_dkv_kernel<DT, DP>), dim3((unsigned)((int64_t)a.B * a.H * nkt)), (rp_lds<DT, DP>(a, 1)), s, a);
+  if (a.dtable) {
+    const int chunks = rp_table_chunks(a, kb), nqb = (a.Nq + kb - 1) / kb;
+    RP_LAUNCH((relpos_dbias_kernel<DT, DP>), dim3((unsigned)((int64_t)a.H * nqb * chunks)), (rp_lds<DT, DP>(a, 2)), s, a, chunks);
+    hipLaunchKernelGGL(relpos_table_kernel, dim3((unsigned)(((int64_t)a.n_buckets * a.H + 3) / 4)), dim3(RP_THREADS), 0, s, a, (int64_t)nqb * chunks,
+                       a.pos_k ? (int64_t)0 : (int64_t)a.B * nqt * 4);
+  }
+  return ofb_launch_status();
+}
+
+#define RP_BY_TYPE(fn, a, s)                                                                                          \
+  switch ((a).dtype * 3 + ((a).d <= 32 ? 0 : (a).d <= 64 ? 1 : 2)) {                                                  \
+    case 0: return fn<RP_F32, 32>(a, s);                                                                              \
+    case 1: return fn<RP_F32, 64>(a, s);                                                                              \
+    case 2: return fn<RP_F32, 128>(a, s);                                                                             \
+    case 3: return fn<RP_BF16, 32>(a, s);                                                                             \
+    case 4: return fn<RP_BF16, 64>(a, s);                                                                             \
+    case 5: return fn<RP_BF16, 128>(a, s);                                                                            \
+    case 6: return fn<RP_F16, 32>(a, s);                                                                              \
+    case 7: return fn<RP_F16, 64>(a, s);                                                                              \
+    default: return fn<RP_F16, 128>(a, s);                                                                            \
+  }
+
+}  // namespace
+
+extern "C" int ofb_relpos_sizes(const ofb_relpos_args* a, int64_t* out4) {
+  if (!a || !out4 || a->B < 1 || a->H < 1 || a->Nq < 1 || a->Nk < 1 || a->width < 1) return OFB_EINVAL;
+  const int64_t rows = (int64_t)a->B * a->H * a->Nq, splits = rp_splits(*a), kb = rp_kb(*a);
+  out4[0] = splits > 1 ? splits * rows * a->d : 0;             // split_o
+  out4[1] = splits > 1 ? splits * rows * 2 : 0;                // split_ml
+  out4[2] = (int64_t)a->H * a->width * ((a->Nq + kb - 1) / kb) * rp_table_chunks(*a, (int)kb);      // partial
+  out4[3] = a->pos_k ? 0 : (int64_t)a->H * 2 * a->B * ((a->Nq + RP_TILE - 1) / RP_TILE) * 4;        // sat
+  return OFB_OK;
+}
+
+extern "C" int ofb_relpos_amax(const ofb_relpos_args* a, int32_t first, int32_t count, void* stream) {
+  if (!a || first < 0 || count < 1 || first + count > 4) return OFB_EINVAL;
+  if (a->B < 1 || a->H < 1 || a->Nq < 1 || a->Nk < 1 || a->d < 8 || a->d % 8 || a->dtype < 0 || a->dtype > 2) return OFB_EINVAL;
+  const void* x[4] = {a->q, a->k, a->v, a->dout};
+  const float* o[4] = {a->bound_q, a->bound_k, a->bound_v, a->bound_do};
+  for (int i = first; i < first + count; ++i)
+    if (!x[i] || !o[i] || !ofb_aligned16(x[i])) return OFB_EINVAL;
+  hipStream_t s = (hipStream_t)stream;
+  const dim3 grid(RP_NBOUND, count);
+  if (a->dtype == RP_F32) hipLaunchKernelGGL((relpos_amax_kernel<RP_F32>), grid, dim3(RP_THREADS), 0, s, *a, first);
+  else if (a->dtype == RP_BF16) hipLaunchKernelGGL((relpos_amax_kernel<RP_BF16>), grid, dim3(RP_THREADS), 0, s, *a, first);
+  else hipLaunchKernelGGL((relpos_amax_kernel<RP_F16>), grid, dim3(RP_THREADS), 0, s, *a, first);
+  return ofb_launch_status();
+}
+
+extern "C" int ofb_relpos_fwd(const ofb_relpos_args* a, void* stream) {
+  if (const int rc = rp_check(a)) return rc;
+  if (!a->out || !ofb_aligned16(a->out) || (a->out32 && !ofb_aligned16(a->out32))) return OFB_EINVAL;
+  for (int64_t s : {a->o_sb, a->o_st, a->o_sh})
+    if (s % 4 || s < 0) return OFB_EINVAL;
+  RP_BY_TYPE(rp_forward, *a, (hipStream_t)stream)
+}
+
+extern "C" int ofb_relpos_bwd(const ofb_relpos_args* a, void* stream) {
+  if (const int rc = rp_check(a)) return rc;
+  if (!a->dout || !a->out32 || !a->stats || !a->delta || !a->dq || !a->dk || !a->dv) return OFB_EINVAL;
+  if (a->dtable && (!a->partial || !a->bucket_start || !a->bucket_order || (!a->pos_k && !a->sat))) return OFB_EINVAL;
+  if (a->dtype != RP_BF16 && (!a->bound_v || !a->bound_do || a->n_bound < 1 || a->n_bound > RP_NBOUND || a->n_bound_do < 1 || a->n_bound_do > RP_NBOUND)) return OFB_EINVAL;
+  for (const void* p : {(const void*)a->dout, (const void*)a->out32, (const void*)a->dq, (const void*)a->dk, (const void*)a->dv})
+    if (!ofb_aligned16(p)) return OFB_EINVAL;
+  const int64_t unit = a->dtype == RP_F32 ? 4 : 8;
+  for (int64_t s : {a->do_sb, a->do_st, a->do_sh})
+    if (s % unit || s < 0) return OFB_EINVAL;
+  for (int64_t s : {a->dq_sb, a->dq_st, a->dq_sh, a->dk_sb, a->dk_st, a->dk_sh, a->dv_sb, a->dv_st, a->dv_sh})
+    if (s % 4 || s < 0) return OFB_EINVAL;
+  RP_BY_TYPE(rp_backward, *a, (hipStream_t)stream)
+}

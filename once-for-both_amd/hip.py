@@ -24,6 +24,8 @@ ACT_NONE, ACT_GELU, ACT_DGELU, ACT_GELU_GRAD, ACT_MULAUX, ACT_GELU_GRAD_T, ACT_M
 SYMBOLS = [
     'ofb_gemm_h', 'ofb_gemm_h_workspace_bytes', 'ofb_gemm_h_colpart_rows', 'ofb_gemm_h_aux_t_floats', 'ofb_hformat_bytes', 'ofb_to_hformat', 'ofb_patchify_hformat', 'ofb_to_hformat_colsum', 'ofb_to_hformat_colsum_nb', 'ofb_to_hformat_multi', 'ofb_from_hformat', 'ofb_colsum_h', 'ofb_colsum_h_slabs', 'ofb_tune', 'ofb_gemm_h_rn_tiles',
     'ofb_splitk_reduce', 'ofb_prof_enable', 'ofb_prof_collect',
+    'ofb_relpos_sizes', 'ofb_relpos_amax', 'ofb_relpos_fwd', 'ofb_relpos_bwd',
+    'ofb_distill_segments', 'ofb_distill_fwd', 'ofb_distill_bwd', 'ofb_top_logits_segments', 'ofb_top_logits',
     'ofb_layernorm_fwd', 'ofb_layernorm_fwd_h', 'ofb_layernorm_bwd_blocks', 'ofb_layernorm_bwd', 'ofb_layernorm_bwd_h', 'ofb_layernorm_bwd_h_rn', 'ofb_colsum_slabs', 'ofb_colsum', 'ofb_colsum_multi',
     'ofb_scale_rows', 'ofb_gate_fold_bwd', 'ofb_amax', 'ofb_attention_fwd', 'ofb_attention_fwd_h', 'ofb_attention_bwd', 'ofb_attention_bwd_wgmax',
     'ofb_gates_fwd', 'ofb_gates_bwd', 'ofb_flops_loss',
@@ -1183,3 +1185,100 @@ def jpeg_decode_pixels(jobs_dev, n, max_blocks, max_w, max_h, coef_dev, planes_d
         raise OfbError('jpeg_decode_pixels: int16 coefficients, uint8 planes / pixels')
     check(lib().ofb_jpeg_decode_pixels(ptr(jobs_dev), _i(n), _i(max_blocks), _i(max_w), _i(max_h), _void_p(coef_dev.data_ptr()),
                                        ptr(planes_dev), ptr(out_dev), stream()), 'ofb_jpeg_decode_pixels')
+
+
+# ---- attention with a relative position bias, distillation from stored top logits (csrc/relpos.hip, csrc/distill.hip): f32, bf16, f16 ------
+DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def on_device(t):
+    """context in which the current device is t's: launches and allocations follow the operands"""
+    if not t.is_cuda:
+        raise OfbError('once-for-both_amd kernels need device tensors (no CPU fallback); got a CPU tensor')
+    return torch.cuda.device(t.device) if _get_device is None or t.device.index != _get_device() else _same_device
+
+
+class _SameDevice:
+    def __enter__(self): return self
+    def __exit__(self, *a): return False
+
+
+_same_device = _SameDevice()
+
+
+class RelposArgs(C.Structure):
+    _fields_ = (
+        [(n, C.c_void_p) for n in ('q', 'k', 'v')]
+        + [(f'{t}_{s}', C.c_int64) for t in ('q', 'k', 'v') for s in ('sb', 'st', 'sh')]
+        + [('out', C.c_void_p)] + [(f'o_{s}', C.c_int64) for s in ('sb', 'st', 'sh')]
+        + [(n, C.c_void_p) for n in ('out32', 'stats', 'table', 'lut', 'bucket_start', 'bucket_order', 'pos_q', 'pos_k', 'key_lens')]
+        + [(n, C.c_int32) for n in ('lo', 'width', 'n_buckets', 'q_offset', 'causal', 'dtype', 'B', 'H', 'Nq', 'Nk', 'd')]
+        + [('scale', C.c_float)]
+        + [(n, C.c_void_p) for n in ('bound_q', 'bound_k', 'bound_v', 'bound_do')]
+        + [('n_bound', C.c_int32), ('n_bound_do', C.c_int32), ('split_o', C.c_void_p), ('split_ml', C.c_void_p), ('dout', C.c_void_p)]
+        + [(f'do_{s}', C.c_int64) for s in ('sb', 'st', 'sh')]
+        + [(n, C.c_void_p) for n in ('dq', 'dk', 'dv')]
+        + [(f'{t}_{s}', C.c_int64) for t in ('dq', 'dk', 'dv') for s in ('sb', 'st', 'sh')]
+        + [(n, C.c_void_p) for n in ('dtable', 'delta', 'partial', 'sat')])
+
+
+RELPOS_BOUNDS = 256                        # partial maxima per tensor that ofb_relpos_amax writes
+
+
+def relpos_tensor(args, name, t):
+    """q, k, v, out (o), dout (do), dq, dk, dv of the argument struct: a [B][tokens][H][d] tensor by address and strides"""
+    setattr(args, {'o': 'out', 'do': 'dout'}.get(name, name), t.data_ptr())
+    sb, st, sh, _ = t.stride()
+    setattr(args, name + '_sb', sb)
+    setattr(args, name + '_st', st)
+    setattr(args, name + '_sh', sh)
+
+
+def relpos_sizes(args):
+    """floats of the workspaces (split_o, split_ml, partial, sat)"""
+    out = (C.c_int64 * 4)()
+    check(lib().ofb_relpos_sizes(C.byref(args), out), 'ofb_relpos_sizes')
+    return list(out)
+
+
+def relpos_amax(args, first, count):
+    check(lib().ofb_relpos_amax(C.byref(args), _i(first), _i(count), stream()), 'ofb_relpos_amax')
+
+
+def relpos_fwd(args):
+    check(lib().ofb_relpos_fwd(C.byref(args), stream()), 'ofb_relpos_fwd')
+
+
+def relpos_bwd(args):
+    check(lib().ofb_relpos_bwd(C.byref(args), stream()), 'ofb_relpos_bwd')
+
+
+def _vp(t):
+    return None if t is None else _void_p(t.data_ptr())
+
+
+def distill_segments(R, V):
+    return int(lib().ofb_distill_segments(C.c_int64(R), _i(V)))
+
+
+def distill_fwd(z, values, indices, rest, tau, stats, part, row_loss, loss_scale, loss):
+    R, V = z.shape
+    check(lib().ofb_distill_fwd(_vp(z), _vp(values), _vp(indices), _i(indices.dtype == torch.int64), _vp(rest), C.c_int64(R), _i(V), _i(values.shape[1]),
+                                _f(tau), _i(DTYPE_CODE[z.dtype]), _vp(stats), _vp(part), _vp(row_loss), C.c_double(loss_scale), _vp(loss), stream()),
+          'ofb_distill_fwd')
+
+
+def distill_bwd(z, values, indices, tau, stats, up, grad_scale, dz):
+    R, V = z.shape
+    check(lib().ofb_distill_bwd(_vp(z), _vp(values), _vp(indices), _i(indices.dtype == torch.int64), C.c_int64(R), _i(V), _i(values.shape[1]), _f(tau),
+                                _i(DTYPE_CODE[z.dtype]), _vp(stats), _vp(up), _i(up.numel() > 1), _f(grad_scale), _vp(dz), stream()), 'ofb_distill_bwd')
+
+
+def top_logits_segments(R, V, K):
+    return int(lib().ofb_top_logits_segments(C.c_int64(R), _i(V), _i(K)))
+
+
+def top_logits(z, K, tau, values, indices, rest, cand, part):
+    R, V = z.shape
+    check(lib().ofb_top_logits(_vp(z), C.c_int64(R), _i(V), _i(K), _f(tau), _i(DTYPE_CODE[z.dtype]), _vp(values), _vp(indices), _vp(rest), _vp(cand),
+                               _vp(part), stream()), 'ofb_top_logits')

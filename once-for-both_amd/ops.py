@@ -872,3 +872,305 @@ class BiMaskGates(torch.autograd.Function):
         hip.gates_bwd(descs_dev, gdev, n)
         ctx.keep2 = (gdev, ghost, keep)
         return (None, None, *outs)
+
+
+# ---------------------------------------------------------------------------------------------------
+# attention with a learned relative position bias (csrc/relpos.hip)
+# ---------------------------------------------------------------------------------------------------
+def _att_operand(t):
+    """t where the kernels can read it as it is (channels contiguous, 16-byte aligned rows), a contiguous copy otherwise"""
+    unit = 16 // t.element_size()
+    sb, st, sh, sd = t.stride()
+    if sd != 1 or sb % unit or st % unit or sh % unit or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+class _RelposCall:
+    """the checked arguments of one call: everything that forward and backward share"""
+    __slots__ = ('buckets', 'scale', 'causal', 'q_offset', 'bound')
+
+    def __init__(self, q, k, v, table, buckets, scale, causal, key_lens, q_offset, bound=None):
+        for name, t in (('q', q), ('k', k), ('v', v)):
+            if not isinstance(t, torch.Tensor) or t.dim() != 4:
+                raise hip.OfbError(f'relpos_attention: {name} must be a (batch, tokens, heads, channels) tensor')
+            if t.dtype not in hip.DTYPE_CODE or t.dtype != q.dtype:
+                raise hip.OfbError(f'relpos_attention: q, k and v must share one of the types float32, bfloat16, float16; {name} is {t.dtype}')
+            if t.device != q.device:
+                raise hip.OfbError('relpos_attention: q, k and v must be on one device')
+        B, Nq, H, d = q.shape
+        if k.shape != v.shape or k.shape[0] != B or k.shape[2:] != q.shape[2:]:
+            raise hip.OfbError(f'relpos_attention: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}: k and v must have the same number of tokens, '
+                               'and batch, heads and channels of q (shared key heads are not supported)')
+        if d % 8 or not 8 <= d <= 128:
+            raise hip.OfbError(f'relpos_attention: {d} channels a head: a multiple of 8 up to 128 is supported')
+        if H < 1:
+            raise hip.OfbError('relpos_attention: at least one head')
+        if table.dtype != torch.float32 or tuple(table.shape) != (buckets.num_buckets, H) or table.device != q.device:
+            raise hip.OfbError(f'relpos_attention: the table must be a float32 ({buckets.num_buckets}, {H}) tensor on the device of q, got {table.dtype} {tuple(table.shape)}')
+        if key_lens is not None and (key_lens.dtype != torch.int32 or tuple(key_lens.shape) != (B,) or key_lens.device != q.device):
+            raise hip.OfbError(f'relpos_attention: key_lens must be an int32 tensor of {B} lengths on the device of q')
+        if buckets.positions is not None:
+            if causal or q_offset:
+                raise hip.OfbError('relpos_attention: causal and q_offset go by the number of a token, not by given positions')
+            if (len(buckets.positions[0]), len(buckets.positions[1])) != (Nq, k.shape[1]):
+                raise hip.OfbError(f'relpos_attention: positions of {len(buckets.positions[0])} queries and {len(buckets.positions[1])} keys, got {Nq} and {k.shape[1]}')
+        if abs(int(q_offset)) > 1 << 28 or max(Nq, k.shape[1]) > 1 << 28:
+            raise hip.OfbError('relpos_attention: positions beyond 2^28 are not supported')
+        if not q.is_cuda:
+            raise hip.OfbError('once-for-both_amd kernels need device tensors (no CPU fallback); got a CPU tensor')
+        self.buckets, self.causal, self.q_offset, self.bound = buckets, bool(causal), int(q_offset), bound
+        self.scale = float(scale) if scale is not None else d ** -0.5
+
+    def args(self, q, k, v, table, key_lens):
+        a, b = hip.RelposArgs(), self.buckets
+        lut, start, order, pq, pk = b.on(q.device)
+        for name, t in (('q', q), ('k', k), ('v', v)):
+            hip.relpos_tensor(a, name, t)
+        a.table, a.lut, a.bucket_start, a.bucket_order = table.data_ptr(), lut.data_ptr(), start.data_ptr(), order.data_ptr()
+        if pq is not None:
+            a.pos_q, a.pos_k = pq.data_ptr(), pk.data_ptr()
+        if key_lens is not None:
+            a.key_lens = key_lens.data_ptr()
+        a.lo, a.width, a.n_buckets, a.q_offset, a.causal, a.dtype = b.lo, b.width, b.num_buckets, self.q_offset, self.causal, hip.DTYPE_CODE[q.dtype]
+        a.B, a.Nq, a.H, a.d = q.shape
+        a.Nk, a.scale = k.shape[1], self.scale
+        return a
+
+    def bounds(self, a, like):
+        """f32: upper bounds of |q|, |k|, |v| for the split into f16 planes - the caller's scalar, or the tensors' own maxima"""
+        if self.bound is not None:
+            a.bound_q = a.bound_k = a.bound_v = self.bound.data_ptr()
+            a.n_bound = 1
+            return self.bound
+        part = torch.empty(3, hip.RELPOS_BOUNDS, device=like.device, dtype=torch.float32)
+        a.bound_q, a.bound_k, a.bound_v = (part.data_ptr() + 4 * hip.RELPOS_BOUNDS * i for i in range(3))
+        a.n_bound = hip.RELPOS_BOUNDS
+        return part
+
+    def forward(self, q, k, v, table, key_lens, keep):
+        """(out, unrounded out, row statistics, bounds): the last three only where `keep` asks for what the backward reads"""
+        with hip.on_device(q):
+            B, Nq, H, d = q.shape
+            out = torch.empty(B, Nq, H, d, device=q.device, dtype=q.dtype)
+            if out.numel() == 0 or k.shape[1] == 0:
+                return out.zero_(), None, None, None
+            a = self.args(q, k, v, table, key_lens)
+            hip.relpos_tensor(a, 'o', out)
+            out32 = stats = bounds = None
+            if keep:
+                out32 = out if q.dtype == torch.float32 else torch.empty(B, Nq, H, d, device=q.device, dtype=torch.float32)
+                stats = torch.empty(B, H, Nq, 2, device=q.device, dtype=torch.float32)
+                a.stats = stats.data_ptr()
+                a.out32 = None if out32 is out else out32.data_ptr()
+            if q.dtype == torch.float32:
+                bounds = self.bounds(a, q)
+                if self.bound is None:
+                    hip.relpos_amax(a, 0, 3)
+            n = hip.relpos_sizes(a)
+            if n[0]:
+                ws = torch.empty(n[0] + n[1], device=q.device, dtype=torch.float32)
+                a.split_o, a.split_ml = ws.data_ptr(), ws.data_ptr() + 4 * n[0]
+            hip.relpos_fwd(a)
+            return out, out32, stats, bounds
+
+    def backward(self, dout, q, k, v, table, key_lens, out32, stats, bounds, dq, dk, dv, want_table):
+        """fills dq, dk, dv and returns the table's gradient (or None)"""
+        with hip.on_device(q):
+            dtable = torch.zeros_like(table) if want_table and stats is None else None
+            if stats is None:                                   # nothing was attended to
+                for t in (dq, dk, dv):
+                    t.zero_()
+                return dtable
+            B, Nq, H, d = q.shape
+            dout = _att_operand(dout)
+            a = self.args(q, k, v, table, key_lens)
+            for name, t in (('do', dout), ('dq', dq), ('dk', dk), ('dv', dv)):
+                hip.relpos_tensor(a, name, t)
+            n = hip.relpos_sizes(a)
+            n = [B * H * Nq, n[2] if want_table else 0, n[3] if want_table else 0]
+            ws = torch.empty(sum(n), device=q.device, dtype=torch.float32)
+            a.out32, a.stats, a.delta = out32.data_ptr(), stats.data_ptr(), ws.data_ptr()
+            if want_table:
+                dtable = torch.empty(table.shape, device=q.device, dtype=torch.float32)
+                a.dtable, a.partial = dtable.data_ptr(), ws.data_ptr() + 4 * n[0]
+                if n[2]:
+                    a.sat = ws.data_ptr() + 4 * (n[0] + n[1])
+            if q.dtype != torch.bfloat16:                       # dS is scaled by a bound of it: maxima of v and dout
+                part = torch.empty(2, hip.RELPOS_BOUNDS, device=q.device, dtype=torch.float32)
+                if q.dtype == torch.float32:
+                    m = hip.RELPOS_BOUNDS if self.bound is None else 1
+                    a.bound_q, a.bound_k, a.bound_v = (bounds.data_ptr() + (4 * m * i if self.bound is None else 0) for i in range(3))
+                    a.n_bound = m
+                else:
+                    a.bound_v, a.n_bound = part.data_ptr(), hip.RELPOS_BOUNDS
+                a.bound_do, a.n_bound_do = part.data_ptr() + 4 * hip.RELPOS_BOUNDS, hip.RELPOS_BOUNDS
+                hip.relpos_amax(a, 3 if q.dtype == torch.float32 else 2, 1 if q.dtype == torch.float32 else 2)
+            hip.relpos_bwd(a)
+            return dtable
+
+
+class RelposAttention(torch.autograd.Function):
+    """softmax(scale q k^T + table[bucket]) v on (B, tokens, H, d) tensors; gradients of q, k, v and the table"""
+
+    @staticmethod
+    def forward(ctx, q, k, v, table, key_lens, call):
+        q, k, v, table = _att_operand(q), _att_operand(k), _att_operand(v), _c(table)
+        out, out32, stats, bounds = call.forward(q, k, v, table, key_lens, True)
+        ctx.save_for_backward(q, k, v, table, key_lens, out32, stats, bounds)
+        ctx.call = call
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, table, key_lens, out32, stats, bounds = ctx.saved_tensors
+        dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
+        dtable = ctx.call.backward(dout, q, k, v, table, key_lens, out32, stats, bounds, dq, dk, dv, ctx.needs_input_grad[3])
+        return dq, dk, dv, dtable, None, None
+
+
+class RelposAttentionPacked(torch.autograd.Function):
+    """the same on a packed (B, N, 3, H, d) tensor, as a qkv projection leaves it; its gradient is packed too"""
+
+    @staticmethod
+    def forward(ctx, qkv, table, key_lens, call):
+        if not qkv.is_contiguous() or qkv.data_ptr() % 16:
+            qkv = qkv.clone(memory_format=torch.contiguous_format)
+        table = _c(table)
+        out, out32, stats, bounds = call.forward(*qkv.unbind(2), table, key_lens, True)
+        ctx.save_for_backward(qkv, table, key_lens, out32, stats, bounds)
+        ctx.call = call
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        qkv, table, key_lens, out32, stats, bounds = ctx.saved_tensors
+        dqkv = torch.empty_like(qkv)
+        dtable = ctx.call.backward(dout, *qkv.unbind(2), table, key_lens, out32, stats, bounds, *dqkv.unbind(2), ctx.needs_input_grad[1])
+        return dqkv, dtable, None, None
+
+
+def relpos_attention(q, k, v, table, buckets, scale=None, causal=False, key_lens=None, q_offset=0):
+    """softmax(scale q k^T + bias) v with a learned bias of the relative position: bias[b, h, i, j] = table[bucket(position of key j - position of query i), h].
+
+    q (B, Nq, H, d), k and v (B, Nk, H, d): float32, bfloat16 or float16, any strides (channels that are not contiguous or rows that are not 16-byte aligned
+    are copied first), d a multiple of 8 up to 128; table (buckets.num_buckets, H) float32; buckets a RelPosBuckets; scale d^-0.5 by default.
+    Key j stands at position j and query i at i + q_offset (new tokens behind a cache: q_offset = Nk - Nq), unless the plan has positions of its own.
+    causal: a query sees the keys at or before its position.  key_lens (B,) int32: keys from there on are padding - they are not read, and
+    their gradients are zero; a length beyond Nk counts as Nk, one below 0 as 0.  A query that sees no key has output and gradients 0.
+    Returns (B, Nq, H, d) of q's type.  Differentiable once, in q, k, v and the table; the same inputs give the same bits."""
+    call = _RelposCall(q, k, v, table, buckets, scale, causal, key_lens, q_offset)
+    if key_lens is not None:
+        key_lens = _c(key_lens)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad):
+        return RelposAttention.apply(q, k, v, table, key_lens, call)
+    return call.forward(_att_operand(q), _att_operand(k), _att_operand(v), _c(table), key_lens, False)[0]
+
+
+def relpos_attention_qkv(qkv, table, buckets, scale=None, causal=False, key_lens=None, bound=None):
+    """relpos_attention of a packed (B, N, 3, H, d) tensor: the gradient of qkv is one packed tensor.  bound (float32 qkv): a device scalar at least as
+    large as every |element|, if the producer has one; measured otherwise."""
+    if not isinstance(qkv, torch.Tensor) or qkv.dim() != 5 or qkv.shape[2] != 3:
+        raise hip.OfbError('relpos_attention_qkv: qkv must be a (batch, tokens, 3, heads, channels) tensor')
+    if bound is not None and (bound.dtype != torch.float32 or bound.numel() != 1 or bound.device != qkv.device):
+        raise hip.OfbError('relpos_attention_qkv: bound must be one float32 on the device of qkv')
+    call = _RelposCall(*qkv.unbind(2), table, buckets, scale, causal, key_lens, 0, bound if qkv.dtype == torch.float32 else None)
+    if key_lens is not None:
+        key_lens = _c(key_lens)
+    if torch.is_grad_enabled() and (qkv.requires_grad or table.requires_grad):
+        return RelposAttentionPacked.apply(qkv, table, key_lens, call)
+    return call.forward(*(_att_operand(t) for t in qkv.unbind(2)), _c(table), key_lens, False)[0]
+
+
+# ---------------------------------------------------------------------------------------------------
+# distillation from a teacher's top logits (csrc/distill.hip)
+# ---------------------------------------------------------------------------------------------------
+def _rows_operand(t):
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _check_logits(what, z, K, temperature):
+    if not isinstance(z, torch.Tensor) or z.dim() != 2 or z.dtype not in hip.DTYPE_CODE:
+        raise hip.OfbError(f'{what}: logits must be a (rows, classes) tensor of float32, bfloat16 or float16')
+    if not 0 < float(temperature) < 3e38:
+        raise hip.OfbError(f'{what}: temperature must be positive and finite, got {temperature}')
+    if not 1 <= K <= min(z.shape[1], 1024):
+        raise hip.OfbError(f'{what}: {K} of {z.shape[1]} classes: 1 to 1024 can be stored, at most all')
+    if z.shape[1] > 1 << 30 or z.shape[0] > 1 << 24:
+        raise hip.OfbError(f'{what}: at most 2^24 rows of 2^30 classes are supported')
+    if not z.is_cuda:
+        raise hip.OfbError('once-for-both_amd kernels need device tensors (no CPU fallback); got a CPU tensor')
+
+
+def top_logits(logits, k, temperature=1.0):
+    """What a teacher stores of a (rows, classes) tensor: (values, indices, rest) - the k largest logits of each row in descending order, in the type of
+    `logits`; their classes, int32 (ties: the lowest class first; NaN counts as the largest); and rest = logsumexp of the OTHER logits / temperature, float32 (-inf if there
+    are none).  No gradient."""
+    z = logits.detach()
+    K = int(k)
+    _check_logits('top_logits', z, K, temperature)
+    with hip.on_device(z):
+        z = _rows_operand(z)
+        R, V = z.shape
+        values, indices = torch.empty(R, K, device=z.device, dtype=z.dtype), torch.empty(R, K, device=z.device, dtype=torch.int32)
+        rest = torch.empty(R, device=z.device, dtype=torch.float32)
+        if R:
+            segs = hip.top_logits_segments(R, V, K)
+            cand = torch.empty(R, segs, K, device=z.device, dtype=torch.int64) if segs > 1 else None
+            part = torch.empty(R, segs, 2, device=z.device, dtype=torch.float32) if segs > 1 else None
+            hip.top_logits(z, K, float(temperature), values, indices, rest, cand, part)
+        return values, indices, rest
+
+
+class DistillTopLogits(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, values, indices, rest, tau, reduction):
+        with hip.on_device(z):
+            z = _rows_operand(z)
+            R, V = z.shape
+            segs = hip.distill_segments(R, V)
+            stats, rows = _new(z, R, 8), _new(z, R)
+            loss = _new(z, 1) if reduction != 'none' else None
+            hip.distill_fwd(z, values, indices, rest, tau, stats, _new(z, R, segs, 2) if segs > 1 else None, rows, 1.0 / R if reduction == 'mean' else 1.0, loss)
+            ctx.save_for_backward(z, values, indices, stats)
+            ctx.tau, ctx.scale = tau, tau / R if reduction == 'mean' else tau
+            return rows if loss is None else loss[0]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, up):
+        z, values, indices, stats = ctx.saved_tensors
+        with hip.on_device(z):
+            dz = torch.empty(z.shape, device=z.device, dtype=z.dtype)
+            up = _c(up).reshape(-1)
+            hip.distill_bwd(z, values, indices, ctx.tau, stats, up, ctx.scale, dz)
+        return dz, None, None, None, None, None
+
+
+def distill_top_logits(logits, values, indices, rest=None, temperature=1.0, reduction='mean'):
+    """Kullback-Leibler divergence of a student from a teacher of whom only the top logits were stored, times temperature^2.
+
+    logits (rows, classes) of the student: float32, bfloat16 or float16; values (rows, K) of the same type and indices (rows, K) int32 or int64: the teacher's logits and
+    their classes, in any order.  An entry whose class is not one of 0 .. classes - 1 (a shorter list: -1), or whose value is -inf, is left out; a class that comes
+    twice counts with both values.  rest (rows,) float32: log-sum-exp of the teacher's other logits / temperature (top_logits) - the classes that were not stored then
+    share the remaining probability as one; without it the stored probabilities are renormalised.  A row without an entry has loss and gradient 0.
+    reduction 'mean' (over the rows), 'sum' or 'none' ((rows,) float32).  Differentiable once, in logits."""
+    if not isinstance(values, torch.Tensor) or not isinstance(indices, torch.Tensor) or values.dim() != 2 or values.shape != indices.shape:
+        raise hip.OfbError('distill_top_logits: values and indices must be two (rows, K) tensors')
+    _check_logits('distill_top_logits', logits, values.shape[1], temperature)
+    if values.shape[0] != logits.shape[0] or values.dtype != logits.dtype or indices.dtype not in (torch.int32, torch.int64):
+        raise hip.OfbError(f'distill_top_logits: {logits.shape[0]} rows of {logits.dtype} need as many stored values of that type and int32 or int64 classes')
+    if rest is not None and (rest.dtype != torch.float32 or tuple(rest.shape) != (logits.shape[0],)):
+        raise hip.OfbError('distill_top_logits: rest must be a float32 tensor of one value per row')
+    if any(t is not None and t.device != logits.device for t in (values, indices, rest)):
+        raise hip.OfbError('distill_top_logits: all tensors must be on one device')
+    if reduction not in ('mean', 'sum', 'none'):
+        raise hip.OfbError(f"distill_top_logits: reduction '{reduction}' is none of mean, sum, none")
+    if logits.shape[0] == 0:
+        if reduction == 'mean':
+            raise hip.OfbError('distill_top_logits: the mean over no rows')
+        return logits.float().sum(1) if reduction == 'none' else logits.float().sum()
+    values, indices = _c(values.detach()), _c(indices)
+    return DistillTopLogits.apply(logits, values, indices, _c(rest.detach()) if rest is not None else None, float(temperature), reduction)
