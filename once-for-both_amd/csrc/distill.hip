@@ -59,22 +59,53 @@ struct ds_row {
   __device__ __forceinline__ int chunks() const { return (end + ds_type<DT>::CH - 1) / ds_type<DT>::CH; }
   __device__ __forceinline__ bool whole(int c) const { return c * ds_type<DT>::CH >= mis && (c + 1) * ds_type<DT>::CH <= end; }
   __device__ __forceinline__ bool has(int c, int i) const { const int u = c * ds_type<DT>::CH + i; return u >= mis && u < end; }
-  // the chunk's values; `fill` where there is no class
+  __device__ __forceinline__ uint4 fetch(int c) const { return *reinterpret_cast<const uint4*>(base + (int64_t)c * 16); }
+  static __device__ __forceinline__ void unpack(uint4 v, float (&x)[ds_type<DT>::CH]) {
+    const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < ds_type<DT>::CH; ++i) {
+      if constexpr (DT == DS_F32) x[i] = __uint_as_float(w[i]);
+      else if constexpr (DT == DS_BF16) x[i] = __uint_as_float((i & 1) ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+      else x[i] = (i & 1) ? ofb_f16_hi(w[i >> 1]) : ofb_f16_lo(w[i >> 1]);
+    }
+  }
+  // runs f(chunk, values) over chunks c0 + thread, c0 + thread + THREADS, ...: `fill` stands where a chunk has no class.  Four chunks are loaded
+  // before the first is used (only the row's first and last chunk can be partial: they are left to the end).
+  template <int THREADS, typename F>
+  __device__ __forceinline__ void each(int c0, int c1, float fill, F f) const {
+    constexpr int CH = ds_type<DT>::CH;
+    int a0 = c0, a1 = c1;
+    if (a0 < a1 && !whole(a0)) ++a0;
+    if (a0 < a1 && !whole(a1 - 1)) --a1;
+    int c = a0 + threadIdx.x;
+    for (; c + 3 * THREADS < a1; c += 4 * THREADS) {
+      uint4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = fetch(c + j * THREADS);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float x[CH];
+        unpack(v[j], x);
+        f(c + j * THREADS, x);
+      }
+    }
+    for (; c < a1; c += THREADS) {
+      float x[CH];
+      unpack(fetch(c), x);
+      f(c, x);
+    }
+    c = threadIdx.x == 0 ? c0 : c1 - 1;                       // the partial ones: thread 0 and thread 1
+    if (threadIdx.x < 2 && c < c1 && !whole(c) && (threadIdx.x == 0 || c > c0 || whole(c0))) {
+      float x[CH];
+      load(c, x, fill);
+      f(c, x);
+    }
+  }
+  // a partial chunk's values; `fill` where there is no class
   __device__ __forceinline__ void load(int c, float (&x)[ds_type<DT>::CH], float fill) const {
     constexpr int CH = ds_type<DT>::CH;
     const char* p = base + (int64_t)c * 16;
-    if (whole(c)) {
-      if constexpr (DT == DS_F32) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(p);
-#pragma unroll
-        for (int i = 0; i < CH; ++i) x[i] = v[i];
-      } else {
-        const uint4 v = *reinterpret_cast<const uint4*>(p);
-        const unsigned w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < CH; ++i) x[i] = ds_value<DT>((typename ds_type<DT>::raw)(w[i >> 1] >> (16 * (i & 1))));
-      }
-    } else {
+    {
 #pragma unroll
       for (int i = 0; i < CH; ++i) x[i] = has(c, i) ? ds_value<DT>(reinterpret_cast<const typename ds_type<DT>::raw*>(p)[i]) : fill;
     }
@@ -174,6 +205,19 @@ __device__ __forceinline__ int ds_class(const ds_args& a, int64_t row, int k, fl
   return (i < 0 || i >= a.V || value == -INFINITY) ? -1 : (int)i;
 }
 
+// whether no entry before k has class i (cls: 16-byte aligned, padded to a multiple of four)
+__device__ __forceinline__ bool ds_first(const int* cls, int k, int i) {
+  bool first = true;
+  for (int e = 0; e < k; e += 4) {
+    const int4 o = *reinterpret_cast<const int4*>(&cls[e]);
+    first &= o.x != i;
+    first &= o.y != i || e + 1 >= k;
+    first &= o.z != i || e + 2 >= k;
+    first &= o.w != i || e + 3 >= k;
+  }
+  return first;
+}
+
 // The row's loss and what the backward needs, from (m_t, s_t) of the classes that are not stored.  The sums over the stored classes are in
 // 64 bits: the loss is a difference of logarithms of the size of log V.
 template <int DT>
@@ -198,8 +242,7 @@ __device__ void ds_finish(const ds_args& a, int64_t row, ds_sum tail, int* cls, 
     const int i = ds_class<DT>(a, row, k, v);
     t[j] = v;
     y[j] = ds_value<DT>(((const typename ds_type<DT>::raw*)a.z)[row * a.V + i]);
-    own[j] = true;                                             // the first entry of a class stands for it in the sum over the classes
-    for (int e = 0; e < k; ++e) own[j] &= cls[e] != i;
+    own[j] = ds_first(cls, k, i);                              // the first entry of a class stands for it in the sum over the classes
     mt = fmaxf(mt, v * a.c);
     m = fmaxf(m, y[j] * a.c);
     mine += own[j];
@@ -253,8 +296,9 @@ __device__ void ds_finish(const ds_args& a, int64_t row, ds_sum tail, int* cls, 
 template <int DT, bool WHOLE>      // WHOLE: one segment a row, which also finishes it
 __global__ __launch_bounds__(DS_THREADS) void distill_fwd_kernel(ds_args a) {
   constexpr int CH = ds_type<DT>::CH;
-  __shared__ __attribute__((aligned(16))) unsigned bits[DS_SEG / 32 + 4];
-  __shared__ __attribute__((aligned(16))) int cls[DS_KMAX];
+  // a bit per class of the segment, and the entries' classes: as much LDS as they take, so that eight workgroups share a CU
+  extern __shared__ __attribute__((aligned(16))) int cls[];
+  unsigned* bits = reinterpret_cast<unsigned*>(cls + ((a.K + 3) & ~3));
   __shared__ double redd[4];
   __shared__ float redf[8];
   const int64_t row = blockIdx.x / a.segs;
@@ -271,9 +315,7 @@ __global__ __launch_bounds__(DS_THREADS) void distill_fwd_kernel(ds_args a) {
   }
   __syncthreads();
   ds_sum sum;
-  for (int c = c0 + threadIdx.x; c < c1; c += DS_THREADS) {
-    float x[CH];
-    r.load(c, x, -INFINITY);
+  r.template each<DS_THREADS>(c0, c1, -INFINITY, [&](int c, float (&x)[CH]) {
     const int u = (c - c0) * CH;
     const unsigned b = (bits[u >> 5] >> (u & 31)) & ((1u << CH) - 1u);
     if (b) {
@@ -282,7 +324,7 @@ __global__ __launch_bounds__(DS_THREADS) void distill_fwd_kernel(ds_args a) {
         if (b >> i & 1) x[i] = -INFINITY;
     }
     sum.add<CH>(x, a.c);
-  }
+  });
   sum = ds_join<DS_THREADS>(sum, redf, redf + 4);
   if constexpr (WHOLE) {
     ds_finish<DT>(a, row, sum, cls, redd, redf);
@@ -299,7 +341,8 @@ __global__ __launch_bounds__(DS_THREADS) void distill_finish_kernel(ds_args a) {
   __shared__ float redf[8];
   const int64_t row = blockIdx.x;
   ds_sum sum;
-  for (int i = 0; i < a.segs; ++i) sum.join(a.part[2 * (row * a.segs + i)], a.part[2 * (row * a.segs + i) + 1]);
+  for (int i = threadIdx.x; i < a.segs; i += DS_THREADS) sum.join(a.part[2 * (row * a.segs + i)], a.part[2 * (row * a.segs + i) + 1]);
+  sum = ds_join<DS_THREADS>(sum, redf, redf + 4);
   ds_finish<DT>(a, row, sum, cls, redd, redf);
 }
 
@@ -316,7 +359,7 @@ template <int DT>
 __global__ __launch_bounds__(DS_THREADS) void distill_bwd_kernel(ds_args a) {
   constexpr int CH = ds_type<DT>::CH;
   typedef typename ds_type<DT>::raw raw;
-  __shared__ int cls[DS_KMAX];
+  __shared__ __attribute__((aligned(16))) int cls[DS_KMAX];
   __shared__ float prob[DS_KMAX];
   const int64_t row = blockIdx.x / a.segs;
   const int seg = blockIdx.x % a.segs;
@@ -327,9 +370,7 @@ __global__ __launch_bounds__(DS_THREADS) void distill_bwd_kernel(ds_args a) {
   const bool used = st[6] != 0.f;
   const float g = a.up[a.up_rows ? row : 0] * a.grad_scale, kappa = st[1] * g;
   char* out = (char*)a.dz + (row * a.V - r.mis) * (int64_t)ds_type<DT>::ES;
-  for (int c = c0 + threadIdx.x; c < c1; c += DS_THREADS) {
-    float x[CH];
-    r.load(c, x, 0.f);
+  r.template each<DS_THREADS>(c0, c1, 0.f, [&](int c, float (&x)[CH]) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) x[i] = used ? __builtin_amdgcn_exp2f(fmaf(x[i], a.c, -mt)) * kappa : 0.f;
     char* p = out + (int64_t)c * 16;
@@ -350,22 +391,26 @@ __global__ __launch_bounds__(DS_THREADS) void distill_bwd_kernel(ds_args a) {
       for (int i = 0; i < CH; ++i)
         if (r.has(c, i)) reinterpret_cast<raw*>(p)[i] = ds_raw<DT>(x[i]);
     }
-  }
+  });
   if (!used) return;
-  for (int k = threadIdx.x; k < a.K; k += DS_THREADS) {
-    float v;
-    cls[k] = ds_class<DT>(a, row, k, v);
+  for (int k = threadIdx.x; k < ((a.K + 3) & ~3); k += DS_THREADS) {
+    float v = 0.f;
+    cls[k] = k < a.K ? ds_class<DT>(a, row, k, v) : -1;
     prob[k] = cls[k] < 0 ? 0.f : __builtin_amdgcn_exp2f(fmaf(v, a.c, -mk)) * ik;
   }
   __syncthreads();                                             // ... and the stores above come before those below
   for (int k = threadIdx.x; k < a.K; k += DS_THREADS) {
     const int i = cls[k], u = i + r.mis;
     if (i < 0 || u < c0 * CH || u >= c1 * CH) continue;
-    bool first = true;
-    for (int e = 0; e < k; ++e) first &= cls[e] != i;
-    if (!first) continue;
+    if (!ds_first(cls, k, i)) continue;
     float p = prob[k];
-    for (int e = k + 1; e < a.K; ++e) p += cls[e] == i ? prob[e] : 0.f;
+    for (int e = (k + 1) & ~3; e < a.K; e += 4) {
+      const int4 o = *reinterpret_cast<const int4*>(&cls[e]);
+      if (o.x == i && e > k) p += prob[e];
+      if (o.y == i && e + 1 > k) p += prob[e + 1];
+      if (o.z == i && e + 2 > k) p += prob[e + 2];
+      if (o.w == i && e + 3 > k) p += prob[e + 3];
+    }
     const int64_t at = row * a.V + i;
     const float q = __builtin_amdgcn_exp2f(fmaf(ds_value<DT>(((const raw*)a.z)[at]), a.c, -m)) * is;
     ((raw*)a.dz)[at] = ds_raw<DT>((q - p) * g);
@@ -426,7 +471,8 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(tl_args a) {
   __shared__ __attribute__((aligned(16))) unsigned long long list[TL_CAP + 2];
   __shared__ float left[TL_CAP];
   __shared__ float redm[THREADS / 64], reds[THREADS / 64];
-  __shared__ int count, total;
+  __shared__ int count;
+  __shared__ unsigned bound;
   unsigned* tops = reinterpret_cast<unsigned*>(left);
   const int64_t row = blockIdx.x / a.segs;
   const int seg = blockIdx.x % a.segs;
@@ -435,78 +481,85 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(tl_args a) {
   const int have = max(0, min(r.end, c1 * CH) - max(r.mis, c0 * CH)), K = min(a.K, have);
 
   // A bound for the K-th largest element: the K-th largest of the threads' own maxima - K different elements are at least that large, and
-  // hardly more than K are when the threads' elements are no sorted run.
-  unsigned top = 0u;
-  for (int c = c0 + threadIdx.x; c < c1; c += THREADS) {
-    float x[CH];
-    r.load(c, x, 0.f);
+  // hardly more than K are when the threads' elements are no sorted run.  (NaN are left out of the maxima; they pass the bound below.)
+  float top = -INFINITY;
+  bool any = false;
+  r.template each<THREADS>(c0, c1, -INFINITY, [&](int c, float (&x)[CH]) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i)
-      if (r.whole(c) || r.has(c, i)) top = max(top, tl_key(x[i]));
-  }
-  if (threadIdx.x == 0) { count = 0; total = 0; }
-  tops[threadIdx.x] = top;
+    for (int i = 0; i < CH; ++i) top = fmaxf(top, x[i]);
+    any = true;
+  });
+  if (threadIdx.x == 0) count = 0;
+  tops[threadIdx.x] = any ? tl_key(top) : 0u;
   __syncthreads();
-  unsigned bound = 0u;
-  {
-    int more = 0;
-    for (int e = 0; e < THREADS; ++e) { const unsigned o = tops[e]; more += (o > top) || (o == top && e < (int)threadIdx.x); }
-    __syncthreads();
-    if (more == K - 1) total = (int)top;                       // exactly one thread (K <= THREADS); 0 where it has no element
-    __syncthreads();
-    bound = K >= 1 && K <= THREADS ? (unsigned)total : 0u;
-    __syncthreads();
-    if (threadIdx.x == 0) total = 0;
-  }
-  // how many are there
-  int n = 0;
-  for (int c = c0 + threadIdx.x; c < c1; c += THREADS) {
-    float x[CH];
-    r.load(c, x, 0.f);
+  if (threadIdx.x < 64) {                                      // one wave bisects the upper 20 bits of the maxima's keys, rounded down
+    unsigned v[THREADS / 64], found = 0u;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) n += (r.whole(c) || r.has(c, i)) && tl_key(x[i]) >= bound;
-  }
-  __syncthreads();
-  if (n) atomicAdd(&total, n);
-  __syncthreads();
-  unsigned long long floor_key = (unsigned long long)bound << 32;
-  if (total > TL_CAP) {
-    // many equal elements, or a sorted run: the K-th largest key itself, bit by bit from the top
-    floor_key = 0ull;
-    for (int bit = 63; bit >= 0; --bit) {
-      const unsigned long long probe = floor_key | (1ull << bit);
-      int k = 0;
-      for (int c = c0 + threadIdx.x; c < c1; c += THREADS) {
-        float x[CH];
-        r.load(c, x, 0.f);
+    for (int i = 0; i < THREADS / 64; ++i) v[i] = tops[threadIdx.x + 64 * i];
+    for (int bit = 31; bit >= 12; --bit) {
+      const unsigned probe = found | (1u << bit);
+      int n = 0;
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          const unsigned cls = (unsigned)(c * CH + i - r.mis);
-          k += (r.whole(c) || r.has(c, i)) && (((unsigned long long)tl_key(x[i]) << 32) | (unsigned)~cls) >= probe;
-        }
-      }
-      __syncthreads();
-      if (threadIdx.x == 0) total = 0;
-      __syncthreads();
-      if (k) atomicAdd(&total, k);
-      __syncthreads();
-      if (total >= K) floor_key = probe;
+      for (int i = 0; i < THREADS / 64; ++i) n += __popcll(__ballot(v[i] >= probe));
+      if (n >= K) found = probe;
     }
+    if (threadIdx.x == 0) bound = found;
   }
+  __syncthreads();
+  // no NaN is less than the bound, and nothing is where the bound is no number: too few threads have elements
+  const float least = tl_float(bound);
   ds_sum sum;
-  for (int c = c0 + threadIdx.x; c < c1; c += THREADS) {
-    float x[CH];
-    r.load(c, x, -INFINITY);
+  r.template each<THREADS>(c0, c1, -INFINITY, [&](int c, float (&x)[CH]) {
+    bool hit = false;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const unsigned cls = (unsigned)(c * CH + i - r.mis);
-      const unsigned long long k = ((unsigned long long)tl_key(x[i]) << 32) | (unsigned)~cls;
-      if ((r.whole(c) || r.has(c, i)) && k >= floor_key) {
-        list[atomicAdd(&count, 1)] = k;
-        x[i] = -INFINITY;
+    for (int i = 0; i < CH; ++i) hit |= !(x[i] < least);
+    if (hit) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        if (!(x[i] < least) && r.has(c, i)) {
+          const int at = atomicAdd(&count, 1);
+          if (at < TL_CAP) list[at] = ((unsigned long long)tl_key(x[i]) << 32) | (unsigned)~(unsigned)(c * CH + i - r.mis);
+          x[i] = -INFINITY;
+        }
       }
     }
     sum.add<CH>(x, a.c);
+  });
+  __syncthreads();
+  int n = count;
+  if (n > TL_CAP) {
+    // many equal elements, or a sorted run: the K-th largest key itself, bit by bit from the top
+    unsigned long long floor_key = 0ull;
+    for (int bit = 63; bit >= 0; --bit) {
+      const unsigned long long probe = floor_key | (1ull << bit);
+      int k = 0;
+      r.template each<THREADS>(c0, c1, 0.f, [&](int c, float (&x)[CH]) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+          k += r.has(c, i) && (((unsigned long long)tl_key(x[i]) << 32) | (unsigned)~(unsigned)(c * CH + i - r.mis)) >= probe;
+      });
+      __syncthreads();
+      if (threadIdx.x == 0) count = 0;
+      __syncthreads();
+      if (k) atomicAdd(&count, k);
+      __syncthreads();
+      if (count >= K) floor_key = probe;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) count = 0;
+    __syncthreads();
+    sum = ds_sum();
+    r.template each<THREADS>(c0, c1, -INFINITY, [&](int c, float (&x)[CH]) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const unsigned long long k = ((unsigned long long)tl_key(x[i]) << 32) | (unsigned)~(unsigned)(c * CH + i - r.mis);
+        if (r.has(c, i) && k >= floor_key) {
+          list[atomicAdd(&count, 1)] = k;
+          x[i] = -INFINITY;
+        }
+      }
+      sum.add<CH>(x, a.c);
+    });
   }
   __syncthreads();
   n = count;
@@ -593,10 +646,12 @@ extern "C" int ofb_distill_fwd(const void* z, const void* values, const void* in
   if (R * a.segs > 0x7fffffff) return OFB_ELIMIT;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)(R * a.segs)), block(DS_THREADS);
+  // (a row spans one chunk more than V classes take where it starts inside one; the last word is only cleared)
+  const int ch = 16 / ds_es(dtype), nc = (V + 2 * ch - 2) / ch, lds = (((K + 3) & ~3) + (nc + a.segs - 1) / a.segs * ch / 32 + 2) * 4;
 #define DS_FWD(DT)                                                                                        \
-  if (a.segs == 1) hipLaunchKernelGGL((distill_fwd_kernel<DT, true>), grid, block, 0, s, a);              \
+  if (a.segs == 1) hipLaunchKernelGGL((distill_fwd_kernel<DT, true>), grid, block, lds, s, a);            \
   else {                                                                                                  \
-    hipLaunchKernelGGL((distill_fwd_kernel<DT, false>), grid, block, 0, s, a);                            \
+    hipLaunchKernelGGL((distill_fwd_kernel<DT, false>), grid, block, lds, s, a);                          \
     hipLaunchKernelGGL((distill_finish_kernel<DT>), dim3((unsigned)R), block, 0, s, a);                   \
   }
   if (dtype == DS_F32) { DS_FWD(DS_F32) } else if (dtype == DS_BF16) { DS_FWD(DS_BF16) } else { DS_FWD(DS_F16) }

@@ -24,6 +24,13 @@
 #define RP_F16 2
 #define RP_THREADS 256
 #define RP_TILE 128              /* queries (forward, dQ) or keys (dK dV, table gradient) of a workgroup: four waves of 32 */
+#ifndef RP_UN_Q
+#define RP_UN_Q 2
+#define RP_UN_K 2
+#define RP_OQ 2
+#define RP_OK 2
+#define RP_OF 3
+#endif
 #define RP_PAD 4                 /* entries of w on either side, so that four consecutive differences need one clamp */
 #define RP_WMAX 4096
 #define RP_PE 14                 /* f16 planes hold P 2^14 */
@@ -232,7 +239,7 @@ __device__ __forceinline__ void rp_bias4(const float* w, int d0, int width, floa
 // keys along the registers, so the softmax of a row is register-local but for one exchange between lane halves, and P^T is the B operand of
 // O^T = V^T P^T as it stands.
 template <int DT, int DP, bool SPLIT>
-__global__ __launch_bounds__(RP_THREADS) void relpos_fwd_kernel(ofb_relpos_args a) {
+__global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 2)) void relpos_fwd_kernel(ofb_relpos_args a) {
   using G = rp_geo<DT, DP>;
   constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -321,8 +328,15 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_fwd_kernel(ofb_relpos_args 
           S[t] = rp_mm<DT, NP>(kf, qf[s], S[t]);
         }
       }
-      // scores in log2 units, with the bias
-      if (a.pos_k) {
+      // scores in log2 units with the bias: s = c_t S + bt, where beyond the table's ends (the whole tile has one bias) S stays as it is
+      const int dmax = j0 + KB - 1 - q0 - a.q_offset, dmin = j0 - (q0 + 31) - a.q_offset;
+      float bt = 0.f, c_t = 1.f;
+      const float wc = w[RP_PAD + (dmax <= lo ? 0 : width - 1)];
+      // (a bias that swallows the scores, and a scale that is not positive, take the general form)
+      if (!a.pos_k && (dmax <= lo || dmin >= hi) && fabsf(wc) < 1e30f && c_s > 0.f) {
+        bt = wc;
+        c_t = c_s;
+      } else if (a.pos_k) {
 #pragma unroll
         for (int t = 0; t < KB / 32; ++t)
 #pragma unroll
@@ -334,24 +348,15 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_fwd_kernel(ofb_relpos_args 
             S[t][r + 3] = fmaf(S[t][r + 3], c_s, w[rp_idx(pj.w - pq - lo, width)]);
           }
       } else {
-        const int dmax = j0 + KB - 1 - q0 - a.q_offset, dmin = j0 - (q0 + 31) - a.q_offset;
-        if (dmax <= lo || dmin >= hi) {                        // the whole tile lies beyond the first or the last difference
-          const float wc = w[RP_PAD + (dmax <= lo ? 0 : width - 1)];
 #pragma unroll
-          for (int t = 0; t < KB / 32; ++t)
+        for (int t = 0; t < KB / 32; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) S[t][r] = fmaf(S[t][r], c_s, wc);
-        } else {
+          for (int r = 0; r < 16; r += 4) {
+            float w4[4];
+            rp_bias4<1>(w, j0 + 32 * t + rp_row(r, hh) - pq - lo, width, w4);
 #pragma unroll
-          for (int t = 0; t < KB / 32; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-              float w4[4];
-              rp_bias4<1>(w, j0 + 32 * t + rp_row(r, hh) - pq - lo, width, w4);
-#pragma unroll
-              for (int u = 0; u < 4; ++u) S[t][r + u] = fmaf(S[t][r + u], c_s, w4[u]);
-            }
-        }
+            for (int u = 0; u < 4; ++u) S[t][r + u] = fmaf(S[t][r + u], c_s, w4[u]);
+          }
       }
       const bool whole = j0 + KB <= kend && (!a.causal || j0 + KB - 1 <= q0 + a.q_offset);
       if (!whole) {
@@ -367,7 +372,7 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_fwd_kernel(ofb_relpos_args 
 #pragma unroll
         for (int r = 0; r < 16; ++r) mb = fmaxf(mb, S[t][r]);
       OFB_XOR_STEP(mb, fmaxf, 32)
-      const float m_new = fmaxf(m, mb);
+      const float m_new = fmaxf(m, fmaf(mb, c_t, bt));
       if (__any(m_new > m)) {                                  // the running maximum moves rarely after the first tiles
         const float alpha = m_new > -INFINITY ? __builtin_amdgcn_exp2f(m - m_new) : 1.f;
         l *= alpha;
@@ -375,7 +380,7 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_fwd_kernel(ofb_relpos_args 
         for (int t = 0; t < DP / 32; ++t) O[t] *= alpha;
         m = m_new;
       }
-      const float mu = m > -INFINITY ? m : 0.f;                // a row that has seen nothing yet: exp2(-inf - 0) = 0
+      const float tb = bt - (m > -INFINITY ? m : 0.f);         // a row that has seen nothing yet: exp2(-inf - 0) = 0
 #pragma unroll
       for (int t = 0; t < KB / 32; ++t) {
 #pragma unroll
@@ -383,9 +388,9 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_fwd_kernel(ofb_relpos_args 
           float p8[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float p = __builtin_amdgcn_exp2f(S[t][8 * s + j] - mu);
+            const float p = __builtin_amdgcn_exp2f(fmaf(S[t][8 * s + j], c_t, tb));
             l += p;
-            p8[j] = p * p_sc;
+            p8[j] = DT == RP_BF16 ? p : p * p_sc;
           }
           rp_frag pf[NP];
           rp_pack8<DT>(p8, pf);
@@ -486,7 +491,7 @@ __device__ __forceinline__ rp_scales rp_all_scales(const ofb_relpos_args& a, flo
 // dQ, D, and the part of the table's gradient that lies beyond the last differences.  The forward's layout: 128 queries a workgroup, the
 // query on the lane; dS^T is the B operand of dQ^T = K^T dS^T from its registers.
 template <int DT, int DP>
-__global__ __launch_bounds__(RP_THREADS) void relpos_dq_kernel(ofb_relpos_args a) {
+__global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 || DT == RP_F32 ? 2 : RP_OQ)) void relpos_dq_kernel(ofb_relpos_args a) {
   using G = rp_geo<DT, DP>;
   constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -516,9 +521,9 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_dq_kernel(ofb_relpos_args a
   if (kb1 > 0) fetch(0);
   rp_bias_vector(a, head, w);
   const rp_scales e = rp_all_scales<DT>(a, red);
-  const float hq = ofb_h_pow2(e.eq), hk = ofb_h_pow2(e.ek), hv = ofb_h_pow2(e.ev), hd = ofb_h_pow2(e.ed), hs = ofb_h_pow2(e.es);
+  const float hq = ofb_h_pow2(e.eq), hk = ofb_h_pow2(e.ek), hv = ofb_h_pow2(e.ev), hd = ofb_h_pow2(e.ed);
   const float c_s = a.scale * 1.44269504088896340736f * ofb_h_pow2(-e.eq) * ofb_h_pow2(-e.ek);
-  const float c_dp = ofb_h_pow2(-e.ed) * ofb_h_pow2(-e.ev);
+  const int ek_ = e.es - e.ed - e.ev;                          // dP's accumulators times 2^ek_ are in dS's scale
   const float c_dq = a.scale * ofb_h_pow2(-e.es) * ofb_h_pow2(-e.ek);
 
   const int q0 = qt * RP_TILE + wv * 32, qi = q0 + (lane & 31);
@@ -548,6 +553,10 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_dq_kernel(ofb_relpos_args a
     m = a.stats[2 * row];
     linv = a.stats[2 * row + 1];
   }
+  // P 2^ek_ = exp2(s - mk) lk; a row without keys has 1 / sum = 0
+  const float mk = NP == 2 ? m : linv > 0.f ? m - __log2f(linv) - (float)ek_ : linv == 0.f ? INFINITY : linv;
+  const float lk = NP == 2 ? __builtin_ldexpf(linv, ek_) : 1.f;
+  const float nD = -__builtin_ldexpf(D, e.ed + e.ev);
   f32x16 dQ[DP / 32];
 #pragma unroll
   for (int t = 0; t < DP / 32; ++t) dQ[t] = rp_zero16();
@@ -565,83 +574,95 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_dq_kernel(ofb_relpos_args a
     const char* kt_ = tiles + buf * G::STAGE;
     const char* vt_ = kt_ + G::TENSOR;
     if (kb + 1 < kb1) fetch(kb + 1);
-#pragma unroll
-    for (int t = 0; t < KB / 32; ++t) {
-      const int j0 = kb * KB + 32 * t;
+#pragma unroll RP_UN_Q
+    for (int t0 = 0; t0 < KB / 32; ++t0) {
+      const int j0 = kb * KB + 32 * t0;
       if (!active || j0 >= kend || (a.causal && j0 > q0 + 31 + a.q_offset)) continue;
-      f32x16 S = rp_zero16(), dP = rp_zero16();
+      f32x16 S = rp_zero16(), dP;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dP[r] = nD;                 // dP - D, in dP's scale
 #pragma unroll
       for (int s = 0; s < DP / 16; ++s) {
         rp_frag kf[NP], vf[NP];
-        rp_rows<DT, DP>(kt_, 32 * t, s, lane, kf);
-        rp_rows<DT, DP>(vt_, 32 * t, s, lane, vf);
+        rp_rows<DT, DP>(kt_, 32 * t0, s, lane, kf);
+        rp_rows<DT, DP>(vt_, 32 * t0, s, lane, vf);
         S = rp_mm<DT, NP>(kf, qf[s], S);
         dP = rp_mm<DT, NP>(vf, df[s], dP);
       }
+      // ds: dS in units of 1 / k, k = the power of two that makes it the second product's operand (dP's own scale is in it too).  P's maximum and
+      // sum are one exponent (bf16, f16) or, for f32, the maximum and a factor: the rounding of a logarithm of the size of 10 would show.
       const bool whole = j0 + 32 <= kend && (!a.causal || j0 + 31 <= q0 + a.q_offset);
       const int dmax = j0 + 31 - q0 - a.q_offset, dmin = j0 - (q0 + 31) - a.q_offset;
-      const bool far = !a.pos_k && (dmax <= lo || dmin >= hi);
-      const float wc = far ? w[RP_PAD + (dmax <= lo ? 0 : width - 1)] : 0.f;
-      float ds[16], ps[16];
+      float ds[16], sum = 0.f;
+      if (whole && !a.pos_k && (dmax <= lo || dmin >= hi)) {
+        const float tb = w[RP_PAD + (dmax <= lo ? 0 : width - 1)] - mk;
+        float psum = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int jr = j0 + rp_row(r, hh);
-        float w4[4];
-        if (far) {
+        for (int r = 0; r < 16; ++r) {
+          float p = __builtin_amdgcn_exp2f(fmaf(S[r], c_s, tb));
+          if constexpr (NP == 2) p *= lk;
+          ds[r] = p * dP[r];
+          sum += ds[r];
+          psum += p;
+        }
+        if (dmax <= lo) { sat_lo += sum; pat_lo += psum; } else { sat_hi += sum; pat_hi += psum; }
+      } else {
+        float t[16];
+        if (a.pos_k) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) w4[u] = wc;
-        } else if (a.pos_k) {
-          const int4 pj = *reinterpret_cast<const int4*>(&pk[buf * KB + 32 * t + rp_row(r, hh)]);
-          w4[0] = w[rp_idx(pj.x - pq - lo, width)];
-          w4[1] = w[rp_idx(pj.y - pq - lo, width)];
-          w4[2] = w[rp_idx(pj.z - pq - lo, width)];
-          w4[3] = w[rp_idx(pj.w - pq - lo, width)];
+          for (int r = 0; r < 16; r += 4) {
+            const int4 pj = *reinterpret_cast<const int4*>(&pk[buf * KB + 32 * t0 + rp_row(r, hh)]);
+            t[r] = w[rp_idx(pj.x - pq - lo, width)];
+            t[r + 1] = w[rp_idx(pj.y - pq - lo, width)];
+            t[r + 2] = w[rp_idx(pj.z - pq - lo, width)];
+            t[r + 3] = w[rp_idx(pj.w - pq - lo, width)];
+          }
         } else {
-          rp_bias4<1>(w, jr - pq - lo, width, w4);
+#pragma unroll
+          for (int r = 0; r < 16; r += 4) {
+            float w4[4];
+            rp_bias4<1>(w, j0 + rp_row(r, hh) - pq - lo, width, w4);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) t[r + u] = w4[u];
+          }
         }
+        if (!whole) {                                          // keys this query does not see: P = 0, whatever S and dP are there
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          float p = __builtin_amdgcn_exp2f(fmaf(S[r + u], c_s, w4[u]) - m) * linv;
-          if (!whole && jr + u >= seen) p = 0.f;
-          float x = p * (fmaf(dP[r + u], c_dp, -D));
-          if (!whole && jr + u >= seen) x = 0.f;               // (0 times a non-finite dP)
-          ds[r + u] = x;
-          ps[r + u] = p;
+          for (int r = 0; r < 16; ++r)
+            if (j0 + rp_row(r, hh) >= seen) { t[r] = -INFINITY; S[r] = dP[r] = 0.f; }
         }
-      }
-      float sum = 0.f;
+        float p[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sum += ds[r];
-      left += sum;
-      if (!a.pos_k && a.sat) {
-        if (far) {
-          float psum = 0.f;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) psum += ps[r];
-          if (dmax <= lo) { sat_lo += sum; pat_lo += psum; } else { sat_hi += sum; pat_hi += psum; }
-        } else if (dmin <= lo || dmax >= hi) {
+        for (int r = 0; r < 16; ++r) {
+          p[r] = __builtin_amdgcn_exp2f(fmaf(S[r], c_s, t[r]) - mk);
+          if constexpr (NP == 2) p[r] *= lk;
+          ds[r] = p[r] * dP[r];
+          sum += ds[r];
+        }
+        if (!a.pos_k && (dmin <= lo || dmax >= hi)) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int diff = j0 + rp_row(r, hh) - pq;
             const bool below = diff <= lo, above = diff >= hi && diff > lo;
             sat_lo += below ? ds[r] : 0.f;
-            pat_lo += below ? ps[r] : 0.f;
+            pat_lo += below ? p[r] : 0.f;
             sat_hi += above ? ds[r] : 0.f;
-            pat_hi += above ? ps[r] : 0.f;
+            pat_hi += above ? p[r] : 0.f;
           }
         }
       }
+      left += sum;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         float x8[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x8[j] = ds[8 * s + j] * hs;
+        for (int j = 0; j < 8; ++j) x8[j] = ds[8 * s + j];
         rp_frag xf[NP];
         rp_pack8<DT>(x8, xf);
 #pragma unroll
         for (int ct = 0; ct < DP / 32; ++ct) {
           rp_frag kf[NP];
-          rp_cols<DT, DP>(kt_, 32 * t + 16 * s, ct, lane, kf);
+          rp_cols<DT, DP>(kt_, 32 * t0 + 16 * s, ct, lane, kf);
           dQ[ct] = rp_mm<DT, NP>(kf, xf, dQ[ct]);
         }
       }
@@ -653,6 +674,11 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_dq_kernel(ofb_relpos_args a
   // kernels that follow read D without it, and the sums above lose it times their share of P.  (The table's gradient is f32 and sums whole rows'
   // parts, where an error that a row's terms share does not average out: without this it was 1e-3 off for bf16.)
   OFB_XOR_STEP(left, ofb_add_, 32)
+  sat_lo = __builtin_ldexpf(sat_lo, -e.es);
+  sat_hi = __builtin_ldexpf(sat_hi, -e.es);
+  pat_lo = __builtin_ldexpf(pat_lo, -ek_);
+  pat_hi = __builtin_ldexpf(pat_hi, -ek_);
+  left = __builtin_ldexpf(left, -e.es);
   if (qok && hh == 0) a.delta[(int64_t)bh * a.Nq + qi] = D + left;
   sat_lo -= left * pat_lo;
   sat_hi -= left * pat_hi;
@@ -677,30 +703,40 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_dq_kernel(ofb_relpos_args a
     }
 }
 
-// a query tile's row statistics in LDS: max, 1 / sum, D, position - each a vector of KB
-template <int KB>
-__device__ __forceinline__ void rp_row_stats(const ofb_relpos_args& a, int64_t bh, int row0, f32x4& v, int& pos) {
+// a query tile's row statistics for LDS: the maximum (with the sum's logarithm and the operand's scale 2^pe in it, or for f32 apart), the factor,
+// -D in dP's scale 2^de; a row without keys or behind the last query gets P = 0
+template <int DT, int KB>
+__device__ __forceinline__ void rp_row_stats(const ofb_relpos_args& a, int64_t bh, int row0, int pe, int de, f32x4& v, int& pos) {
   const int i = row0 + threadIdx.x;
-  v = f32x4{0.f, 0.f, 0.f, 0.f};
+  v = f32x4{DT == RP_F32 ? 0.f : INFINITY, 0.f, 0.f, 0.f};
   pos = 0;
   if (threadIdx.x < KB && i < a.Nq) {
     const int64_t row = bh * a.Nq + i;
-    v[0] = a.stats[2 * row];
-    v[1] = a.stats[2 * row + 1];
-    v[2] = a.delta[row];
+    const float m = a.stats[2 * row], l = a.stats[2 * row + 1];
+    if constexpr (DT == RP_F32) { v[0] = m; v[1] = __builtin_ldexpf(l, pe); }
+    else v[0] = l > 0.f ? m - __log2f(l) - (float)pe : l == 0.f ? INFINITY : l;
+    v[2] = -__builtin_ldexpf(a.delta[row], de);
     pos = a.pos_q ? a.pos_q[i] : i + a.q_offset;
   }
 }
 
-// P and dS of a 32 x 32 tile, rows = queries i0 .. (LDS tiles qt_ and dt_ at row tr), the wave's key on the lane
+// P and dS of a 32 x 32 tile, rows = queries i0 .. (LDS tiles qt_ and dt_ at row tr), the wave's key on the lane.  st: row statistics m, l, -D of
+// the tile's queries, P = exp2(s - m) (times l for f32; l is in m otherwise), -D in dP's scale.  P comes out times the p_sc that is in the statistics,
+// dS = P dP times that and dP's scale.
 template <int DT, int DP>
 __device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char* qt_, const char* dt_, int tr, const rp_frag (&kf)[DP / 16][rp_type<DT>::NP],
                                            const rp_frag (&vf)[DP / 16][rp_type<DT>::NP], const float* st, const int* ps, const float* w, int i0, int j0,
-                                           int kj, int pkj, bool kok, float c_s, float c_dp, float (&P)[16], float (&dS)[16]) {
+                                           int kj, int pkj, bool kok, bool kwhole, float c_s, float (&P)[16], float (&dS)[16]) {
   using G = rp_geo<DT, DP>;
   constexpr int NP = G::NP, KB = G::KB;
   const int lane = threadIdx.x & 63, hh = lane >> 5, lo = a.lo, width = a.width, hi = lo + width - 1;
-  f32x16 S = rp_zero16(), dP = rp_zero16();
+  f32x16 S = rp_zero16(), dP;
+#pragma unroll
+  for (int r = 0; r < 16; r += 4) {
+    const f32x4 d4 = *reinterpret_cast<const f32x4*>(&st[2 * KB + tr + rp_row(r, hh)]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) dP[r + u] = d4[u];
+  }
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
     rp_frag qa[NP], da[NP];
@@ -710,34 +746,46 @@ __device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char*
     dP = rp_mm<DT, NP>(da, vf[s], dP);
   }
   const int dmax = j0 + 31 - i0 - a.q_offset, dmin = j0 - (i0 + 31) - a.q_offset;
-  const bool far = !a.pos_q && (dmax <= lo || dmin >= hi);
-  const float wc = far ? w[RP_PAD + (dmax <= lo ? 0 : width - 1)] : 0.f;
   const bool cut = a.causal && j0 + 31 > i0 + a.q_offset;
+  float t[16];
+  if (!a.pos_q && (dmax <= lo || dmin >= hi)) {
+    const float wc = w[RP_PAD + (dmax <= lo ? 0 : width - 1)];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t[r] = wc;
+  } else if (a.pos_q) {
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int4 pi = *reinterpret_cast<const int4*>(&ps[tr + rp_row(r, hh)]);
+      t[r] = w[rp_idx(pkj - pi.x - lo, width)];
+      t[r + 1] = w[rp_idx(pkj - pi.y - lo, width)];
+      t[r + 2] = w[rp_idx(pkj - pi.z - lo, width)];
+      t[r + 3] = w[rp_idx(pkj - pi.w - lo, width)];
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      float w4[4];
+      rp_bias4<-1>(w, kj - (i0 + rp_row(r, hh) + a.q_offset) - lo, width, w4);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) t[r + u] = w4[u];
+    }
+  }
+  if (!kwhole || cut) {                                        // queries that do not see this key: P = 0, whatever S and dP are there
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (!kok || (cut && kj > i0 + rp_row(r, hh) + a.q_offset)) { t[r] = -INFINITY; S[r] = dP[r] = 0.f; }
+  }
 #pragma unroll
   for (int r = 0; r < 16; r += 4) {
     const int rr = rp_row(r, hh);
-    const f32x4 m4 = *reinterpret_cast<const f32x4*>(&st[tr + rr]), l4 = *reinterpret_cast<const f32x4*>(&st[KB + tr + rr]),
-                d4 = *reinterpret_cast<const f32x4*>(&st[2 * KB + tr + rr]);
-    float w4[4];
-    if (far) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) w4[u] = wc;
-    } else if (a.pos_q) {
-      const int4 pi = *reinterpret_cast<const int4*>(&ps[tr + rr]);
-      w4[0] = w[rp_idx(pkj - pi.x - lo, width)];
-      w4[1] = w[rp_idx(pkj - pi.y - lo, width)];
-      w4[2] = w[rp_idx(pkj - pi.z - lo, width)];
-      w4[3] = w[rp_idx(pkj - pi.w - lo, width)];
-    } else {
-      rp_bias4<-1>(w, kj - (i0 + rr + a.q_offset) - lo, width, w4);
-    }
+    const f32x4 m4 = *reinterpret_cast<const f32x4*>(&st[tr + rr]);
+    f32x4 l4 = {1.f, 1.f, 1.f, 1.f};
+    if constexpr (NP == 2) l4 = *reinterpret_cast<const f32x4*>(&st[KB + tr + rr]);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      float p = __builtin_amdgcn_exp2f(fmaf(S[r + u], c_s, w4[u]) - m4[u]) * l4[u];
-      float x = p * fmaf(dP[r + u], c_dp, -d4[u]);
-      if (!kok || (cut && kj > i0 + rr + u + a.q_offset)) p = x = 0.f;
-      P[r + u] = p;
-      dS[r + u] = x;
+      P[r + u] = __builtin_amdgcn_exp2f(fmaf(S[r + u], c_s, t[r + u] - m4[u]));
+      if constexpr (NP == 2) P[r + u] *= l4[u];
+      dS[r + u] = P[r + u] * dP[r + u];
     }
   }
 }
@@ -745,7 +793,7 @@ __device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char*
 // dK and dV: a workgroup owns 128 keys of one head (a wave 32, key on the lane, K and V in registers), queries stream through LDS.
 // S = Q K^T and dP = dO V^T have queries along the registers: P and dS are the B operands of dV^T = dO^T P and dK^T = Q^T dS.
 template <int DT, int DP>
-__global__ __launch_bounds__(RP_THREADS) void relpos_dkv_kernel(ofb_relpos_args a) {
+__global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OK : 1)) void relpos_dkv_kernel(ofb_relpos_args a) {
   using G = rp_geo<DT, DP>;
   constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -766,22 +814,21 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_dkv_kernel(ofb_relpos_args 
   int qb0 = 0, qb1 = (a.Nq + KB - 1) / KB;
   if (a.causal) qb0 = min(qb1, max(0, j_first - a.q_offset) / KB);
   if (j_first >= kend) qb0 = qb1;                              // nobody sees these keys: their gradients are zeros
+  const rp_scales e = rp_all_scales<DT>(a, red);
   rp_stage<DT, DP> qs_, ds_;
   f32x4 st_next;
   int ps_next;
   auto fetch = [&](int qb) {
     qs_.load(qp, a.q_st * ES, qb * KB, a.Nq, a.d);
     ds_.load(dp, a.do_st * ES, qb * KB, a.Nq, a.d);
-    rp_row_stats<KB>(a, bh, qb * KB, st_next, ps_next);
+    rp_row_stats<DT, KB>(a, bh, qb * KB, DT == RP_BF16 ? 0 : RP_PE, e.ed + e.ev, st_next, ps_next);
   };
-  if (qb0 < qb1) fetch(qb0);
   rp_bias_vector(a, head, w);
-  const rp_scales e = rp_all_scales<DT>(a, red);
-  const float hq = ofb_h_pow2(e.eq), hk = ofb_h_pow2(e.ek), hv = ofb_h_pow2(e.ev), hd = ofb_h_pow2(e.ed), hs = ofb_h_pow2(e.es);
+  if (qb0 < qb1) fetch(qb0);
+  const float hq = ofb_h_pow2(e.eq), hk = ofb_h_pow2(e.ek), hv = ofb_h_pow2(e.ev), hd = ofb_h_pow2(e.ed);
   const float c_s = a.scale * 1.44269504088896340736f * ofb_h_pow2(-e.eq) * ofb_h_pow2(-e.ek);
-  const float c_dp = ofb_h_pow2(-e.ed) * ofb_h_pow2(-e.ev);
+  const float c_x = DT == RP_BF16 ? 1.f : ofb_h_pow2(e.es - e.ed - e.ev - RP_PE);      // dS from rp_tile_ds to the operand's scale
   const float c_dk = a.scale * ofb_h_pow2(-e.es) * ofb_h_pow2(-e.eq);
-  const float p_sc = DT == RP_BF16 ? 1.f : ofb_h_pow2(RP_PE);
   const float c_dv = DT == RP_BF16 ? 1.f : ofb_h_pow2(-RP_PE) * ofb_h_pow2(-e.ed);
 
   const int j0 = j_first + wv * 32, kj = j0 + (lane & 31);
@@ -818,17 +865,17 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_dkv_kernel(ofb_relpos_args 
     const char* qt_ = tiles + buf * G::STAGE;
     const char* dt_ = qt_ + G::TENSOR;
     if (qb + 1 < qb1) fetch(qb + 1);
-#pragma unroll
+#pragma unroll RP_UN_K
     for (int t = 0; t < KB / 32; ++t) {
       const int i0 = qb * KB + 32 * t;
       if (!active || i0 >= a.Nq || (a.causal && j0 > i0 + 31 + a.q_offset)) continue;
       float P[16], dS[16];
-      rp_tile_ds<DT, DP>(a, qt_, dt_, 32 * t, kf, vf, st + buf * 3 * KB, ps + buf * KB, w, i0, j0, kj, pkj, kok, c_s, c_dp, P, dS);
+      rp_tile_ds<DT, DP>(a, qt_, dt_, 32 * t, kf, vf, st + buf * 3 * KB, ps + buf * KB, w, i0, j0, kj, pkj, kok, j0 + 32 <= kend, c_s, P, dS);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         float p8[8], x8[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { p8[j] = P[8 * s + j] * p_sc; x8[j] = dS[8 * s + j] * hs; }
+        for (int j = 0; j < 8; ++j) { p8[j] = P[8 * s + j]; x8[j] = DT == RP_BF16 ? dS[8 * s + j] : dS[8 * s + j] * c_x; }
         rp_frag pf[NP], xf[NP];
         rp_pack8<DT>(p8, pf);
         rp_pack8<DT>(x8, xf);
@@ -865,7 +912,7 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_dkv_kernel(ofb_relpos_args 
 // difference in LDS: whole numbers of 2^-40 of the tile's largest |dS|, so that the order of the additions does not matter.  Without
 // position arrays only the tiles with differences strictly between the first and the last are visited (relpos_dq_kernel sums the rest).
 template <int DT, int DP>
-__global__ __launch_bounds__(RP_THREADS) void relpos_dbias_kernel(ofb_relpos_args a, int chunks) {
+__global__ __launch_bounds__(RP_THREADS, (DT == RP_F32 ? 1 : DP <= 64 ? 2 : 3)) void relpos_dbias_kernel(ofb_relpos_args a, int chunks) {
   using G = rp_geo<DT, DP>;
   constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -886,7 +933,7 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_dbias_kernel(ofb_relpos_arg
   const rp_scales e = rp_all_scales<DT>(a, red);
   const float hq = ofb_h_pow2(e.eq), hk = ofb_h_pow2(e.ek), hv = ofb_h_pow2(e.ev), hd = ofb_h_pow2(e.ed);
   const float c_s = a.scale * 1.44269504088896340736f * ofb_h_pow2(-e.eq) * ofb_h_pow2(-e.ek);
-  const float c_dp = ofb_h_pow2(-e.ed) * ofb_h_pow2(-e.ev);
+  const float c_x = ofb_h_pow2(-e.ed) * ofb_h_pow2(-e.ev);
   const int i_first = qt * KB, i_last = min(a.Nq, i_first + KB) - 1, lo = a.lo, width = a.width, hi = lo + width - 1;
   int kt0 = 0, kt1 = (a.Nk + RP_TILE - 1) / RP_TILE;
   if (!a.pos_k) {                                              // keys with lo < j - (i + q_offset) < hi for some query of the tile
@@ -912,7 +959,7 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_dbias_kernel(ofb_relpos_arg
       int ps_next;
       qs_.load((const char*)a.q + (b * a.q_sb + head * a.q_sh) * ES, a.q_st * ES, i_first, a.Nq, a.d);
       ds_.load((const char*)a.dout + (b * a.do_sb + head * a.do_sh) * ES, a.do_st * ES, i_first, a.Nq, a.d);
-      rp_row_stats<KB>(a, (int64_t)b * a.H + head, i_first, st_next, ps_next);
+      rp_row_stats<DT, KB>(a, (int64_t)b * a.H + head, i_first, 0, e.ed + e.ev, st_next, ps_next);
       const char* kp = (const char*)a.k + (b * a.k_sb + head * a.k_sh) * ES;
       const char* vp = (const char*)a.v + (b * a.v_sb + head * a.v_sh) * ES;
       const bool kok = kj < kend;
@@ -942,9 +989,9 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_dbias_kernel(ofb_relpos_arg
         const int i0 = i_first + 32 * t;
         if (j0 >= kend || i0 >= a.Nq || (a.causal && j0 > i0 + 31 + a.q_offset)) continue;
         float P[16], dS[16];
-        rp_tile_ds<DT, DP>(a, tiles, tiles + G::TENSOR, 32 * t, kf, vf, st, ps, w, i0, j0, kj, pkj, kok, c_s, c_dp, P, dS);
+        rp_tile_ds<DT, DP>(a, tiles, tiles + G::TENSOR, 32 * t, kf, vf, st, ps, w, i0, j0, kj, pkj, kok, j0 + 32 <= kend, c_s, P, dS);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sum[t][r] += dS[r];
+        for (int r = 0; r < 16; ++r) sum[t][r] += DT == RP_F32 ? dS[r] * c_x : dS[r];
       }
     }
     float mx = 0.f;
