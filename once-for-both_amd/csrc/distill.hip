@@ -23,6 +23,7 @@
 #define DS_STATS 8                /* floats kept per row: m_t, kappa, m, 1/s, m_teacher, 1/s_teacher, used, 0 */
 #define TL_CAP 4096               /* candidates of a row or segment that are ranked at once */
 #define TL_THREADS 1024
+#define TL_SMALL 256              /* threads for lists of up to TL_SMALL / 2: 1024 x 100003 bf16, 64 kept: 90 us, 512 threads 103 us, 1024 threads 99 us */
 
 namespace {
 
@@ -69,9 +70,12 @@ struct ds_row {
       else x[i] = (i & 1) ? ofb_f16_hi(w[i >> 1]) : ofb_f16_lo(w[i >> 1]);
     }
   }
-  // runs f(chunk, values) over chunks c0 + thread, c0 + thread + THREADS, ...: `fill` stands where a chunk has no class.  Four chunks are loaded
-  // before the first is used (only the row's first and last chunk can be partial: they are left to the end).
-  template <int THREADS, typename F>
+  // runs f(chunk, values) over chunks c0 + thread, c0 + thread + THREADS, ...: `fill` stands where a chunk has no class.  Four chunks at a time
+  // are loaded and handed over as one array (element i is of chunk + i / CH * THREADS): loads in flight, and one rescaling of a running sum for
+  // all of them (2048 x 100003 bf16, forward of the loss: 158 us a chunk at a time, 135 us with four loads in flight, 130 us like this).  Not
+  // TOGETHER: one chunk after the other, four loads in flight all the same (the backward, whose results would take the registers of a second
+  // workgroup: 163 against 171 us).  Only the row's first and last chunk can be partial: they are left to the end.
+  template <int THREADS, bool TOGETHER = true, typename F>
   __device__ __forceinline__ void each(int c0, int c1, float fill, F f) const {
     constexpr int CH = ds_type<DT>::CH;
     int a0 = c0, a1 = c1;
@@ -82,11 +86,18 @@ struct ds_row {
       uint4 v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = fetch(c + j * THREADS);
+      if constexpr (TOGETHER) {
+        float x[4 * CH];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float x[CH];
-        unpack(v[j], x);
-        f(c + j * THREADS, x);
+        for (int j = 0; j < 4; ++j) unpack(v[j], *reinterpret_cast<float(*)[CH]>(x + j * CH));
+        f(c, x);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float x[CH];
+          unpack(v[j], x);
+          f(c + j * THREADS, x);
+        }
       }
     }
     for (; c < a1; c += THREADS) {
@@ -142,17 +153,6 @@ __device__ __forceinline__ double ds_wave_sum(double v) {
   return v;
 }
 // workgroup reductions; every thread gets the result (red: one word per wave, free before and after)
-template <int THREADS>
-__device__ __forceinline__ float ds_max(float v, float* red) {
-  v = ofb_wave_max(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = red[0];
-#pragma unroll
-  for (int i = 1; i < THREADS / 64; ++i) v = fmaxf(v, red[i]);
-  return v;
-}
 template <int THREADS>
 __device__ __forceinline__ double ds_total(double v, double* red) {
   v = ds_wave_sum(v);
@@ -218,68 +218,70 @@ __device__ __forceinline__ bool ds_first(const int* cls, int k, int i) {
   return first;
 }
 
-// The row's loss and what the backward needs, from (m_t, s_t) of the classes that are not stored.  The sums over the stored classes are in
-// 64 bits: the loss is a difference of logarithms of the size of log V.
+// a row's entries in LDS: class (or -1), stored value, the student's logit, and the same or -inf where an earlier entry has the class (the first
+// stands for it in sums over the classes)
+struct ds_entries {
+  int* cls;
+  float *t, *y, *own;
+  __device__ __forceinline__ ds_entries(int* at, int K) : cls(at), t((float*)at + ((K + 3) & ~3)), y(t + ((K + 3) & ~3)), own(y + ((K + 3) & ~3)) {}
+  static constexpr int words(int K) { return 4 * ((K + 3) & ~3); }
+};
 template <int DT>
-__device__ void ds_finish(const ds_args& a, int64_t row, ds_sum tail, int* cls, double* redd, float* redf) {
-  constexpr int PER = DS_KMAX / DS_THREADS;
-  float t[PER], y[PER];
-  bool own[PER];
+__device__ __forceinline__ int ds_load_entries(const ds_args& a, int64_t row, ds_entries e) {      // -> how many classes there are
   for (int k = threadIdx.x; k < ((a.K + 3) & ~3); k += DS_THREADS) {
     float v = 0.f;
-    cls[k] = k < a.K ? ds_class<DT>(a, row, k, v) : -1;
+    const int i = k < a.K ? ds_class<DT>(a, row, k, v) : -1;
+    e.cls[k] = i;
+    e.t[k] = v;
+    e.y[k] = i < 0 ? 0.f : ds_value<DT>(((const typename ds_type<DT>::raw*)a.z)[row * a.V + i]);
   }
   __syncthreads();
-  float mt = -INFINITY, m = tail.m;
-  int mine = 0, any = 0;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int k = threadIdx.x + DS_THREADS * j;
-    own[j] = false;
-    t[j] = y[j] = 0.f;
-    if (k >= a.K || cls[k] < 0) continue;
-    float v;
-    const int i = ds_class<DT>(a, row, k, v);
-    t[j] = v;
-    y[j] = ds_value<DT>(((const typename ds_type<DT>::raw*)a.z)[row * a.V + i]);
-    own[j] = ds_first(cls, k, i);                              // the first entry of a class stands for it in the sum over the classes
-    mt = fmaxf(mt, v * a.c);
-    m = fmaxf(m, y[j] * a.c);
-    mine += own[j];
-    any = 1;
+  int classes = 0;
+  for (int k0 = 0; k0 < a.K; k0 += DS_THREADS) {
+    const int k = k0 + threadIdx.x;
+    const bool first = k < a.K && e.cls[k] >= 0 && ds_first(e.cls, k, e.cls[k]);
+    if (k < a.K) e.own[k] = first ? e.y[k] : -INFINITY;
+    classes += __syncthreads_count(first);
   }
-  const double stored = ds_total<DS_THREADS>((double)mine, redd);
-  any = __syncthreads_or(any);
-  const bool all = stored >= (double)a.V;                      // every class is stored: there is no rest
+  return classes;
+}
+
+// The row's loss and what the backward needs, from (m_t, s_t) of the classes that are not stored: one wave (the other waves of the workgroup are
+// done, and nothing waits for a barrier).  The sums over the stored classes are in 64 bits: the loss is a difference of logarithms of the size of log V.
+__device__ void ds_finish(const ds_args& a, int64_t row, ds_sum tail, ds_entries e, int classes) {
+  const int lane = threadIdx.x & 63;
+  float mt = -INFINITY, m = tail.m;
+  for (int k = lane; k < a.K; k += 64) {
+    if (e.cls[k] < 0) continue;
+    mt = fmaxf(mt, e.t[k] * a.c);
+    m = fmaxf(m, e.y[k] * a.c);
+  }
+  mt = ofb_wave_max(mt);
+  m = ofb_wave_max(m);
+  const bool any = classes > 0, all = classes >= a.V;                              // every class is stored: there is no rest
   const float r2 = (a.rest && !all) ? a.rest[row] * 1.44269504088896340736f : -INFINITY;
-  mt = fmaxf(ds_max<DS_THREADS>(mt, redf), r2);
-  m = ds_max<DS_THREADS>(m, redf);
+  mt = fmaxf(mt, r2);
   const float mtu = mt > -INFINITY ? mt : 0.f, mu = m > -INFINITY ? m : 0.f;
   double st = 0.0, s = 0.0;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int k = threadIdx.x + DS_THREADS * j;
-    if (k >= a.K || cls[k] < 0) continue;
-    st += (double)__builtin_amdgcn_exp2f(fmaf(t[j], a.c, -mtu));
-    if (own[j]) s += (double)__builtin_amdgcn_exp2f(fmaf(y[j], a.c, -mu));
+  for (int k = lane; k < a.K; k += 64) {
+    if (e.cls[k] < 0) continue;
+    st += (double)__builtin_amdgcn_exp2f(fmaf(e.t[k], a.c, -mtu));
+    s += (double)__builtin_amdgcn_exp2f(fmaf(e.own[k], a.c, -mu));
   }
   const float er = __builtin_amdgcn_exp2f(r2 - mtu), et = tail.s > 0.f ? tail.s * __builtin_amdgcn_exp2f(tail.m - mu) : tail.s;
-  st = ds_total<DS_THREADS>(st, redd) + (double)er;
-  s = ds_total<DS_THREADS>(s, redd) + (double)et;
+  st = ds_wave_sum(st) + (double)er;
+  s = ds_wave_sum(s) + (double)et;
   const double L2 = (double)mtu + log2(st), A2 = (double)mu + log2(s), ci = 1.0 / st;
   double loss = 0.0;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int k = threadIdx.x + DS_THREADS * j;
-    if (k >= a.K || cls[k] < 0) continue;
-    const double p = (double)__builtin_amdgcn_exp2f(fmaf(t[j], a.c, -mtu)) * ci;
-    loss += p * ((double)t[j] * (double)a.c - L2 - (double)y[j] * (double)a.c + A2);
+  for (int k = lane; k < a.K; k += 64) {
+    if (e.cls[k] < 0) continue;
+    const double p = (double)__builtin_amdgcn_exp2f(fmaf(e.t[k], a.c, -mtu)) * ci;
+    loss += p * ((double)e.t[k] * (double)a.c - L2 - (double)e.y[k] * (double)a.c + A2);
   }
-  loss = ds_total<DS_THREADS>(loss, redd);
-  const bool used = any || r2 > -INFINITY;
+  loss = ds_wave_sum(loss);
   const double pr = (double)er * ci;
   if (pr > 0.0) loss += pr * ((double)r2 - L2 - ((double)tail.m + log2((double)tail.s) - A2));
-  if (threadIdx.x == 0) {
+  if (lane == 0) {
     float* o = a.stats + row * DS_STATS;
     o[0] = tail.m > -INFINITY ? tail.m : 0.f;
     o[1] = tail.s == 0.f ? 0.f : (float)(((double)et / s - pr) / (double)tail.s);
@@ -287,47 +289,54 @@ __device__ void ds_finish(const ds_args& a, int64_t row, ds_sum tail, int* cls, 
     o[3] = (float)(1.0 / s);
     o[4] = mtu;
     o[5] = (float)ci;
-    o[6] = (any && used) ? 1.f : 0.f;
+    o[6] = any ? 1.f : 0.f;
     o[7] = 0.f;
-    a.row_loss[row] = (any && used) ? (float)(loss * 0.69314718055994530942 * (double)a.tau * (double)a.tau) : 0.f;
+    a.row_loss[row] = any ? (float)(loss * 0.69314718055994530942 * (double)a.tau * (double)a.tau) : 0.f;
   }
 }
 
 template <int DT, bool WHOLE>      // WHOLE: one segment a row, which also finishes it
 __global__ __launch_bounds__(DS_THREADS) void distill_fwd_kernel(ds_args a) {
   constexpr int CH = ds_type<DT>::CH;
-  // a bit per class of the segment, and the entries' classes: as much LDS as they take, so that eight workgroups share a CU
-  extern __shared__ __attribute__((aligned(16))) int cls[];
-  unsigned* bits = reinterpret_cast<unsigned*>(cls + ((a.K + 3) & ~3));
-  __shared__ double redd[4];
+  // a bit per class of the segment and the entries: as much LDS as they take, so that eight workgroups share a CU
+  extern __shared__ __attribute__((aligned(16))) int lds[];
+  const ds_entries e(lds, a.K);
+  unsigned* bits = reinterpret_cast<unsigned*>(lds + ds_entries::words(a.K));
   __shared__ float redf[8];
   const int64_t row = blockIdx.x / a.segs;
   const int seg = blockIdx.x % a.segs;
   const ds_row<DT> r(a.z, row, a.V);
   const int nc = r.chunks(), per = (nc + a.segs - 1) / a.segs, c0 = min(nc, seg * per), c1 = min(nc, c0 + per);
   for (int i = threadIdx.x; i < (c1 - c0) * CH / 32 + 1; i += DS_THREADS) bits[i] = 0u;
+  int classes = 0;
+  if constexpr (WHOLE) classes = ds_load_entries<DT>(a, row, e);
   __syncthreads();
   for (int k = threadIdx.x; k < a.K; k += DS_THREADS) {
     float v;
-    const int i = ds_class<DT>(a, row, k, v);
-    const int u = i + r.mis - c0 * CH;
+    const int i = WHOLE ? e.cls[k] : ds_class<DT>(a, row, k, v), u = i + r.mis - c0 * CH;
     if (i >= 0 && u >= 0 && u < (c1 - c0) * CH) atomicOr(&bits[u >> 5], 1u << (u & 31));
   }
   __syncthreads();
   ds_sum sum;
-  r.template each<DS_THREADS>(c0, c1, -INFINITY, [&](int c, float (&x)[CH]) {
-    const int u = (c - c0) * CH;
-    const unsigned b = (bits[u >> 5] >> (u & 31)) & ((1u << CH) - 1u);
-    if (b) {
+  r.template each<DS_THREADS>(c0, c1, -INFINITY, [&](int c, auto& x) {
+    constexpr int N = sizeof(x) / 4, B = N / CH;
+    unsigned b[B], any = 0u;
 #pragma unroll
-      for (int i = 0; i < CH; ++i)
-        if (b >> i & 1) x[i] = -INFINITY;
+    for (int j = 0; j < B; ++j) {
+      const int u = (c + j * DS_THREADS - c0) * CH;
+      b[j] = (bits[u >> 5] >> (u & 31)) & ((1u << CH) - 1u);
+      any |= b[j];
     }
-    sum.add<CH>(x, a.c);
+    if (any) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (b[i / CH] >> (i % CH) & 1) x[i] = -INFINITY;
+    }
+    sum.add<N>(x, a.c);
   });
   sum = ds_join<DS_THREADS>(sum, redf, redf + 4);
   if constexpr (WHOLE) {
-    ds_finish<DT>(a, row, sum, cls, redd, redf);
+    if (threadIdx.x < 64) ds_finish(a, row, sum, e, classes);
   } else if (threadIdx.x == 0) {
     a.part[2 * blockIdx.x] = sum.m;
     a.part[2 * blockIdx.x + 1] = sum.s;
@@ -336,14 +345,15 @@ __global__ __launch_bounds__(DS_THREADS) void distill_fwd_kernel(ds_args a) {
 
 template <int DT>
 __global__ __launch_bounds__(DS_THREADS) void distill_finish_kernel(ds_args a) {
-  __shared__ __attribute__((aligned(16))) int cls[DS_KMAX];
-  __shared__ double redd[4];
+  extern __shared__ __attribute__((aligned(16))) int lds[];
+  const ds_entries e(lds, a.K);
   __shared__ float redf[8];
   const int64_t row = blockIdx.x;
   ds_sum sum;
   for (int i = threadIdx.x; i < a.segs; i += DS_THREADS) sum.join(a.part[2 * (row * a.segs + i)], a.part[2 * (row * a.segs + i) + 1]);
+  const int classes = ds_load_entries<DT>(a, row, e);
   sum = ds_join<DS_THREADS>(sum, redf, redf + 4);
-  ds_finish<DT>(a, row, sum, cls, redd, redf);
+  if (threadIdx.x < 64) ds_finish(a, row, sum, e, classes);
 }
 
 __global__ __launch_bounds__(DS_THREADS) void distill_reduce_kernel(const float* __restrict__ row_loss, int64_t R, double scale, float* __restrict__ out) {
@@ -370,7 +380,7 @@ __global__ __launch_bounds__(DS_THREADS) void distill_bwd_kernel(ds_args a) {
   const bool used = st[6] != 0.f;
   const float g = a.up[a.up_rows ? row : 0] * a.grad_scale, kappa = st[1] * g;
   char* out = (char*)a.dz + (row * a.V - r.mis) * (int64_t)ds_type<DT>::ES;
-  r.template each<DS_THREADS>(c0, c1, 0.f, [&](int c, float (&x)[CH]) {
+  r.template each<DS_THREADS, false>(c0, c1, 0.f, [&](int c, float (&x)[CH]) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) x[i] = used ? __builtin_amdgcn_exp2f(fmaf(x[i], a.c, -mt)) * kappa : 0.f;
     char* p = out + (int64_t)c * 16;
@@ -484,9 +494,9 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(tl_args a) {
   // hardly more than K are when the threads' elements are no sorted run.  (NaN are left out of the maxima; they pass the bound below.)
   float top = -INFINITY;
   bool any = false;
-  r.template each<THREADS>(c0, c1, -INFINITY, [&](int c, float (&x)[CH]) {
+  r.template each<THREADS>(c0, c1, -INFINITY, [&](int, auto& x) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i) top = fmaxf(top, x[i]);
+    for (int i = 0; i < (int)(sizeof(x) / 4); ++i) top = fmaxf(top, x[i]);
     any = true;
   });
   if (threadIdx.x == 0) count = 0;
@@ -509,21 +519,23 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(tl_args a) {
   // no NaN is less than the bound, and nothing is where the bound is no number: too few threads have elements
   const float least = tl_float(bound);
   ds_sum sum;
-  r.template each<THREADS>(c0, c1, -INFINITY, [&](int c, float (&x)[CH]) {
+  r.template each<THREADS>(c0, c1, -INFINITY, [&](int c, auto& x) {
+    constexpr int N = sizeof(x) / 4;
     bool hit = false;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) hit |= !(x[i] < least);
+    for (int i = 0; i < N; ++i) hit |= !(x[i] < least);
     if (hit) {
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        if (!(x[i] < least) && r.has(c, i)) {
+      for (int i = 0; i < N; ++i) {
+        const int at_c = c + i / CH * THREADS;
+        if (!(x[i] < least) && r.has(at_c, i % CH)) {
           const int at = atomicAdd(&count, 1);
-          if (at < TL_CAP) list[at] = ((unsigned long long)tl_key(x[i]) << 32) | (unsigned)~(unsigned)(c * CH + i - r.mis);
+          if (at < TL_CAP) list[at] = ((unsigned long long)tl_key(x[i]) << 32) | (unsigned)~(unsigned)(at_c * CH + i % CH - r.mis);
           x[i] = -INFINITY;
         }
       }
     }
-    sum.add<CH>(x, a.c);
+    sum.add<N>(x, a.c);
   });
   __syncthreads();
   int n = count;
@@ -533,10 +545,12 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(tl_args a) {
     for (int bit = 63; bit >= 0; --bit) {
       const unsigned long long probe = floor_key | (1ull << bit);
       int k = 0;
-      r.template each<THREADS>(c0, c1, 0.f, [&](int c, float (&x)[CH]) {
+      r.template each<THREADS>(c0, c1, 0.f, [&](int c, auto& x) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i)
-          k += r.has(c, i) && (((unsigned long long)tl_key(x[i]) << 32) | (unsigned)~(unsigned)(c * CH + i - r.mis)) >= probe;
+        for (int i = 0; i < (int)(sizeof(x) / 4); ++i) {
+          const int at_c = c + i / CH * THREADS;
+          k += r.has(at_c, i % CH) && (((unsigned long long)tl_key(x[i]) << 32) | (unsigned)~(unsigned)(at_c * CH + i % CH - r.mis)) >= probe;
+        }
       });
       __syncthreads();
       if (threadIdx.x == 0) count = 0;
@@ -549,16 +563,18 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(tl_args a) {
     if (threadIdx.x == 0) count = 0;
     __syncthreads();
     sum = ds_sum();
-    r.template each<THREADS>(c0, c1, -INFINITY, [&](int c, float (&x)[CH]) {
+    r.template each<THREADS>(c0, c1, -INFINITY, [&](int c, auto& x) {
+      constexpr int N = sizeof(x) / 4;
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const unsigned long long k = ((unsigned long long)tl_key(x[i]) << 32) | (unsigned)~(unsigned)(c * CH + i - r.mis);
-        if (r.has(c, i) && k >= floor_key) {
+      for (int i = 0; i < N; ++i) {
+        const int at_c = c + i / CH * THREADS;
+        const unsigned long long k = ((unsigned long long)tl_key(x[i]) << 32) | (unsigned)~(unsigned)(at_c * CH + i % CH - r.mis);
+        if (r.has(at_c, i % CH) && k >= floor_key) {
           list[atomicAdd(&count, 1)] = k;
           x[i] = -INFINITY;
         }
       }
-      sum.add<CH>(x, a.c);
+      sum.add<N>(x, a.c);
     });
   }
   __syncthreads();
@@ -647,12 +663,12 @@ extern "C" int ofb_distill_fwd(const void* z, const void* values, const void* in
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)(R * a.segs)), block(DS_THREADS);
   // (a row spans one chunk more than V classes take where it starts inside one; the last word is only cleared)
-  const int ch = 16 / ds_es(dtype), nc = (V + 2 * ch - 2) / ch, lds = (((K + 3) & ~3) + (nc + a.segs - 1) / a.segs * ch / 32 + 2) * 4;
+  const int ch = 16 / ds_es(dtype), nc = (V + 2 * ch - 2) / ch, lds = (ds_entries::words(K) + (nc + a.segs - 1) / a.segs * ch / 32 + 2) * 4;
 #define DS_FWD(DT)                                                                                        \
   if (a.segs == 1) hipLaunchKernelGGL((distill_fwd_kernel<DT, true>), grid, block, lds, s, a);            \
   else {                                                                                                  \
     hipLaunchKernelGGL((distill_fwd_kernel<DT, false>), grid, block, lds, s, a);                          \
-    hipLaunchKernelGGL((distill_finish_kernel<DT>), dim3((unsigned)R), block, 0, s, a);                   \
+    hipLaunchKernelGGL((distill_finish_kernel<DT>), dim3((unsigned)R), block, ds_entries::words(K) * 4, s, a);                   \
   }
   if (dtype == DS_F32) { DS_FWD(DS_F32) } else if (dtype == DS_BF16) { DS_FWD(DS_BF16) } else { DS_FWD(DS_F16) }
   if (loss) hipLaunchKernelGGL(distill_reduce_kernel, dim3(1), block, 0, s, row_loss, R, loss_scale, loss);
@@ -684,13 +700,12 @@ extern "C" int ofb_top_logits(const void* z, int64_t R, int32_t V, int32_t K, fl
   if (R * a.segs > 0x7fffffff) return OFB_ELIMIT;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)(R * a.segs));
-  // few classes and a short list: a small workgroup ranks fewer maxima
 #define TL_RUN(DT)                                                                                                        \
   if (a.segs > 1) {                                                                                                       \
     hipLaunchKernelGGL((top_logits_kernel<DT, TL_THREADS, false>), grid, dim3(TL_THREADS), 0, s, a);                      \
     hipLaunchKernelGGL((top_logits_join_kernel<DT>), dim3((unsigned)R), dim3(TL_THREADS), 0, s, a);                       \
-  } else if (V <= 8192 && K <= 128) {                                                                                     \
-    hipLaunchKernelGGL((top_logits_kernel<DT, 256, true>), grid, dim3(256), 0, s, a);                                     \
+  } else if (K <= TL_SMALL / 2) {                                                                                         \
+    hipLaunchKernelGGL((top_logits_kernel<DT, TL_SMALL, true>), grid, dim3(TL_SMALL), 0, s, a);                                     \
   } else {                                                                                                                \
     hipLaunchKernelGGL((top_logits_kernel<DT, TL_THREADS, true>), grid, dim3(TL_THREADS), 0, s, a);                       \
   }
