@@ -30,6 +30,7 @@
 #define RP_OQ 2
 #define RP_OK 2
 #define RP_OF 3
+#define RP_OB 2
 #endif
 #define RP_PAD 4                 /* entries of w on either side, so that four consecutive differences need one clamp */
 #define RP_WMAX 4096
@@ -48,9 +49,11 @@ template <int DT> struct rp_type { static constexpr int NP = 1, ES = 2; };
 template <> struct rp_type<RP_F32> { static constexpr int NP = 2, ES = 4; };
 
 // rows of a streamed tile: 64, or 32 where two planes or wide heads would take the LDS of a second workgroup
-template <int DT, int DP> struct rp_geo {
+template <int DT, int DP> constexpr int rp_kb_of() { return (rp_type<DT>::NP == 1 && DP <= 64) ? 64 : 32; }
+template <int DP> constexpr int rp_qb_of() { return DP <= 64 ? 64 : 32; }          // queries of a tile of the table's gradient
+template <int DT, int DP, int ROWS = rp_kb_of<DT, DP>()> struct rp_geo {
   static constexpr int NP = rp_type<DT>::NP;
-  static constexpr int KB = (NP == 1 && DP <= 64) ? 64 : 32;
+  static constexpr int KB = ROWS;
   static constexpr int PITCH = DP * 2 + 16;                  // bytes of a row of one plane: 8 rows' 16-byte chunks fall into different banks
   static constexpr int PLANE = KB * PITCH;
   static constexpr int TENSOR = NP * PLANE;
@@ -140,9 +143,9 @@ __device__ __forceinline__ void rp_store4(char* p, float a, float b, float c, fl
 }
 
 // a [rows][DP] tile on its way from memory to LDS: one register image per thread, loaded a tile ahead
-template <int DT, int DP>
+template <int DT, int DP, int ROWS = rp_kb_of<DT, DP>()>
 struct rp_stage {
-  using G = rp_geo<DT, DP>;
+  using G = rp_geo<DT, DP, ROWS>;
   rp_chunk<DT> c[G::PER];
   __device__ __forceinline__ void load(const char* base, int64_t row_bytes, int row0, int row_end, int d) {
 #pragma unroll
@@ -166,17 +169,17 @@ struct rp_stage {
 };
 
 // A operand from an LDS tile, rows along the tile's rows: k-step ks of row0 + (l & 31)
-template <int DT, int DP>
+template <int DT, int DP, int ROWS = rp_kb_of<DT, DP>()>
 __device__ __forceinline__ void rp_rows(const char* lds, int row0, int ks, int lane, rp_frag (&out)[rp_type<DT>::NP]) {
-  using G = rp_geo<DT, DP>;
+  using G = rp_geo<DT, DP, ROWS>;
 #pragma unroll
   for (int p = 0; p < G::NP; ++p) out[p] = *reinterpret_cast<const rp_frag*>(lds + p * G::PLANE + (row0 + (lane & 31)) * G::PITCH + (2 * ks + (lane >> 5)) * 16);
 }
 // A operand from an LDS tile, rows along the tile's columns (channels 32 ct ..), k-slots = tile rows row0 + 8 (j >> 2) + 4 hh + (j & 3).
 // ds_read_b64_tr_b16: in each group of 16 lanes, lane 4 e + q addresses four channels of row e, lane i receives four rows of channel i.
-template <int DT, int DP>
+template <int DT, int DP, int ROWS = rp_kb_of<DT, DP>()>
 __device__ __forceinline__ void rp_cols(const char* lds, int row0, int ct, int lane, rp_frag (&out)[rp_type<DT>::NP]) {
-  using G = rp_geo<DT, DP>;
+  using G = rp_geo<DT, DP, ROWS>;
   const int off = (row0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * G::PITCH + (32 * ct + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
 #pragma unroll
   for (int p = 0; p < G::NP; ++p) {
@@ -189,15 +192,20 @@ __device__ __forceinline__ void rp_cols(const char* lds, int row0, int ct, int l
 
 struct rp_scales { int eq, ek, ev, ed, es; };
 
-// max of a tensor's partial maxima, by every thread of the workgroup (n <= RP_NBOUND; an absent vector counts as 0)
-__device__ __forceinline__ float rp_bound(const float* part, int n, float* red) {
-  float v = 0.f;
-  if (part && (int)threadIdx.x < n) v = part[threadIdx.x];
-  v = ofb_wave_max(v);
+// maxima of N tensors from their partial maxima (n of each <= RP_NBOUND), by every thread of the workgroup; red: [4][N]
+template <int N>
+__device__ __forceinline__ void rp_bounds(const float* const (&part)[N], const int (&n)[N], float (&out)[N], float* red) {
+  float v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = (int)threadIdx.x < n[i] ? part[i][threadIdx.x] : 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = ofb_wave_max(v[i]);
+  if ((threadIdx.x & 63) == 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i) red[(threadIdx.x >> 6) * N + i] = v[i];
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[i] = fmaxf(fmaxf(red[i], red[N + i]), fmaxf(red[2 * N + i], red[3 * N + i]));
 }
 
 // the head's bias by difference, times log2 e, padded by RP_PAD copies of its ends
@@ -213,23 +221,26 @@ __device__ __forceinline__ int rp_keys_of(const ofb_relpos_args& a, int b) {
   return min(max(n, 0), a.Nk);
 }
 
-__device__ __forceinline__ int rp_idx(int diff, int width) { return min(max(diff, 0), width - 1) + RP_PAD; }
+typedef __attribute__((address_space(3))) const float rp_lds_float;
+// LDS address of w[RP_PAD]: the entry of difference lo
+__device__ __forceinline__ int rp_lds_base(const float* w) { return (int)(uintptr_t)(rp_lds_float*)(w + RP_PAD); }
+// the bias at an LDS address, clamped to the head's vector: one instruction (the compiler makes two of min and max), and a read
+__device__ __forceinline__ float rp_bias1(int at, int first, int last) {
+  int c;
+  asm("v_med3_i32 %0, %1, %2, %3" : "=v"(c) : "v"(at), "v"(first), "v"(last));
+  return *(rp_lds_float*)(uintptr_t)(unsigned)c;
+}
 
 // register r of an accumulator <-> row of the 32 x 32 tile
 __device__ __forceinline__ int rp_row(int r, int hh) { return 8 * (r >> 2) + 4 * hh + (r & 3); }
 
 // the biases of the four pairs whose differences are d0, d0 + step, ... (step +1 or -1): one clamp, one 16-byte read
 template <int STEP>
-__device__ __forceinline__ void rp_bias4(const float* w, int d0, int width, float (&out)[4]) {
-  if constexpr (STEP > 0) {
-    const float* p = w + RP_PAD + min(max(d0, -RP_PAD), width);
+__device__ __forceinline__ void rp_bias4(int w_first, int d0, int width, float (&out)[4]) {
+  const int at = w_first + 4 * min(max(STEP > 0 ? d0 : d0 - 3, -RP_PAD), width);
+  rp_lds_float* p = (rp_lds_float*)(uintptr_t)(unsigned)at;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) out[j] = p[j];
-  } else {
-    const float* p = w + RP_PAD + min(max(d0 - 3, -RP_PAD), width);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) out[j] = p[3 - j];
-  }
+  for (int j = 0; j < 4; ++j) out[j] = p[STEP > 0 ? j : 3 - j];
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -243,11 +254,11 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 
   using G = rp_geo<DT, DP>;
   constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ float red[4];
+  __shared__ float red[16];
   float* w = reinterpret_cast<float*>(smem);
   int* pk = reinterpret_cast<int*>(smem + ((a.width + 2 * RP_PAD + 3) & ~3) * 4);
   char* tiles = reinterpret_cast<char*>(pk + 2 * KB);
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, hh = lane >> 5;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const int nqt = (a.Nq + RP_TILE - 1) / RP_TILE;
   const int id = ofb_xcd_remap(blockIdx.x, gridDim.x);
   const int qt = id % nqt, bh = id / nqt, head = bh % a.H, b = bh / a.H;
@@ -270,20 +281,20 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 
   auto fetch = [&](int kb) {
     ks_.load(kp, a.k_st * ES, kb * KB, kend, a.d);
     vs_.load(vp, a.v_st * ES, kb * KB, kend, a.d);
-    if (a.pos_k && threadIdx.x < KB) { const int j = kb * KB + threadIdx.x; pk_next = j < kend ? a.pos_k[j] : 0; }
+    if (a.pos_k && threadIdx.x < KB) { const int j = kb * KB + threadIdx.x; pk_next = j < kend ? 4 * a.pos_k[j] : 0; }
   };
   if (kb0 < kb1) fetch(kb0);
   rp_bias_vector(a, head, w);
   float hq = 1.f, hk = 1.f, hv = 1.f, c_s = a.scale * 1.44269504088896340736f, c_o = 1.f;
   if constexpr (DT == RP_F32) {
-    const int eq = ofb_h_exp(rp_bound(a.bound_q, a.n_bound, red)), ek = ofb_h_exp(rp_bound(a.bound_k, a.n_bound, red)),
-              ev = ofb_h_exp(rp_bound(a.bound_v, a.n_bound, red));
+    float top[3];
+    rp_bounds<3>({a.bound_q, a.bound_k, a.bound_v}, {a.n_bound, a.n_bound, a.n_bound}, top, red);
+    const int eq = ofb_h_exp(top[0]), ek = ofb_h_exp(top[1]), ev = ofb_h_exp(top[2]);
     hq = ofb_h_pow2(eq); hk = ofb_h_pow2(ek); hv = ofb_h_pow2(ev);
     c_s = c_s * ofb_h_pow2(-eq) * ofb_h_pow2(-ek);
     c_o = ofb_h_pow2(-ev);
   }
-  if constexpr (DT != RP_BF16) c_o *= ofb_h_pow2(-RP_PE);
-  const float p_sc = DT == RP_BF16 ? 1.f : ofb_h_pow2(RP_PE);
+  constexpr float p_exp = DT == RP_BF16 ? 0.f : (float)RP_PE;  // P and its sum are held times 2^p_exp
 
   const int q0 = qt * RP_TILE + wv * 32, qi = q0 + (lane & 31);
   const bool active = q0 < a.Nq, qok = qi < a.Nq;
@@ -309,7 +320,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 
   };
   if (kb0 < kb1) commit(0);
   __syncthreads();
-  const int lo = a.lo, width = a.width, hi = lo + width - 1;
+  const int lo = a.lo, width = a.width, hi = lo + width - 1, w_first = rp_lds_base(w), w_last = w_first + 4 * (width - 1), pq4 = 4 * (pq + lo) - w_first;
   for (int kb = kb0; kb < kb1; ++kb) {
     const int buf = (kb - kb0) & 1;
     const char* kt_ = tiles + buf * G::STAGE;
@@ -342,10 +353,10 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 
 #pragma unroll
           for (int r = 0; r < 16; r += 4) {
             const int4 pj = *reinterpret_cast<const int4*>(&pk[buf * KB + 32 * t + rp_row(r, hh)]);
-            S[t][r] = fmaf(S[t][r], c_s, w[rp_idx(pj.x - pq - lo, width)]);
-            S[t][r + 1] = fmaf(S[t][r + 1], c_s, w[rp_idx(pj.y - pq - lo, width)]);
-            S[t][r + 2] = fmaf(S[t][r + 2], c_s, w[rp_idx(pj.z - pq - lo, width)]);
-            S[t][r + 3] = fmaf(S[t][r + 3], c_s, w[rp_idx(pj.w - pq - lo, width)]);
+            S[t][r] = fmaf(S[t][r], c_s, rp_bias1(pj.x - pq4, w_first, w_last));
+            S[t][r + 1] = fmaf(S[t][r + 1], c_s, rp_bias1(pj.y - pq4, w_first, w_last));
+            S[t][r + 2] = fmaf(S[t][r + 2], c_s, rp_bias1(pj.z - pq4, w_first, w_last));
+            S[t][r + 3] = fmaf(S[t][r + 3], c_s, rp_bias1(pj.w - pq4, w_first, w_last));
           }
       } else {
 #pragma unroll
@@ -353,7 +364,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 
 #pragma unroll
           for (int r = 0; r < 16; r += 4) {
             float w4[4];
-            rp_bias4<1>(w, j0 + 32 * t + rp_row(r, hh) - pq - lo, width, w4);
+            rp_bias4<1>(w_first, j0 + 32 * t + rp_row(r, hh) - pq - lo, width, w4);
 #pragma unroll
             for (int u = 0; u < 4; ++u) S[t][r + u] = fmaf(S[t][r + u], c_s, w4[u]);
           }
@@ -380,7 +391,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 
         for (int t = 0; t < DP / 32; ++t) O[t] *= alpha;
         m = m_new;
       }
-      const float tb = bt - (m > -INFINITY ? m : 0.f);         // a row that has seen nothing yet: exp2(-inf - 0) = 0
+      const float tb = bt - (m > -INFINITY ? m : 0.f) + p_exp;         // a row that has seen nothing yet: exp2(-inf - 0) = 0
 #pragma unroll
       for (int t = 0; t < KB / 32; ++t) {
 #pragma unroll
@@ -390,7 +401,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 
           for (int j = 0; j < 8; ++j) {
             const float p = __builtin_amdgcn_exp2f(fmaf(S[t][8 * s + j], c_t, tb));
             l += p;
-            p8[j] = DT == RP_BF16 ? p : p * p_sc;
+            p8[j] = p;
           }
           rp_frag pf[NP];
           rp_pack8<DT>(p8, pf);
@@ -410,7 +421,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 
   if (!qok) return;
   if constexpr (SPLIT) {                                       // partial sums in units of exp2(m), joined by relpos_join_kernel
     const int64_t row = ((int64_t)blockIdx.y * a.B * a.H + bh) * a.Nq + qi;
-    if (hh == 0) { a.split_ml[2 * row] = m; a.split_ml[2 * row + 1] = l; }
+    if (hh == 0) { a.split_ml[2 * row] = m - p_exp; a.split_ml[2 * row + 1] = l; }
 #pragma unroll
     for (int ct = 0; ct < DP / 32; ++ct)
 #pragma unroll
@@ -423,7 +434,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 
     if (a.stats && hh == 0) {
       float* st = a.stats + 2 * ((int64_t)bh * a.Nq + qi);
       st[0] = m > -INFINITY ? m : 0.f;
-      st[1] = linv;
+      st[1] = __builtin_ldexpf(linv, (int)p_exp);
     }
     const float f = linv * c_o;
     char* op = (char*)a.out + (b * a.o_sb + qi * a.o_st + head * a.o_sh) * ES;
@@ -476,14 +487,20 @@ template <int DT>
 __device__ __forceinline__ rp_scales rp_all_scales(const ofb_relpos_args& a, float* red) {
   rp_scales e = {0, 0, 0, 0, 0};
   if constexpr (DT != RP_BF16) {
-    const float bv = rp_bound(a.bound_v, a.n_bound, red), bd = rp_bound(a.bound_do, a.n_bound_do, red);
-    e.es = ofb_h_exp(2.f * a.d * bv * bd);                     // |dS| <= P (|dP| + |D|) <= 2 d max|dO| max|V|
+    float top[4] = {0.f, 0.f, 0.f, 0.f};
     if constexpr (DT == RP_F32) {
-      e.eq = ofb_h_exp(rp_bound(a.bound_q, a.n_bound, red));
-      e.ek = ofb_h_exp(rp_bound(a.bound_k, a.n_bound, red));
-      e.ev = ofb_h_exp(bv);
-      e.ed = ofb_h_exp(bd);
+      rp_bounds<4>({a.bound_q, a.bound_k, a.bound_v, a.bound_do}, {a.n_bound, a.n_bound, a.n_bound, a.n_bound_do}, top, red);
+      e.eq = ofb_h_exp(top[0]);
+      e.ek = ofb_h_exp(top[1]);
+      e.ev = ofb_h_exp(top[2]);
+      e.ed = ofb_h_exp(top[3]);
+    } else {
+      float two[2];
+      rp_bounds<2>({a.bound_v, a.bound_do}, {a.n_bound, a.n_bound_do}, two, red);
+      top[2] = two[0];
+      top[3] = two[1];
     }
+    e.es = ofb_h_exp(2.f * a.d * top[2] * top[3]);             // |dS| <= P (|dP| + |D|) <= 2 d max|dO| max|V|
   }
   return e;
 }
@@ -495,11 +512,11 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
   using G = rp_geo<DT, DP>;
   constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ float red[4];
+  __shared__ float red[16];
   float* w = reinterpret_cast<float*>(smem);
   int* pk = reinterpret_cast<int*>(smem + ((a.width + 2 * RP_PAD + 3) & ~3) * 4);
   char* tiles = reinterpret_cast<char*>(pk + 2 * KB);
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, hh = lane >> 5;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const int nqt = (a.Nq + RP_TILE - 1) / RP_TILE;
   const int id = ofb_xcd_remap(blockIdx.x, gridDim.x);
   const int qt = id % nqt, bh = id / nqt, head = bh % a.H, b = bh / a.H;
@@ -516,7 +533,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
   auto fetch = [&](int kb) {
     ks_.load(kp, a.k_st * ES, kb * KB, kend, a.d);
     vs_.load(vp, a.v_st * ES, kb * KB, kend, a.d);
-    if (a.pos_k && threadIdx.x < KB) { const int j = kb * KB + threadIdx.x; pk_next = j < kend ? a.pos_k[j] : 0; }
+    if (a.pos_k && threadIdx.x < KB) { const int j = kb * KB + threadIdx.x; pk_next = j < kend ? 4 * a.pos_k[j] : 0; }
   };
   if (kb1 > 0) fetch(0);
   rp_bias_vector(a, head, w);
@@ -568,7 +585,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
   };
   if (kb1 > 0) commit(0);
   __syncthreads();
-  const int lo = a.lo, width = a.width, hi = lo + width - 1;
+  const int lo = a.lo, width = a.width, hi = lo + width - 1, w_first = rp_lds_base(w), w_last = w_first + 4 * (width - 1), pq4 = 4 * (pq + lo) - w_first;
   for (int kb = 0; kb < kb1; ++kb) {
     const int buf = kb & 1;
     const char* kt_ = tiles + buf * G::STAGE;
@@ -612,21 +629,22 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
 #pragma unroll
           for (int r = 0; r < 16; r += 4) {
             const int4 pj = *reinterpret_cast<const int4*>(&pk[buf * KB + 32 * t0 + rp_row(r, hh)]);
-            t[r] = w[rp_idx(pj.x - pq - lo, width)];
-            t[r + 1] = w[rp_idx(pj.y - pq - lo, width)];
-            t[r + 2] = w[rp_idx(pj.z - pq - lo, width)];
-            t[r + 3] = w[rp_idx(pj.w - pq - lo, width)];
+            t[r] = rp_bias1(pj.x - pq4, w_first, w_last);
+            t[r + 1] = rp_bias1(pj.y - pq4, w_first, w_last);
+            t[r + 2] = rp_bias1(pj.z - pq4, w_first, w_last);
+            t[r + 3] = rp_bias1(pj.w - pq4, w_first, w_last);
           }
         } else {
 #pragma unroll
           for (int r = 0; r < 16; r += 4) {
             float w4[4];
-            rp_bias4<1>(w, j0 + rp_row(r, hh) - pq - lo, width, w4);
+            rp_bias4<1>(w_first, j0 + rp_row(r, hh) - pq - lo, width, w4);
 #pragma unroll
             for (int u = 0; u < 4; ++u) t[r + u] = w4[u];
           }
         }
         if (!whole) {                                          // keys this query does not see: P = 0, whatever S and dP are there
+          asm volatile("");
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (j0 + rp_row(r, hh) >= seen) { t[r] = -INFINITY; S[r] = dP[r] = 0.f; }
@@ -640,6 +658,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
           sum += ds[r];
         }
         if (!a.pos_k && (dmin <= lo || dmax >= hi)) {
+          asm volatile("");                                    // (a branch: as selects on every tile this was a quarter of the kernel)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int diff = j0 + rp_row(r, hh) - pq;
@@ -716,20 +735,21 @@ __device__ __forceinline__ void rp_row_stats(const ofb_relpos_args& a, int64_t b
     if constexpr (DT == RP_F32) { v[0] = m; v[1] = __builtin_ldexpf(l, pe); }
     else v[0] = l > 0.f ? m - __log2f(l) - (float)pe : l == 0.f ? INFINITY : l;
     v[2] = -__builtin_ldexpf(a.delta[row], de);
-    pos = a.pos_q ? a.pos_q[i] : i + a.q_offset;
+    pos = a.pos_q ? 4 * a.pos_q[i] : i + a.q_offset;
   }
 }
 
 // P and dS of a 32 x 32 tile, rows = queries i0 .. (LDS tiles qt_ and dt_ at row tr), the wave's key on the lane.  st: row statistics m, l, -D of
 // the tile's queries, P = exp2(s - m) (times l for f32; l is in m otherwise), -D in dP's scale.  P comes out times the p_sc that is in the statistics,
 // dS = P dP times that and dP's scale.
-template <int DT, int DP>
+template <int DT, int DP, int ROWS>
 __device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char* qt_, const char* dt_, int tr, const rp_frag (&kf)[DP / 16][rp_type<DT>::NP],
                                            const rp_frag (&vf)[DP / 16][rp_type<DT>::NP], const float* st, const int* ps, const float* w, int i0, int j0,
                                            int kj, int pkj, bool kok, bool kwhole, float c_s, float (&P)[16], float (&dS)[16]) {
-  using G = rp_geo<DT, DP>;
+  using G = rp_geo<DT, DP, ROWS>;
   constexpr int NP = G::NP, KB = G::KB;
-  const int lane = threadIdx.x & 63, hh = lane >> 5, lo = a.lo, width = a.width, hi = lo + width - 1;
+  const int lane = threadIdx.x & 63, hh = lane >> 5, lo = a.lo, width = a.width, hi = lo + width - 1, w_first = rp_lds_base(w),
+            w_last = w_first + 4 * (width - 1), pk4 = 4 * (pkj - lo) + w_first;
   f32x16 S = rp_zero16(), dP;
 #pragma unroll
   for (int r = 0; r < 16; r += 4) {
@@ -740,8 +760,8 @@ __device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char*
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
     rp_frag qa[NP], da[NP];
-    rp_rows<DT, DP>(qt_, tr, s, lane, qa);
-    rp_rows<DT, DP>(dt_, tr, s, lane, da);
+    rp_rows<DT, DP, ROWS>(qt_, tr, s, lane, qa);
+    rp_rows<DT, DP, ROWS>(dt_, tr, s, lane, da);
     S = rp_mm<DT, NP>(qa, kf[s], S);
     dP = rp_mm<DT, NP>(da, vf[s], dP);
   }
@@ -756,21 +776,22 @@ __device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char*
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
       const int4 pi = *reinterpret_cast<const int4*>(&ps[tr + rp_row(r, hh)]);
-      t[r] = w[rp_idx(pkj - pi.x - lo, width)];
-      t[r + 1] = w[rp_idx(pkj - pi.y - lo, width)];
-      t[r + 2] = w[rp_idx(pkj - pi.z - lo, width)];
-      t[r + 3] = w[rp_idx(pkj - pi.w - lo, width)];
+      t[r] = rp_bias1(pk4 - pi.x, w_first, w_last);
+      t[r + 1] = rp_bias1(pk4 - pi.y, w_first, w_last);
+      t[r + 2] = rp_bias1(pk4 - pi.z, w_first, w_last);
+      t[r + 3] = rp_bias1(pk4 - pi.w, w_first, w_last);
     }
   } else {
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
       float w4[4];
-      rp_bias4<-1>(w, kj - (i0 + rp_row(r, hh) + a.q_offset) - lo, width, w4);
+      rp_bias4<-1>(w_first, kj - (i0 + rp_row(r, hh) + a.q_offset) - lo, width, w4);
 #pragma unroll
       for (int u = 0; u < 4; ++u) t[r + u] = w4[u];
     }
   }
   if (!kwhole || cut) {                                        // queries that do not see this key: P = 0, whatever S and dP are there
+    asm volatile("");
 #pragma unroll
     for (int r = 0; r < 16; ++r)
       if (!kok || (cut && kj > i0 + rp_row(r, hh) + a.q_offset)) { t[r] = -INFINITY; S[r] = dP[r] = 0.f; }
@@ -797,12 +818,12 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OK : 1)) void relpos_dkv
   using G = rp_geo<DT, DP>;
   constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ float red[4];
+  __shared__ float red[16];
   float* w = reinterpret_cast<float*>(smem);
   float* st = reinterpret_cast<float*>(smem + ((a.width + 2 * RP_PAD + 3) & ~3) * 4);      // [2][3][KB]
   int* ps = reinterpret_cast<int*>(st + 6 * KB);                                            // [2][KB]
   char* tiles = reinterpret_cast<char*>(ps + 2 * KB);
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, hh = lane >> 5;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const int nkt = (a.Nk + RP_TILE - 1) / RP_TILE;
   const int id = ofb_xcd_remap(blockIdx.x, gridDim.x);
   const int kt = id % nkt, bh = id / nkt, head = bh % a.H, b = bh / a.H;
@@ -870,7 +891,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OK : 1)) void relpos_dkv
       const int i0 = qb * KB + 32 * t;
       if (!active || i0 >= a.Nq || (a.causal && j0 > i0 + 31 + a.q_offset)) continue;
       float P[16], dS[16];
-      rp_tile_ds<DT, DP>(a, qt_, dt_, 32 * t, kf, vf, st + buf * 3 * KB, ps + buf * KB, w, i0, j0, kj, pkj, kok, j0 + 32 <= kend, c_s, P, dS);
+      rp_tile_ds<DT, DP, KB>(a, qt_, dt_, 32 * t, kf, vf, st + buf * 3 * KB, ps + buf * KB, w, i0, j0, kj, pkj, kok, j0 + 32 <= kend, c_s, P, dS);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         float p8[8], x8[8];
@@ -912,11 +933,11 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OK : 1)) void relpos_dkv
 // difference in LDS: whole numbers of 2^-40 of the tile's largest |dS|, so that the order of the additions does not matter.  Without
 // position arrays only the tiles with differences strictly between the first and the last are visited (relpos_dq_kernel sums the rest).
 template <int DT, int DP>
-__global__ __launch_bounds__(RP_THREADS, (DT == RP_F32 ? 1 : DP <= 64 ? 2 : 3)) void relpos_dbias_kernel(ofb_relpos_args a, int chunks) {
-  using G = rp_geo<DT, DP>;
+__global__ __launch_bounds__(RP_THREADS, (RP_OB)) void relpos_dbias_kernel(ofb_relpos_args a, int chunks) {
+  using G = rp_geo<DT, DP, rp_qb_of<DP>()>;
   constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ float red[4];
+  __shared__ float red[16];
   const int wpad = (a.width + 2 * RP_PAD + 3) & ~3;
   float* w = reinterpret_cast<float*>(smem);
   float* st = w + wpad;                                                                     // [3][KB]
@@ -924,7 +945,7 @@ __global__ __launch_bounds__(RP_THREADS, (DT == RP_F32 ? 1 : DP <= 64 ? 2 : 3)) 
   unsigned long long* hist = reinterpret_cast<unsigned long long*>(ps + KB);                // [wpad]
   double* acc = reinterpret_cast<double*>(hist + wpad);                                     // [wpad]
   char* tiles = reinterpret_cast<char*>(acc + wpad);
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, hh = lane >> 5;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const int nqt = (a.Nq + KB - 1) / KB;
   const int chunk = blockIdx.x % chunks, qt = (blockIdx.x / chunks) % nqt, head = blockIdx.x / (chunks * nqt);
   const int b0 = (int)((int64_t)a.B * chunk / chunks), b1 = (int)((int64_t)a.B * (chunk + 1) / chunks);
@@ -954,7 +975,7 @@ __global__ __launch_bounds__(RP_THREADS, (DT == RP_F32 ? 1 : DP <= 64 ? 2 : 3)) 
     for (int b = b0; b < b1; ++b) {
       const int kend = rp_keys_of(a, b);
       if (kt * RP_TILE >= kend) continue;
-      rp_stage<DT, DP> qs_, ds_;
+      rp_stage<DT, DP, KB> qs_, ds_;
       f32x4 st_next;
       int ps_next;
       qs_.load((const char*)a.q + (b * a.q_sb + head * a.q_sh) * ES, a.q_st * ES, i_first, a.Nq, a.d);
@@ -989,7 +1010,7 @@ __global__ __launch_bounds__(RP_THREADS, (DT == RP_F32 ? 1 : DP <= 64 ? 2 : 3)) 
         const int i0 = i_first + 32 * t;
         if (j0 >= kend || i0 >= a.Nq || (a.causal && j0 > i0 + 31 + a.q_offset)) continue;
         float P[16], dS[16];
-        rp_tile_ds<DT, DP>(a, tiles, tiles + G::TENSOR, 32 * t, kf, vf, st, ps, w, i0, j0, kj, pkj, kok, j0 + 32 <= kend, c_s, P, dS);
+        rp_tile_ds<DT, DP, KB>(a, tiles, tiles + G::TENSOR, 32 * t, kf, vf, st, ps, w, i0, j0, kj, pkj, kok, j0 + 32 <= kend, c_s, P, dS);
 #pragma unroll
         for (int r = 0; r < 16; ++r) sum[t][r] += DT == RP_F32 ? dS[r] * c_x : dS[r];
       }
@@ -1016,7 +1037,7 @@ __global__ __launch_bounds__(RP_THREADS, (DT == RP_F32 ? 1 : DP <= 64 ? 2 : 3)) 
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int i = i_first + 32 * t + rp_row(r, hh);
-          const int diff = pkj - (a.pos_q ? ps[32 * t + rp_row(r, hh)] : i + a.q_offset);
+          const int diff = pkj - (a.pos_q ? ps[32 * t + rp_row(r, hh)] / 4 : i + a.q_offset);
           const float x = sum[t][r];
           if (x != 0.f && fabsf(x) < 3.0e38f && (a.pos_k || (diff > lo && diff < hi)))
             atomicAdd(&hist[min(max(diff - lo, 0), width - 1)], (unsigned long long)__double2ll_rn((double)x * up));
@@ -1071,19 +1092,34 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_amax_kernel(ofb_relpos_args
   const int tokens = key ? a.Nk : a.Nq;
   float v = 0.f;
   const int64_t rows = (int64_t)a.B * tokens;
-  // one token after the other per group of threads: `per` chunks each
+  // a group of threads per token (`per` chunks each), four tokens' loads in flight
   const int group = min(per, RP_THREADS), groups = RP_THREADS / group, g = threadIdx.x / group, t0 = threadIdx.x % group;
+  const int64_t step = (int64_t)gridDim.x * groups;
   if (g < groups) {
-    for (int64_t row = (int64_t)blockIdx.x * groups + g; row < rows; row += (int64_t)gridDim.x * groups) {
-      const int b = (int)(row / tokens), i = (int)(row - (int64_t)b * tokens);
-      int end = rp_keys_of(a, b);
-      if (key) { if (i >= (a.causal ? min(end, max(0, a.Nq + a.q_offset)) : end)) continue; }
-      else if (end == 0 || (a.causal && i + a.q_offset < 0)) continue;       // a query that sees nothing
-      for (int c = t0; c < per; c += group) {
-        const int head = c / (a.d / 8), ch = (c % (a.d / 8)) * 8;
-        const rp_chunk<DT> q = rp_load_chunk<DT>(x + (b * sb + (int64_t)i * st + head * sh + ch) * ES);
+    for (int64_t row = (int64_t)blockIdx.x * groups + g; row < rows; row += 4 * step) {
+      const char* p[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v = fmaxf(v, fabsf(rp_chunk_at<DT>(q, j)));
+      for (int u = 0; u < 4; ++u) {
+        const int64_t at = row + u * step;
+        const int b = (int)(at / tokens), i = (int)(at - (int64_t)b * tokens);
+        p[u] = nullptr;
+        if (at >= rows) continue;
+        const int end = rp_keys_of(a, b);
+        const bool seen = key ? i < (a.causal ? min(end, max(0, a.Nq + a.q_offset)) : end) : end > 0 && !(a.causal && i + a.q_offset < 0);
+        if (seen) p[u] = x + (b * sb + (int64_t)i * st) * ES;
+      }
+      for (int c = t0; c < per; c += group) {
+        const int64_t off = ((c / (a.d / 8)) * sh + (c % (a.d / 8)) * 8) * ES;
+        rp_chunk<DT> q[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          q[u] = rp_zero_chunk<DT>();
+          if (p[u]) q[u] = rp_load_chunk<DT>(p[u] + off);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v = fmaxf(v, fabsf(rp_chunk_at<DT>(q[u], j)));
       }
     }
   }
@@ -1099,7 +1135,8 @@ template <int DT, int DP> int rp_lds(const ofb_relpos_args& a, int kind) {      
   const int w = ((a.width + 2 * RP_PAD + 3) & ~3) * 4;
   if (kind == 0) return w + 2 * G::KB * 4 + 2 * G::STAGE;
   if (kind == 1) return w + 8 * G::KB * 4 + 2 * G::STAGE;
-  return w * 5 + 4 * G::KB * 4 + G::STAGE;
+  using B = rp_geo<DT, DP, rp_qb_of<DP>()>;
+  return w * 5 + 4 * B::KB * 4 + B::STAGE;
 }
 
 template <typename F> int rp_allow(F* f, int bytes) {
@@ -1118,6 +1155,7 @@ int rp_table_chunks(const ofb_relpos_args& a, int kb) {
   return (int)(want < a.B ? (want < 1 ? 1 : want) : a.B);
 }
 int rp_kb(const ofb_relpos_args& a) { return a.dtype != RP_F32 && a.d <= 64 ? 64 : 32; }
+int rp_qb(const ofb_relpos_args& a) { return a.d <= 64 ? 64 : 32; }
 
 // key ranges of the forward: where the query tiles leave most of the chip idle, ranges of at least four tiles
 int rp_splits(const ofb_relpos_args& a) {
@@ -1132,8 +1170,8 @@ int rp_check(const ofb_relpos_args* a) {
   if (!a || !a->q || !a->k || !a->v || !a->table || !a->lut) return OFB_EINVAL;
   if (a->B < 1 || a->H < 1 || a->Nq < 1 || a->Nk < 1 || a->d < 8 || a->d % 8 || a->dtype < 0 || a->dtype > 2) return OFB_EINVAL;
   if (a->width < 1 || a->n_buckets < 1 || (!a->pos_q) != (!a->pos_k) || (a->pos_q && a->causal)) return OFB_EINVAL;
-  if (a->d > 128 || a->width > RP_WMAX || a->Nq > (1 << 29) || a->Nk > (1 << 29)) return OFB_ELIMIT;
-  if (a->q_offset > (1 << 29) || a->q_offset < -(1 << 29) || a->lo > (1 << 29) || a->lo < -(1 << 29)) return OFB_ELIMIT;
+  if (a->d > 128 || a->width > RP_WMAX || a->Nq > (1 << 26) || a->Nk > (1 << 26)) return OFB_ELIMIT;
+  if (a->q_offset > (1 << 26) || a->q_offset < -(1 << 26) || a->lo > (1 << 26) || a->lo < -(1 << 26)) return OFB_ELIMIT;
   const int64_t tiles = (int64_t)a->B * a->H * (((int64_t)(a->Nq > a->Nk ? a->Nq : a->Nk) + 31) / 32);
   if (tiles > 0x3fffffff) return OFB_ELIMIT;
   const int64_t unit = a->dtype == RP_F32 ? 4 : 8;             // 16-byte loads
@@ -1159,7 +1197,7 @@ template <int DT, int DP> int rp_forward(const ofb_relpos_args& a, hipStream_t s
 }
 
 template <int DT, int DP> int rp_backward(const ofb_relpos_args& a, hipStream_t s) {
-  const int kb = rp_geo<DT, DP>::KB, nqt = (a.Nq + RP_TILE - 1) / RP_TILE, nkt = (a.Nk + RP_TILE - 1) / RP_TILE;
+  const int kb = rp_qb_of<DP>(), nqt = (a.Nq + RP_TILE - 1) / RP_TILE, nkt = (a.Nk + RP_TILE - 1) / RP_TILE;
   RP_LAUNCH((relpos_dq_kernel<DT, DP>), dim3((unsigned)((int64_t)a.B * a.H * nqt)), (rp_lds<DT, DP>(a, 0)), s, a);
   RP_LAUNCH((relpos_dkv_kernel<DT, DP>), dim3((unsigned)((int64_t)a.B * a.H * nkt)), (rp_lds<DT, DP>(a, 1)), s, a);
   if (a.dtable) {
@@ -1188,7 +1226,7 @@ template <int DT, int DP> int rp_backward(const ofb_relpos_args& a, hipStream_t 
 
 extern "C" int ofb_relpos_sizes(const ofb_relpos_args* a, int64_t* out4) {
   if (!a || !out4 || a->B < 1 || a->H < 1 || a->Nq < 1 || a->Nk < 1 || a->width < 1) return OFB_EINVAL;
-  const int64_t rows = (int64_t)a->B * a->H * a->Nq, splits = rp_splits(*a), kb = rp_kb(*a);
+  const int64_t rows = (int64_t)a->B * a->H * a->Nq, splits = rp_splits(*a), kb = rp_qb(*a);
   out4[0] = splits > 1 ? splits * rows * a->d : 0;             // split_o
   out4[1] = splits > 1 ? splits * rows * 2 : 0;                // split_ml
   out4[2] = (int64_t)a->H * a->width * ((a->Nq + kb - 1) / kb) * rp_table_chunks(*a, (int)kb);      // partial

@@ -915,8 +915,8 @@ class _RelposCall:
                 raise hip.OfbError('relpos_attention: causal and q_offset go by the number of a token, not by given positions')
             if (len(buckets.positions[0]), len(buckets.positions[1])) != (Nq, k.shape[1]):
                 raise hip.OfbError(f'relpos_attention: positions of {len(buckets.positions[0])} queries and {len(buckets.positions[1])} keys, got {Nq} and {k.shape[1]}')
-        if abs(int(q_offset)) > 1 << 28 or max(Nq, k.shape[1]) > 1 << 28:
-            raise hip.OfbError('relpos_attention: positions beyond 2^28 are not supported')
+        if abs(int(q_offset)) > 1 << 26 or max(Nq, k.shape[1]) > 1 << 26:
+            raise hip.OfbError('relpos_attention: positions beyond 2^26 are not supported')
         if not q.is_cuda:
             raise hip.OfbError('once-for-both_amd kernels need device tensors (no CPU fallback); got a CPU tensor')
         self.buckets, self.causal, self.q_offset, self.bound = buckets, bool(causal), int(q_offset), bound

@@ -8,7 +8,7 @@ import torch
 from .hip import OfbError
 
 MAX_WIDTH = 4096
-_FAR = 1 << 28
+_FAR = 1 << 26                         # (four times a difference of two positions and `lo` stays a 32-bit number)
 
 
 class RelPosBuckets:
@@ -35,12 +35,12 @@ class RelPosBuckets:
         if len(self.lut) > MAX_WIDTH:
             raise OfbError(f'RelPosBuckets: {len(self.lut)} different differences, at most {MAX_WIDTH} are supported')
         if abs(self.lo) > _FAR:
-            raise OfbError('RelPosBuckets: differences beyond 2^28 are not supported')
+            raise OfbError('RelPosBuckets: differences beyond 2^26 are not supported')
         self.positions = None
         if positions is not None:
             self.positions = tuple([int(x) for x in (p.tolist() if isinstance(p, torch.Tensor) else p)] for p in positions)
             if len(self.positions) != 2 or any(abs(x) > _FAR for p in self.positions for x in p):
-                raise OfbError('RelPosBuckets: positions are two sequences of whole numbers within 2^28')
+                raise OfbError('RelPosBuckets: positions are two sequences of whole numbers within 2^26')
         self._on = {}
 
     def __getstate__(self):
