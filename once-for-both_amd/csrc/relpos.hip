@@ -225,22 +225,23 @@ typedef __attribute__((address_space(3))) const float rp_lds_float;
 // LDS address of w[RP_PAD]: the entry of difference lo
 __device__ __forceinline__ int rp_lds_base(const float* w) { return (int)(uintptr_t)(rp_lds_float*)(w + RP_PAD); }
 // the bias at an LDS address, clamped to the head's vector: one instruction (the compiler makes two of min and max), and a read
-__device__ __forceinline__ float rp_bias1(int at, int first, int last) {
-  int c;
+__device__ __forceinline__ float rp_bias1(int at, int first, int last, int& c) {
   asm("v_med3_i32 %0, %1, %2, %3" : "=v"(c) : "v"(at), "v"(first), "v"(last));
   return *(rp_lds_float*)(uintptr_t)(unsigned)c;
 }
+__device__ __forceinline__ float rp_bias1(int at, int first, int last) { int c; return rp_bias1(at, first, last, c); }
 
 // register r of an accumulator <-> row of the 32 x 32 tile
 __device__ __forceinline__ int rp_row(int r, int hh) { return 8 * (r >> 2) + 4 * hh + (r & 3); }
 
 // the biases of the four pairs whose differences are d0, d0 + step, ... (step +1 or -1): one clamp, one 16-byte read
 template <int STEP>
-__device__ __forceinline__ void rp_bias4(int w_first, int d0, int width, float (&out)[4]) {
+__device__ __forceinline__ int rp_bias4(int w_first, int d0, int width, float (&out)[4]) {
   const int at = w_first + 4 * min(max(STEP > 0 ? d0 : d0 - 3, -RP_PAD), width);
   rp_lds_float* p = (rp_lds_float*)(uintptr_t)(unsigned)at;
 #pragma unroll
   for (int j = 0; j < 4; ++j) out[j] = p[STEP > 0 ? j : 3 - j];
+  return at;                                                   // (STEP +1: the first one's LDS address)
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -505,16 +506,21 @@ __device__ __forceinline__ rp_scales rp_all_scales(const ofb_relpos_args& a, flo
   return e;
 }
 
-// dQ, D, and the part of the table's gradient that lies beyond the last differences.  The forward's layout: 128 queries a workgroup, the
-// query on the lane; dS^T is the B operand of dQ^T = K^T dS^T from its registers.
+// dQ and D.  The forward's layout: 128 queries a workgroup, the query on the lane; dS^T is the B operand of dQ^T = K^T dS^T from its registers.
+// The table's gradient: tiles that lie wholly beyond the first or last difference add up to two numbers.  The other pairs go to a histogram by
+// difference in LDS - for f32, whose D is exact enough from the start; for bf16 and f16, whose D is only known when a row is done, the pairs
+// beyond the ends are summed here (and corrected at the end) and relpos_dbias_kernel visits the others again.
 template <int DT, int DP>
 __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 || DT == RP_F32 ? 2 : RP_OQ)) void relpos_dq_kernel(ofb_relpos_args a) {
   using G = rp_geo<DT, DP>;
   constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float red[16];
+  constexpr bool HIST = DT == RP_F32;
+  const int wpad = (a.width + 2 * RP_PAD + 3) & ~3;
   float* w = reinterpret_cast<float*>(smem);
-  int* pk = reinterpret_cast<int*>(smem + ((a.width + 2 * RP_PAD + 3) & ~3) * 4);
+  unsigned long long* hist = reinterpret_cast<unsigned long long*>(w + wpad);               // [wpad], where HIST
+  int* pk = reinterpret_cast<int*>(w + (HIST ? 3 : 1) * wpad);
   char* tiles = reinterpret_cast<char*>(pk + 2 * KB);
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const int nqt = (a.Nq + RP_TILE - 1) / RP_TILE;
@@ -537,6 +543,8 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
   };
   if (kb1 > 0) fetch(0);
   rp_bias_vector(a, head, w);
+  if constexpr (HIST)
+    for (int i = threadIdx.x; i < wpad; i += RP_THREADS) hist[i] = 0ull;
   const rp_scales e = rp_all_scales<DT>(a, red);
   const float hq = ofb_h_pow2(e.eq), hk = ofb_h_pow2(e.ek), hv = ofb_h_pow2(e.ev), hd = ofb_h_pow2(e.ed);
   const float c_s = a.scale * 1.44269504088896340736f * ofb_h_pow2(-e.eq) * ofb_h_pow2(-e.ek);
@@ -625,22 +633,23 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
         if (dmax <= lo) { sat_lo += sum; pat_lo += psum; } else { sat_hi += sum; pat_hi += psum; }
       } else {
         float t[16];
+        int at[16];                                            // LDS addresses of the pairs' biases (HIST)
         if (a.pos_k) {
 #pragma unroll
           for (int r = 0; r < 16; r += 4) {
             const int4 pj = *reinterpret_cast<const int4*>(&pk[buf * KB + 32 * t0 + rp_row(r, hh)]);
-            t[r] = rp_bias1(pj.x - pq4, w_first, w_last);
-            t[r + 1] = rp_bias1(pj.y - pq4, w_first, w_last);
-            t[r + 2] = rp_bias1(pj.z - pq4, w_first, w_last);
-            t[r + 3] = rp_bias1(pj.w - pq4, w_first, w_last);
+            t[r] = rp_bias1(pj.x - pq4, w_first, w_last, at[r]);
+            t[r + 1] = rp_bias1(pj.y - pq4, w_first, w_last, at[r + 1]);
+            t[r + 2] = rp_bias1(pj.z - pq4, w_first, w_last, at[r + 2]);
+            t[r + 3] = rp_bias1(pj.w - pq4, w_first, w_last, at[r + 3]);
           }
         } else {
 #pragma unroll
           for (int r = 0; r < 16; r += 4) {
             float w4[4];
-            rp_bias4<1>(w_first, j0 + rp_row(r, hh) - pq - lo, width, w4);
+            at[r] = rp_bias4<1>(w_first, j0 + rp_row(r, hh) - pq - lo, width, w4);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) t[r + u] = w4[u];
+            for (int u = 0; u < 4; ++u) { t[r + u] = w4[u]; at[r + u] = at[r] + 4 * u; }
           }
         }
         if (!whole) {                                          // keys this query does not see: P = 0, whatever S and dP are there
@@ -657,7 +666,19 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
           ds[r] = p[r] * dP[r];
           sum += ds[r];
         }
-        if (!a.pos_k && (dmin <= lo || dmax >= hi)) {
+        if constexpr (HIST) {
+          // The pair's dS to its difference's bin, as a whole number of 2^-38 of the operand's scale: |ds| < 2^15 and a row's |ds| sum to less than
+          // that, so 128 rows stay below 2^60, and the order of the additions does not matter.  High word: floor(64 ds), low word: the rest.
+          if (a.dtable) {
+            asm volatile("");
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float y = ds[r] * 64.f;
+              const unsigned long long v = ((unsigned long long)(unsigned)(int)floorf(y) << 32) | (unsigned)(__builtin_amdgcn_fractf(y) * 4294967296.f);
+              atomicAdd(&hist[(at[r] - w_first) / 4 + RP_PAD], v);
+            }
+          }
+        } else if (!a.pos_k && (dmin <= lo || dmax >= hi)) {
           asm volatile("");                                    // (a branch: as selects on every tile this was a quarter of the kernel)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
@@ -709,6 +730,21 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
       const int64_t n = (int64_t)a.B * nqt * 4, at = ((int64_t)b * nqt + qt) * 4 + wv;
       a.sat[(2 * (int64_t)head) * n + at] = sat_lo;
       a.sat[(2 * (int64_t)head + 1) * n + at] = sat_hi;
+    }
+  }
+  if constexpr (HIST) {
+    if (a.dtable) {
+      const bool bad = __syncthreads_or(!(fabsf(left) < 3.0e38f));         // (the conversions drop NaN and infinities)
+      const float unit = __builtin_ldexpf(1.f, -38);
+      const int64_t rows = (int64_t)a.B * nqt, at = (int64_t)b * nqt + qt;
+      for (int i = threadIdx.x; i < width; i += RP_THREADS) {
+        long long v = (long long)hist[i + RP_PAD];
+        if (i == 0)
+          for (int u = 0; u < RP_PAD; ++u) v += (long long)hist[u];
+        if (i == width - 1)
+          for (int u = 0; u < RP_PAD; ++u) v += (long long)hist[width + RP_PAD + u];
+        a.partial[((int64_t)head * width + i) * rows + at] = bad ? __builtin_nanf("") : (float)__builtin_ldexp((double)v * (double)unit, -e.es);
+      }
     }
   }
   if (!qok) return;
@@ -1062,15 +1098,14 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_table_kernel(ofb_relpos_arg
   double sum = 0.0;
   for (int e = a.bucket_start[c]; e < a.bucket_start[c + 1]; ++e) {
     const int i = a.bucket_order[e];
-    if (nsat > 0 && (i == 0 || i == a.width - 1)) {            // (a single difference takes both)
-      for (int side = i == 0 ? 0 : 1; side < (i == a.width - 1 ? 2 : 1); ++side) {
+    if (nsat > 0) {                                            // beyond the ends (a single difference takes both sides)
+      for (int side = i == 0 ? 0 : 1; side < (i == a.width - 1 ? 2 : i == 0 ? 1 : 0); ++side) {
         const float* p = a.sat + (2 * (int64_t)head + side) * nsat;
         for (int64_t r = lane; r < nsat; r += 64) sum += (double)p[r];
       }
-    } else {
-      const float* p = a.partial + ((int64_t)head * a.width + i) * rows;
-      for (int64_t r = lane; r < rows; r += 64) sum += (double)p[r];
     }
+    const float* p = a.partial + ((int64_t)head * a.width + i) * rows;
+    for (int64_t r = lane; r < rows; r += 64) sum += (double)p[r];
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
@@ -1130,11 +1165,12 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_amax_kernel(ofb_relpos_args
   if (threadIdx.x == 0) out[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
-template <int DT, int DP> int rp_lds(const ofb_relpos_args& a, int kind) {       // 0 forward / dQ, 1 dK dV, 2 table gradient
+template <int DT, int DP> int rp_lds(const ofb_relpos_args& a, int kind) {       // 0 forward, 1 dK dV, 2 table gradient, 3 dQ
   using G = rp_geo<DT, DP>;
   const int w = ((a.width + 2 * RP_PAD + 3) & ~3) * 4;
   if (kind == 0) return w + 2 * G::KB * 4 + 2 * G::STAGE;
   if (kind == 1) return w + 8 * G::KB * 4 + 2 * G::STAGE;
+  if (kind == 3) return w * (DT == RP_F32 ? 3 : 1) + 2 * G::KB * 4 + 2 * G::STAGE;
   using B = rp_geo<DT, DP, rp_qb_of<DP>()>;
   return w * 5 + 4 * B::KB * 4 + B::STAGE;
 }
@@ -1156,6 +1192,11 @@ int rp_table_chunks(const ofb_relpos_args& a, int kb) {
 }
 int rp_kb(const ofb_relpos_args& a) { return a.dtype != RP_F32 && a.d <= 64 ? 64 : 32; }
 int rp_qb(const ofb_relpos_args& a) { return a.d <= 64 ? 64 : 32; }
+// workgroups per head that leave a part of the table's gradient
+int64_t rp_table_rows(const ofb_relpos_args& a) {
+  if (a.dtype == RP_F32) return (int64_t)a.B * ((a.Nq + RP_TILE - 1) / RP_TILE);
+  return (int64_t)((a.Nq + rp_qb(a) - 1) / rp_qb(a)) * rp_table_chunks(a, rp_qb(a));
+}
 
 // key ranges of the forward: where the query tiles leave most of the chip idle, ranges of at least four tiles
 int rp_splits(const ofb_relpos_args& a) {
@@ -1197,13 +1238,15 @@ template <int DT, int DP> int rp_forward(const ofb_relpos_args& a, hipStream_t s
 }
 
 template <int DT, int DP> int rp_backward(const ofb_relpos_args& a, hipStream_t s) {
-  const int kb = rp_qb_of<DP>(), nqt = (a.Nq + RP_TILE - 1) / RP_TILE, nkt = (a.Nk + RP_TILE - 1) / RP_TILE;
-  RP_LAUNCH((relpos_dq_kernel<DT, DP>), dim3((unsigned)((int64_t)a.B * a.H * nqt)), (rp_lds<DT, DP>(a, 0)), s, a);
+  const int nqt = (a.Nq + RP_TILE - 1) / RP_TILE, nkt = (a.Nk + RP_TILE - 1) / RP_TILE;
+  RP_LAUNCH((relpos_dq_kernel<DT, DP>), dim3((unsigned)((int64_t)a.B * a.H * nqt)), (rp_lds<DT, DP>(a, 3)), s, a);
   RP_LAUNCH((relpos_dkv_kernel<DT, DP>), dim3((unsigned)((int64_t)a.B * a.H * nkt)), (rp_lds<DT, DP>(a, 1)), s, a);
   if (a.dtable) {
-    const int chunks = rp_table_chunks(a, kb), nqb = (a.Nq + kb - 1) / kb;
-    RP_LAUNCH((relpos_dbias_kernel<DT, DP>), dim3((unsigned)((int64_t)a.H * nqb * chunks)), (rp_lds<DT, DP>(a, 2)), s, a, chunks);
-    hipLaunchKernelGGL(relpos_table_kernel, dim3((unsigned)(((int64_t)a.n_buckets * a.H + 3) / 4)), dim3(RP_THREADS), 0, s, a, (int64_t)nqb * chunks,
+    if constexpr (DT != RP_F32) {
+      const int chunks = rp_table_chunks(a, rp_qb_of<DP>());
+      RP_LAUNCH((relpos_dbias_kernel<DT, DP>), dim3((unsigned)(a.H * rp_table_rows(a))), (rp_lds<DT, DP>(a, 2)), s, a, chunks);
+    }
+    hipLaunchKernelGGL(relpos_table_kernel, dim3((unsigned)(((int64_t)a.n_buckets * a.H + 3) / 4)), dim3(RP_THREADS), 0, s, a, rp_table_rows(a),
                        a.pos_k ? (int64_t)0 : (int64_t)a.B * nqt * 4);
   }
   return ofb_launch_status();
@@ -1226,10 +1269,10 @@ template <int DT, int DP> int rp_backward(const ofb_relpos_args& a, hipStream_t 
 
 extern "C" int ofb_relpos_sizes(const ofb_relpos_args* a, int64_t* out4) {
   if (!a || !out4 || a->B < 1 || a->H < 1 || a->Nq < 1 || a->Nk < 1 || a->width < 1) return OFB_EINVAL;
-  const int64_t rows = (int64_t)a->B * a->H * a->Nq, splits = rp_splits(*a), kb = rp_qb(*a);
+  const int64_t rows = (int64_t)a->B * a->H * a->Nq, splits = rp_splits(*a);
   out4[0] = splits > 1 ? splits * rows * a->d : 0;             // split_o
   out4[1] = splits > 1 ? splits * rows * 2 : 0;                // split_ml
-  out4[2] = (int64_t)a->H * a->width * ((a->Nq + kb - 1) / kb) * rp_table_chunks(*a, (int)kb);      // partial
+  out4[2] = (int64_t)a->H * a->width * rp_table_rows(*a);      // partial
   out4[3] = a->pos_k ? 0 : (int64_t)a->H * 2 * a->B * ((a->Nq + RP_TILE - 1) / RP_TILE) * 4;        // sat
   return OFB_OK;
 }
