@@ -30,7 +30,6 @@
 #define RP_OQ 2
 #define RP_OK 2
 #define RP_OF 3
-#define RP_OB 2
 #endif
 #define RP_PAD 4                 /* entries of w on either side, so that four consecutive differences need one clamp */
 #define RP_WMAX 4096
@@ -49,11 +48,9 @@ template <int DT> struct rp_type { static constexpr int NP = 1, ES = 2; };
 template <> struct rp_type<RP_F32> { static constexpr int NP = 2, ES = 4; };
 
 // rows of a streamed tile: 64, or 32 where two planes or wide heads would take the LDS of a second workgroup
-template <int DT, int DP> constexpr int rp_kb_of() { return (rp_type<DT>::NP == 1 && DP <= 64) ? 64 : 32; }
-template <int DP> constexpr int rp_qb_of() { return DP <= 64 ? 64 : 32; }          // queries of a tile of the table's gradient
-template <int DT, int DP, int ROWS = rp_kb_of<DT, DP>()> struct rp_geo {
+template <int DT, int DP> struct rp_geo {
   static constexpr int NP = rp_type<DT>::NP;
-  static constexpr int KB = ROWS;
+  static constexpr int KB = (rp_type<DT>::NP == 1 && DP <= 64) ? 64 : 32;
   static constexpr int PITCH = DP * 2 + 16;                  // bytes of a row of one plane: 8 rows' 16-byte chunks fall into different banks
   static constexpr int PLANE = KB * PITCH;
   static constexpr int TENSOR = NP * PLANE;
@@ -143,9 +140,9 @@ __device__ __forceinline__ void rp_store4(char* p, float a, float b, float c, fl
 }
 
 // a [rows][DP] tile on its way from memory to LDS: one register image per thread, loaded a tile ahead
-template <int DT, int DP, int ROWS = rp_kb_of<DT, DP>()>
+template <int DT, int DP>
 struct rp_stage {
-  using G = rp_geo<DT, DP, ROWS>;
+  using G = rp_geo<DT, DP>;
   rp_chunk<DT> c[G::PER];
   __device__ __forceinline__ void load(const char* base, int64_t row_bytes, int row0, int row_end, int d) {
 #pragma unroll
@@ -169,17 +166,17 @@ struct rp_stage {
 };
 
 // A operand from an LDS tile, rows along the tile's rows: k-step ks of row0 + (l & 31)
-template <int DT, int DP, int ROWS = rp_kb_of<DT, DP>()>
+template <int DT, int DP>
 __device__ __forceinline__ void rp_rows(const char* lds, int row0, int ks, int lane, rp_frag (&out)[rp_type<DT>::NP]) {
-  using G = rp_geo<DT, DP, ROWS>;
+  using G = rp_geo<DT, DP>;
 #pragma unroll
   for (int p = 0; p < G::NP; ++p) out[p] = *reinterpret_cast<const rp_frag*>(lds + p * G::PLANE + (row0 + (lane & 31)) * G::PITCH + (2 * ks + (lane >> 5)) * 16);
 }
 // A operand from an LDS tile, rows along the tile's columns (channels 32 ct ..), k-slots = tile rows row0 + 8 (j >> 2) + 4 hh + (j & 3).
 // ds_read_b64_tr_b16: in each group of 16 lanes, lane 4 e + q addresses four channels of row e, lane i receives four rows of channel i.
-template <int DT, int DP, int ROWS = rp_kb_of<DT, DP>()>
+template <int DT, int DP>
 __device__ __forceinline__ void rp_cols(const char* lds, int row0, int ct, int lane, rp_frag (&out)[rp_type<DT>::NP]) {
-  using G = rp_geo<DT, DP, ROWS>;
+  using G = rp_geo<DT, DP>;
   const int off = (row0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * G::PITCH + (32 * ct + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
 #pragma unroll
   for (int p = 0; p < G::NP; ++p) {
@@ -507,20 +504,21 @@ __device__ __forceinline__ rp_scales rp_all_scales(const ofb_relpos_args& a, flo
 }
 
 // dQ and D.  The forward's layout: 128 queries a workgroup, the query on the lane; dS^T is the B operand of dQ^T = K^T dS^T from its registers.
-// The table's gradient: tiles that lie wholly beyond the first or last difference add up to two numbers.  The other pairs go to a histogram by
-// difference in LDS - for f32, whose D is exact enough from the start; for bf16 and f16, whose D is only known when a row is done, the pairs
-// beyond the ends are summed here (and corrected at the end) and relpos_dbias_kernel visits the others again.
+// The table's gradient: tiles that lie wholly beyond the first or last difference add up to two numbers, the other pairs go to a histogram by
+// difference in LDS, as whole numbers, so that the order of the additions does not matter.  For f32 that happens on the way.  For bf16 and f16 D is
+// only known when a row is done (see below): the tiles with pairs between the ends are then visited once more, for S and dP alone.  (A pass of its own
+// that summed dS over the batch first, one histogram per pair of tiles, took 170 us beside 98 us of this kernel for the 14 x 14 grid, B 128, 6 x 64
+// f32, where this takes 124 us.)
 template <int DT, int DP>
 __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 || DT == RP_F32 ? 2 : RP_OQ)) void relpos_dq_kernel(ofb_relpos_args a) {
   using G = rp_geo<DT, DP>;
   constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float red[16];
-  constexpr bool HIST = DT == RP_F32;
   const int wpad = (a.width + 2 * RP_PAD + 3) & ~3;
   float* w = reinterpret_cast<float*>(smem);
-  unsigned long long* hist = reinterpret_cast<unsigned long long*>(w + wpad);               // [wpad], where HIST
-  int* pk = reinterpret_cast<int*>(w + (HIST ? 3 : 1) * wpad);
+  unsigned long long* hist = reinterpret_cast<unsigned long long*>(w + wpad);               // [wpad]
+  int* pk = reinterpret_cast<int*>(w + 3 * wpad);
   char* tiles = reinterpret_cast<char*>(pk + 2 * KB);
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const int nqt = (a.Nq + RP_TILE - 1) / RP_TILE;
@@ -543,8 +541,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
   };
   if (kb1 > 0) fetch(0);
   rp_bias_vector(a, head, w);
-  if constexpr (HIST)
-    for (int i = threadIdx.x; i < wpad; i += RP_THREADS) hist[i] = 0ull;
+  for (int i = threadIdx.x; i < wpad; i += RP_THREADS) hist[i] = 0ull;
   const rp_scales e = rp_all_scales<DT>(a, red);
   const float hq = ofb_h_pow2(e.eq), hk = ofb_h_pow2(e.ek), hv = ofb_h_pow2(e.ev), hd = ofb_h_pow2(e.ed);
   const float c_s = a.scale * 1.44269504088896340736f * ofb_h_pow2(-e.eq) * ofb_h_pow2(-e.ek);
@@ -594,6 +591,72 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
   if (kb1 > 0) commit(0);
   __syncthreads();
   const int lo = a.lo, width = a.width, hi = lo + width - 1, w_first = rp_lds_base(w), w_last = w_first + 4 * (width - 1), pq4 = 4 * (pq + lo) - w_first;
+  // S and dP - D (in dP's scale) of 32 keys
+  auto products = [&](const char* kt_, const char* vt_, int t0, float nd, f32x16& S, f32x16& dP) {
+    S = rp_zero16();
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dP[r] = nd;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      rp_frag kf[NP], vf[NP];
+      rp_rows<DT, DP>(kt_, 32 * t0, s, lane, kf);
+      rp_rows<DT, DP>(vt_, 32 * t0, s, lane, vf);
+      S = rp_mm<DT, NP>(kf, qf[s], S);
+      dP = rp_mm<DT, NP>(vf, df[s], dP);
+    }
+  };
+  // ds: dS in units of 1 / k, k = the power of two that makes it the second product's operand (dP's own scale is in it too).  P's maximum and
+  // sum are one exponent (bf16, f16) or, for f32, the maximum and a factor: the rounding of a logarithm of the size of 10 would show.
+  // at: the LDS addresses of the pairs' biases.
+  auto general = [&](f32x16& S, f32x16& dP, int buf, int t0, int j0, bool whole, float (&ds)[16], int (&at)[16]) {
+    float t[16];
+    if (a.pos_k) {
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int4 pj = *reinterpret_cast<const int4*>(&pk[buf * KB + 32 * t0 + rp_row(r, hh)]);
+        t[r] = rp_bias1(pj.x - pq4, w_first, w_last, at[r]);
+        t[r + 1] = rp_bias1(pj.y - pq4, w_first, w_last, at[r + 1]);
+        t[r + 2] = rp_bias1(pj.z - pq4, w_first, w_last, at[r + 2]);
+        t[r + 3] = rp_bias1(pj.w - pq4, w_first, w_last, at[r + 3]);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        float w4[4];
+        at[r] = rp_bias4<1>(w_first, j0 + rp_row(r, hh) - pq - lo, width, w4);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) { t[r + u] = w4[u]; at[r + u] = at[r] + 4 * u; }
+      }
+    }
+    if (!whole) {                                              // keys this query does not see: P = 0, whatever S and dP are there
+      asm volatile("");
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (j0 + rp_row(r, hh) >= seen) { t[r] = -INFINITY; S[r] = dP[r] = 0.f; }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      float p = __builtin_amdgcn_exp2f(fmaf(S[r], c_s, t[r]) - mk);
+      if constexpr (NP == 2) p *= lk;
+      ds[r] = p * dP[r];
+    }
+  };
+  // adds the pairs to their bins as whole numbers of 2^-32 / mul: high word floor(mul ds), low word the rest
+  auto bins = [&](const float (&ds)[16], const int (&at)[16], float mul) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float y = ds[r] * mul;
+      const unsigned long long v = ((unsigned long long)(unsigned)(int)floorf(y) << 32) | (unsigned)(__builtin_amdgcn_fractf(y) * 4294967296.f);
+      atomicAdd(reinterpret_cast<unsigned long long*>(reinterpret_cast<char*>(hist) + 2 * (at[r] - w_first + 4 * RP_PAD)), v);
+    }
+  };
+  auto visible = [&](int j0) { return active && j0 < kend && !(a.causal && j0 > q0 + 31 + a.q_offset); };
+  auto is_whole = [&](int j0, int n, int first) { return j0 + n <= kend && (!a.causal || j0 + n - 1 <= first + a.q_offset); };
+  // the whole tile of keys j0 .. j0 + n - 1 and queries first .. last lies beyond an end: -1, 1 or 0
+  auto beyond = [&](int j0, int n, int first, int last) {
+    return a.pos_k ? 0 : j0 + n - 1 - first - a.q_offset <= lo ? -1 : j0 - last - a.q_offset >= hi ? 1 : 0;
+  };
+  float most = 0.f;                                            // the largest |ds| that goes to a bin
   for (int kb = 0; kb < kb1; ++kb) {
     const int buf = kb & 1;
     const char* kt_ = tiles + buf * G::STAGE;
@@ -602,25 +665,14 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
 #pragma unroll RP_UN_Q
     for (int t0 = 0; t0 < KB / 32; ++t0) {
       const int j0 = kb * KB + 32 * t0;
-      if (!active || j0 >= kend || (a.causal && j0 > q0 + 31 + a.q_offset)) continue;
-      f32x16 S = rp_zero16(), dP;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) dP[r] = nD;                 // dP - D, in dP's scale
-#pragma unroll
-      for (int s = 0; s < DP / 16; ++s) {
-        rp_frag kf[NP], vf[NP];
-        rp_rows<DT, DP>(kt_, 32 * t0, s, lane, kf);
-        rp_rows<DT, DP>(vt_, 32 * t0, s, lane, vf);
-        S = rp_mm<DT, NP>(kf, qf[s], S);
-        dP = rp_mm<DT, NP>(vf, df[s], dP);
-      }
-      // ds: dS in units of 1 / k, k = the power of two that makes it the second product's operand (dP's own scale is in it too).  P's maximum and
-      // sum are one exponent (bf16, f16) or, for f32, the maximum and a factor: the rounding of a logarithm of the size of 10 would show.
-      const bool whole = j0 + 32 <= kend && (!a.causal || j0 + 31 <= q0 + a.q_offset);
-      const int dmax = j0 + 31 - q0 - a.q_offset, dmin = j0 - (q0 + 31) - a.q_offset;
+      if (!visible(j0)) continue;
+      f32x16 S, dP;
+      products(kt_, vt_, t0, nD, S, dP);
+      const bool whole = is_whole(j0, 32, q0);
+      const int side = beyond(j0, 32, q0, q0 + 31);
       float ds[16], sum = 0.f;
-      if (whole && !a.pos_k && (dmax <= lo || dmin >= hi)) {
-        const float tb = w[RP_PAD + (dmax <= lo ? 0 : width - 1)] - mk;
+      if (whole && side) {
+        const float tb = w[RP_PAD + (side < 0 ? 0 : width - 1)] - mk;
         float psum = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -630,65 +682,17 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
           sum += ds[r];
           psum += p;
         }
-        if (dmax <= lo) { sat_lo += sum; pat_lo += psum; } else { sat_hi += sum; pat_hi += psum; }
+        if (side < 0) { sat_lo += sum; pat_lo += psum; } else { sat_hi += sum; pat_hi += psum; }
       } else {
-        float t[16];
-        int at[16];                                            // LDS addresses of the pairs' biases (HIST)
-        if (a.pos_k) {
+        int at[16];
+        general(S, dP, buf, t0, j0, whole, ds, at);
 #pragma unroll
-          for (int r = 0; r < 16; r += 4) {
-            const int4 pj = *reinterpret_cast<const int4*>(&pk[buf * KB + 32 * t0 + rp_row(r, hh)]);
-            t[r] = rp_bias1(pj.x - pq4, w_first, w_last, at[r]);
-            t[r + 1] = rp_bias1(pj.y - pq4, w_first, w_last, at[r + 1]);
-            t[r + 2] = rp_bias1(pj.z - pq4, w_first, w_last, at[r + 2]);
-            t[r + 3] = rp_bias1(pj.w - pq4, w_first, w_last, at[r + 3]);
-          }
+        for (int r = 0; r < 16; ++r) sum += ds[r];
+        if constexpr (DT == RP_F32) {                          // |ds| < 2^15, and a row's |ds| sum to less than that: 128 rows stay below 2^60
+          if (a.dtable) { asm volatile(""); bins(ds, at, 64.f); }
         } else {
 #pragma unroll
-          for (int r = 0; r < 16; r += 4) {
-            float w4[4];
-            at[r] = rp_bias4<1>(w_first, j0 + rp_row(r, hh) - pq - lo, width, w4);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) { t[r + u] = w4[u]; at[r + u] = at[r] + 4 * u; }
-          }
-        }
-        if (!whole) {                                          // keys this query does not see: P = 0, whatever S and dP are there
-          asm volatile("");
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (j0 + rp_row(r, hh) >= seen) { t[r] = -INFINITY; S[r] = dP[r] = 0.f; }
-        }
-        float p[16];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          p[r] = __builtin_amdgcn_exp2f(fmaf(S[r], c_s, t[r]) - mk);
-          if constexpr (NP == 2) p[r] *= lk;
-          ds[r] = p[r] * dP[r];
-          sum += ds[r];
-        }
-        if constexpr (HIST) {
-          // The pair's dS to its difference's bin, as a whole number of 2^-38 of the operand's scale: |ds| < 2^15 and a row's |ds| sum to less than
-          // that, so 128 rows stay below 2^60, and the order of the additions does not matter.  High word: floor(64 ds), low word: the rest.
-          if (a.dtable) {
-            asm volatile("");
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const float y = ds[r] * 64.f;
-              const unsigned long long v = ((unsigned long long)(unsigned)(int)floorf(y) << 32) | (unsigned)(__builtin_amdgcn_fractf(y) * 4294967296.f);
-              atomicAdd(&hist[(at[r] - w_first) / 4 + RP_PAD], v);
-            }
-          }
-        } else if (!a.pos_k && (dmin <= lo || dmax >= hi)) {
-          asm volatile("");                                    // (a branch: as selects on every tile this was a quarter of the kernel)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int diff = j0 + rp_row(r, hh) - pq;
-            const bool below = diff <= lo, above = diff >= hi && diff > lo;
-            sat_lo += below ? ds[r] : 0.f;
-            pat_lo += below ? p[r] : 0.f;
-            sat_hi += above ? ds[r] : 0.f;
-            pat_hi += above ? p[r] : 0.f;
-          }
+          for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(ds[r]));
         }
       }
       left += sum;
@@ -710,52 +714,82 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
     if (kb + 1 < kb1) commit(buf ^ 1);
     __syncthreads();
   }
+  if (qok) {
+    char* op = (char*)a.dq + (b * a.dq_sb + qi * a.dq_st + head * a.dq_sh) * ES;
+#pragma unroll
+    for (int ct = 0; ct < DP / 32; ++ct)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int ch = 32 * ct + rp_row(r, hh);
+        if (ch < a.d) rp_store4<DT>(op + ch * ES, dQ[ct][r] * c_dq, dQ[ct][r + 1] * c_dq, dQ[ct][r + 2] * c_dq, dQ[ct][r + 3] * c_dq);
+      }
+  }
   // D came from an output whose P was rounded for the product.  A row of dS sums to zero, so what this row's sum is off by is D's error: the
   // kernels that follow read D without it, and the sums above lose it times their share of P.  (The table's gradient is f32 and sums whole rows'
   // parts, where an error that a row's terms share does not average out: without this it was 1e-3 off for bf16.)
   OFB_XOR_STEP(left, ofb_add_, 32)
-  sat_lo = __builtin_ldexpf(sat_lo, -e.es);
-  sat_hi = __builtin_ldexpf(sat_hi, -e.es);
-  pat_lo = __builtin_ldexpf(pat_lo, -ek_);
-  pat_hi = __builtin_ldexpf(pat_hi, -ek_);
-  left = __builtin_ldexpf(left, -e.es);
-  if (qok && hh == 0) a.delta[(int64_t)bh * a.Nq + qi] = D + left;
-  sat_lo -= left * pat_lo;
-  sat_hi -= left * pat_hi;
+  if (qok && hh == 0) a.delta[(int64_t)bh * a.Nq + qi] = D + __builtin_ldexpf(left, -e.es);
+  if (!a.dtable) return;
   if (a.sat) {
-    if (!qok) sat_lo = sat_hi = 0.f;                           // (P of a row behind the last query is 0 anyway)
-    sat_lo = ofb_wave_sum(sat_lo);
-    sat_hi = ofb_wave_sum(sat_hi);
+    const float k = __builtin_ldexpf(left, -ek_);              // (P is held times 2^ek_)
+    sat_lo = ofb_wave_sum(sat_lo - k * pat_lo);
+    sat_hi = ofb_wave_sum(sat_hi - k * pat_hi);
     if (lane == 0) {
       const int64_t n = (int64_t)a.B * nqt * 4, at = ((int64_t)b * nqt + qt) * 4 + wv;
-      a.sat[(2 * (int64_t)head) * n + at] = sat_lo;
-      a.sat[(2 * (int64_t)head + 1) * n + at] = sat_hi;
+      a.sat[(2 * (int64_t)head) * n + at] = __builtin_ldexpf(sat_lo, -e.es);
+      a.sat[(2 * (int64_t)head + 1) * n + at] = __builtin_ldexpf(sat_hi, -e.es);
     }
   }
-  if constexpr (HIST) {
-    if (a.dtable) {
-      const bool bad = __syncthreads_or(!(fabsf(left) < 3.0e38f));         // (the conversions drop NaN and infinities)
-      const float unit = __builtin_ldexpf(1.f, -38);
-      const int64_t rows = (int64_t)a.B * nqt, at = (int64_t)b * nqt + qt;
-      for (int i = threadIdx.x; i < width; i += RP_THREADS) {
-        long long v = (long long)hist[i + RP_PAD];
-        if (i == 0)
-          for (int u = 0; u < RP_PAD; ++u) v += (long long)hist[u];
-        if (i == width - 1)
-          for (int u = 0; u < RP_PAD; ++u) v += (long long)hist[width + RP_PAD + u];
-        a.partial[((int64_t)head * width + i) * rows + at] = bad ? __builtin_nanf("") : (float)__builtin_ldexp((double)v * (double)unit, -e.es);
+  const bool bad = __syncthreads_or(!(fabsf(left) < 3.0e38f));             // (the conversions drop NaN and infinities)
+  int unit = 38;
+  if constexpr (DT != RP_F32) {
+    // once more over the tiles with pairs between the ends, with the D that is known now; bins of 2^-unit, such that all pairs of the
+    // workgroup could be as large as the largest
+    most = ofb_wave_max(most + fabsf(left));
+    if (lane == 0) red[wv] = most;
+    __syncthreads();
+    most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    int ex = 0;
+    if (most > 0.f) frexpf(most, &ex);
+    unit = 62 - max(ex, -60) - (7 + 32 - __clz(a.Nk));
+    const float mul = __builtin_ldexpf(1.f, unit - 32), nd = nD - __builtin_ldexpf(left, e.ed + e.ev - e.es);
+    auto next = [&](int kb) {
+      while (kb < kb1 && is_whole(kb * KB, KB, qt * RP_TILE) && beyond(kb * KB, KB, qt * RP_TILE, q_last)) ++kb;
+      return kb;
+    };
+    int kb = bad ? kb1 : next(0), buf = 0;
+    if (kb < kb1) { fetch(kb); commit(0); }
+    __syncthreads();
+    while (kb < kb1) {
+      const char* kt_ = tiles + buf * G::STAGE;
+      const int after = next(kb + 1);
+      if (after < kb1) fetch(after);
+      for (int t0 = 0; t0 < KB / 32; ++t0) {
+        const int j0 = kb * KB + 32 * t0;
+        const bool whole = is_whole(j0, 32, q0);
+        if (!visible(j0) || (whole && beyond(j0, 32, q0, q0 + 31))) continue;
+        f32x16 S, dP;
+        float ds[16];
+        int at[16];
+        products(kt_, kt_ + G::TENSOR, t0, nd, S, dP);
+        general(S, dP, buf, t0, j0, whole, ds, at);
+        bins(ds, at, mul);
       }
+      if (after < kb1) commit(buf ^ 1);
+      __syncthreads();
+      kb = after;
+      buf ^= 1;
     }
   }
-  if (!qok) return;
-  char* op = (char*)a.dq + (b * a.dq_sb + qi * a.dq_st + head * a.dq_sh) * ES;
-#pragma unroll
-  for (int ct = 0; ct < DP / 32; ++ct)
-#pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const int ch = 32 * ct + rp_row(r, hh);
-      if (ch < a.d) rp_store4<DT>(op + ch * ES, dQ[ct][r] * c_dq, dQ[ct][r + 1] * c_dq, dQ[ct][r + 2] * c_dq, dQ[ct][r + 3] * c_dq);
-    }
+  const int64_t rows = (int64_t)a.B * nqt, at = (int64_t)b * nqt + qt;
+  for (int i = threadIdx.x; i < width; i += RP_THREADS) {
+    long long v = (long long)hist[i + RP_PAD];
+    if (i == 0)
+      for (int u = 0; u < RP_PAD; ++u) v += (long long)hist[u];
+    if (i == width - 1)
+      for (int u = 0; u < RP_PAD; ++u) v += (long long)hist[width + RP_PAD + u];
+    a.partial[((int64_t)head * width + i) * rows + at] = bad ? __builtin_nanf("") : (float)__builtin_ldexp((double)v, -unit - e.es);
+  }
 }
 
 // a query tile's row statistics for LDS: the maximum (with the sum's logarithm and the operand's scale 2^pe in it, or for f32 apart), the factor,
@@ -778,11 +812,11 @@ __device__ __forceinline__ void rp_row_stats(const ofb_relpos_args& a, int64_t b
 // P and dS of a 32 x 32 tile, rows = queries i0 .. (LDS tiles qt_ and dt_ at row tr), the wave's key on the lane.  st: row statistics m, l, -D of
 // the tile's queries, P = exp2(s - m) (times l for f32; l is in m otherwise), -D in dP's scale.  P comes out times the p_sc that is in the statistics,
 // dS = P dP times that and dP's scale.
-template <int DT, int DP, int ROWS>
+template <int DT, int DP>
 __device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char* qt_, const char* dt_, int tr, const rp_frag (&kf)[DP / 16][rp_type<DT>::NP],
                                            const rp_frag (&vf)[DP / 16][rp_type<DT>::NP], const float* st, const int* ps, const float* w, int i0, int j0,
                                            int kj, int pkj, bool kok, bool kwhole, float c_s, float (&P)[16], float (&dS)[16]) {
-  using G = rp_geo<DT, DP, ROWS>;
+  using G = rp_geo<DT, DP>;
   constexpr int NP = G::NP, KB = G::KB;
   const int lane = threadIdx.x & 63, hh = lane >> 5, lo = a.lo, width = a.width, hi = lo + width - 1, w_first = rp_lds_base(w),
             w_last = w_first + 4 * (width - 1), pk4 = 4 * (pkj - lo) + w_first;
@@ -796,8 +830,8 @@ __device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char*
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
     rp_frag qa[NP], da[NP];
-    rp_rows<DT, DP, ROWS>(qt_, tr, s, lane, qa);
-    rp_rows<DT, DP, ROWS>(dt_, tr, s, lane, da);
+    rp_rows<DT, DP>(qt_, tr, s, lane, qa);
+    rp_rows<DT, DP>(dt_, tr, s, lane, da);
     S = rp_mm<DT, NP>(qa, kf[s], S);
     dP = rp_mm<DT, NP>(da, vf[s], dP);
   }
@@ -927,7 +961,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OK : 1)) void relpos_dkv
       const int i0 = qb * KB + 32 * t;
       if (!active || i0 >= a.Nq || (a.causal && j0 > i0 + 31 + a.q_offset)) continue;
       float P[16], dS[16];
-      rp_tile_ds<DT, DP, KB>(a, qt_, dt_, 32 * t, kf, vf, st + buf * 3 * KB, ps + buf * KB, w, i0, j0, kj, pkj, kok, j0 + 32 <= kend, c_s, P, dS);
+      rp_tile_ds<DT, DP>(a, qt_, dt_, 32 * t, kf, vf, st + buf * 3 * KB, ps + buf * KB, w, i0, j0, kj, pkj, kok, j0 + 32 <= kend, c_s, P, dS);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         float p8[8], x8[8];
@@ -962,132 +996,6 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OK : 1)) void relpos_dkv
         rp_store4<DT>(ovp + ch * ES, dV[ct][r] * c_dv, dV[ct][r + 1] * c_dv, dV[ct][r + 2] * c_dv, dV[ct][r + 3] * c_dv);
       }
     }
-}
-
-// The table's gradient by difference.  A workgroup owns one head, one query tile and one part of the batch; for every key tile of 128 it sums
-// dS over its part of the batch in registers (so a pair's bucket is looked up once, not once per sample), then adds the tile to a histogram by
-// difference in LDS: whole numbers of 2^-40 of the tile's largest |dS|, so that the order of the additions does not matter.  Without
-// position arrays only the tiles with differences strictly between the first and the last are visited (relpos_dq_kernel sums the rest).
-template <int DT, int DP>
-__global__ __launch_bounds__(RP_THREADS, (RP_OB)) void relpos_dbias_kernel(ofb_relpos_args a, int chunks) {
-  using G = rp_geo<DT, DP, rp_qb_of<DP>()>;
-  constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ float red[16];
-  const int wpad = (a.width + 2 * RP_PAD + 3) & ~3;
-  float* w = reinterpret_cast<float*>(smem);
-  float* st = w + wpad;                                                                     // [3][KB]
-  int* ps = reinterpret_cast<int*>(st + 3 * KB);                                            // [KB]
-  unsigned long long* hist = reinterpret_cast<unsigned long long*>(ps + KB);                // [wpad]
-  double* acc = reinterpret_cast<double*>(hist + wpad);                                     // [wpad]
-  char* tiles = reinterpret_cast<char*>(acc + wpad);
-  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
-  const int nqt = (a.Nq + KB - 1) / KB;
-  const int chunk = blockIdx.x % chunks, qt = (blockIdx.x / chunks) % nqt, head = blockIdx.x / (chunks * nqt);
-  const int b0 = (int)((int64_t)a.B * chunk / chunks), b1 = (int)((int64_t)a.B * (chunk + 1) / chunks);
-  rp_bias_vector(a, head, w);
-  for (int i = threadIdx.x; i < wpad; i += RP_THREADS) { hist[i] = 0ull; acc[i] = 0.0; }
-  const rp_scales e = rp_all_scales<DT>(a, red);
-  const float hq = ofb_h_pow2(e.eq), hk = ofb_h_pow2(e.ek), hv = ofb_h_pow2(e.ev), hd = ofb_h_pow2(e.ed);
-  const float c_s = a.scale * 1.44269504088896340736f * ofb_h_pow2(-e.eq) * ofb_h_pow2(-e.ek);
-  const float c_x = ofb_h_pow2(-e.ed) * ofb_h_pow2(-e.ev);
-  const int i_first = qt * KB, i_last = min(a.Nq, i_first + KB) - 1, lo = a.lo, width = a.width, hi = lo + width - 1;
-  int kt0 = 0, kt1 = (a.Nk + RP_TILE - 1) / RP_TILE;
-  if (!a.pos_k) {                                              // keys with lo < j - (i + q_offset) < hi for some query of the tile
-    const int64_t jmin = max((int64_t)0, (int64_t)i_first + a.q_offset + lo + 1), jmax = min((int64_t)a.Nk - 1, (int64_t)i_last + a.q_offset + hi - 1);
-    kt0 = (int)min((int64_t)kt1, jmin / RP_TILE);
-    kt1 = jmax < jmin ? kt0 : (int)(jmax / RP_TILE) + 1;
-  }
-  bool poison = false;
-  for (int kt = kt0; kt < kt1; ++kt) {
-    const int j0 = kt * RP_TILE + wv * 32, kj = j0 + (lane & 31);
-    if (a.causal && kt * RP_TILE > i_last + a.q_offset) break;
-    const int pkj = a.pos_k ? (kj < a.Nk ? a.pos_k[kj] : 0) : kj;
-    float sum[KB / 32][16];
-#pragma unroll
-    for (int t = 0; t < KB / 32; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sum[t][r] = 0.f;
-    for (int b = b0; b < b1; ++b) {
-      const int kend = rp_keys_of(a, b);
-      if (kt * RP_TILE >= kend) continue;
-      rp_stage<DT, DP, KB> qs_, ds_;
-      f32x4 st_next;
-      int ps_next;
-      qs_.load((const char*)a.q + (b * a.q_sb + head * a.q_sh) * ES, a.q_st * ES, i_first, a.Nq, a.d);
-      ds_.load((const char*)a.dout + (b * a.do_sb + head * a.do_sh) * ES, a.do_st * ES, i_first, a.Nq, a.d);
-      rp_row_stats<DT, KB>(a, (int64_t)b * a.H + head, i_first, 0, e.ed + e.ev, st_next, ps_next);
-      const char* kp = (const char*)a.k + (b * a.k_sb + head * a.k_sh) * ES;
-      const char* vp = (const char*)a.v + (b * a.v_sb + head * a.v_sh) * ES;
-      const bool kok = kj < kend;
-      rp_frag kf[DP / 16][NP], vf[DP / 16][NP];
-#pragma unroll
-      for (int s = 0; s < DP / 16; ++s) {
-        const int ch = 16 * s + 8 * hh;
-        rp_chunk<DT> c = rp_zero_chunk<DT>(), g = rp_zero_chunk<DT>();
-        if (kok && ch < a.d) {
-          c = rp_load_chunk<DT>(kp + (int64_t)kj * a.k_st * ES + ch * ES);
-          g = rp_load_chunk<DT>(vp + (int64_t)kj * a.v_st * ES + ch * ES);
-        }
-        rp_planes<DT>(c, hk, kf[s]);
-        rp_planes<DT>(g, hv, vf[s]);
-      }
-      __syncthreads();                                         // the tile before has been read
-      qs_.store(tiles, hq);
-      ds_.store(tiles + G::TENSOR, hd);
-      if (threadIdx.x < KB) {
-#pragma unroll
-        for (int u = 0; u < 3; ++u) st[u * KB + threadIdx.x] = st_next[u];
-        ps[threadIdx.x] = ps_next;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int t = 0; t < KB / 32; ++t) {
-        const int i0 = i_first + 32 * t;
-        if (j0 >= kend || i0 >= a.Nq || (a.causal && j0 > i0 + 31 + a.q_offset)) continue;
-        float P[16], dS[16];
-        rp_tile_ds<DT, DP, KB>(a, tiles, tiles + G::TENSOR, 32 * t, kf, vf, st, ps, w, i0, j0, kj, pkj, kok, j0 + 32 <= kend, c_s, P, dS);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sum[t][r] += DT == RP_F32 ? dS[r] * c_x : dS[r];
-      }
-    }
-    float mx = 0.f;
-#pragma unroll
-    for (int t = 0; t < KB / 32; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        mx = fmaxf(mx, fabsf(sum[t][r]));
-        poison |= !(fabsf(sum[t][r]) < 3.0e38f);
-      }
-    mx = ofb_wave_max(mx);
-    __syncthreads();
-    if (lane == 0) red[wv] = mx;
-    __syncthreads();
-    mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    if (mx > 0.f && mx < 3.0e38f) {                            // (the same in every thread)
-      int ex;
-      frexpf(mx, &ex);
-      const double up = __builtin_ldexp(1.0, 40 - ex), down = __builtin_ldexp(1.0, ex - 40);
-#pragma unroll
-      for (int t = 0; t < KB / 32; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int i = i_first + 32 * t + rp_row(r, hh);
-          const int diff = pkj - (a.pos_q ? ps[32 * t + rp_row(r, hh)] / 4 : i + a.q_offset);
-          const float x = sum[t][r];
-          if (x != 0.f && fabsf(x) < 3.0e38f && (a.pos_k || (diff > lo && diff < hi)))
-            atomicAdd(&hist[min(max(diff - lo, 0), width - 1)], (unsigned long long)__double2ll_rn((double)x * up));
-        }
-      __syncthreads();
-      for (int i = threadIdx.x; i < width; i += RP_THREADS) {
-        acc[i] += (double)(long long)hist[i] * down;
-        hist[i] = 0ull;
-      }
-    }
-  }
-  const bool bad = __syncthreads_or(poison);
-  const int64_t rows = (int64_t)nqt * chunks, at = (int64_t)qt * chunks + chunk;
-  for (int i = threadIdx.x; i < width; i += RP_THREADS) a.partial[((int64_t)head * width + i) * rows + at] = bad ? __builtin_nanf("") : (float)acc[i];
 }
 
 // table gradient: one wave per (bucket, head) adds up the differences of its bucket over all workgroups, in a fixed order and in 64 bits
@@ -1165,14 +1073,10 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_amax_kernel(ofb_relpos_args
   if (threadIdx.x == 0) out[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
-template <int DT, int DP> int rp_lds(const ofb_relpos_args& a, int kind) {       // 0 forward, 1 dK dV, 2 table gradient, 3 dQ
+template <int DT, int DP> int rp_lds(const ofb_relpos_args& a, int kind) {       // 0 forward, 1 dQ, 2 dK dV
   using G = rp_geo<DT, DP>;
   const int w = ((a.width + 2 * RP_PAD + 3) & ~3) * 4;
-  if (kind == 0) return w + 2 * G::KB * 4 + 2 * G::STAGE;
-  if (kind == 1) return w + 8 * G::KB * 4 + 2 * G::STAGE;
-  if (kind == 3) return w * (DT == RP_F32 ? 3 : 1) + 2 * G::KB * 4 + 2 * G::STAGE;
-  using B = rp_geo<DT, DP, rp_qb_of<DP>()>;
-  return w * 5 + 4 * B::KB * 4 + B::STAGE;
+  return w * (kind == 1 ? 3 : 1) + (kind == 2 ? 8 : 2) * G::KB * 4 + 2 * G::STAGE;
 }
 
 template <typename F> int rp_allow(F* f, int bytes) {
@@ -1184,19 +1088,9 @@ template <typename F> int rp_allow(F* f, int bytes) {
     hipLaunchKernelGGL(kernel, grid, dim3(RP_THREADS), lds, stream, __VA_ARGS__);                                    \
   } while (0)
 
-// queries per workgroup and the batch parts of the table gradient: enough workgroups for the chip, no more partial rows than that takes
-int rp_table_chunks(const ofb_relpos_args& a, int kb) {
-  const int64_t tiles = (int64_t)a.H * ((a.Nq + kb - 1) / kb);
-  const int64_t want = (768 + tiles - 1) / tiles;
-  return (int)(want < a.B ? (want < 1 ? 1 : want) : a.B);
-}
 int rp_kb(const ofb_relpos_args& a) { return a.dtype != RP_F32 && a.d <= 64 ? 64 : 32; }
-int rp_qb(const ofb_relpos_args& a) { return a.d <= 64 ? 64 : 32; }
 // workgroups per head that leave a part of the table's gradient
-int64_t rp_table_rows(const ofb_relpos_args& a) {
-  if (a.dtype == RP_F32) return (int64_t)a.B * ((a.Nq + RP_TILE - 1) / RP_TILE);
-  return (int64_t)((a.Nq + rp_qb(a) - 1) / rp_qb(a)) * rp_table_chunks(a, rp_qb(a));
-}
+int64_t rp_table_rows(const ofb_relpos_args& a) { return (int64_t)a.B * ((a.Nq + RP_TILE - 1) / RP_TILE); }
 
 // key ranges of the forward: where the query tiles leave most of the chip idle, ranges of at least four tiles
 int rp_splits(const ofb_relpos_args& a) {
@@ -1239,13 +1133,9 @@ template <int DT, int DP> int rp_forward(const ofb_relpos_args& a, hipStream_t s
 
 template <int DT, int DP> int rp_backward(const ofb_relpos_args& a, hipStream_t s) {
   const int nqt = (a.Nq + RP_TILE - 1) / RP_TILE, nkt = (a.Nk + RP_TILE - 1) / RP_TILE;
-  RP_LAUNCH((relpos_dq_kernel<DT, DP>), dim3((unsigned)((int64_t)a.B * a.H * nqt)), (rp_lds<DT, DP>(a, 3)), s, a);
-  RP_LAUNCH((relpos_dkv_kernel<DT, DP>), dim3((unsigned)((int64_t)a.B * a.H * nkt)), (rp_lds<DT, DP>(a, 1)), s, a);
+  RP_LAUNCH((relpos_dq_kernel<DT, DP>), dim3((unsigned)((int64_t)a.B * a.H * nqt)), (rp_lds<DT, DP>(a, 1)), s, a);
+  RP_LAUNCH((relpos_dkv_kernel<DT, DP>), dim3((unsigned)((int64_t)a.B * a.H * nkt)), (rp_lds<DT, DP>(a, 2)), s, a);
   if (a.dtable) {
-    if constexpr (DT != RP_F32) {
-      const int chunks = rp_table_chunks(a, rp_qb_of<DP>());
-      RP_LAUNCH((relpos_dbias_kernel<DT, DP>), dim3((unsigned)(a.H * rp_table_rows(a))), (rp_lds<DT, DP>(a, 2)), s, a, chunks);
-    }
     hipLaunchKernelGGL(relpos_table_kernel, dim3((unsigned)(((int64_t)a.n_buckets * a.H + 3) / 4)), dim3(RP_THREADS), 0, s, a, rp_table_rows(a),
                        a.pos_k ? (int64_t)0 : (int64_t)a.B * nqt * 4);
   }
