@@ -1092,11 +1092,12 @@ int rp_kb(const ofb_relpos_args& a) { return a.dtype != RP_F32 && a.d <= 64 ? 64
 // workgroups per head that leave a part of the table's gradient
 int64_t rp_table_rows(const ofb_relpos_args& a) { return (int64_t)a.B * ((a.Nq + RP_TILE - 1) / RP_TILE); }
 
-// key ranges of the forward: where the query tiles leave most of the chip idle, ranges of at least four tiles
+// key ranges of the forward, where the query tiles leave the chip idle: a range costs a partial output, written and read again, for every query.  Up to 32
+// queries (one wave; the others stage) that is nothing beside the keys.  For more, only whole multiples are worth it: 4 x 1025 causal queries, 8 heads of
+// 128 f16, are 288 workgroups and take 40 + 27 us in four ranges, 54 us in one.
 int rp_splits(const ofb_relpos_args& a) {
   const int64_t wgs = (int64_t)a.B * a.H * ((a.Nq + RP_TILE - 1) / RP_TILE), nkb = (a.Nk + rp_kb(a) - 1) / rp_kb(a);
-  if (wgs >= 512 || nkb < 8) return 1;
-  const int64_t want = (1024 + wgs - 1) / wgs, most = nkb / 4;
+  const int64_t want = a.Nq <= 32 ? (1024 + wgs - 1) / wgs : 512 / wgs, most = nkb / 4;
   const int64_t s = want < most ? want : most;
   return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
