@@ -384,9 +384,10 @@ class MAEPatchEmbed(PatchEmbed, _Searchable):
 
 class Attention(nn.Module):
     """plain multi-head attention (reference models/layers.py:368-414); head_dim inferred from qkv width so
-    pruned checkpoints work (finetune path)."""
+    pruned checkpoints work (finetune path).  rel_pos (a RelPosBuckets for as many tokens as the layer will see): each head also
+    learns a bias per bucket of relative positions, `relative_position_bias_table` (buckets, heads), added to its scores."""
 
-    def __init__(self, dim, num_heads=8, qkv_bias=False, qk_scale=None, attn_drop=0., proj_drop=0., num_patches=197):
+    def __init__(self, dim, num_heads=8, qkv_bias=False, qk_scale=None, attn_drop=0., proj_drop=0., num_patches=197, rel_pos=None):
         super().__init__()
         self.num_heads = num_heads
         self.num_patches = num_patches
@@ -399,8 +400,14 @@ class Attention(nn.Module):
         self.proj_drop = nn.Dropout(proj_drop)
         if attn_drop or proj_drop:
             raise NotImplementedError('attention/projection dropout is 0 on the OFB path')
+        self.rel_pos = rel_pos
+        if rel_pos is not None:
+            self.relative_position_bias_table = nn.Parameter(torch.zeros(rel_pos.num_buckets, num_heads))
 
     def _branch(self, x, resid, gate, rowscale, heads):
+        if getattr(self, 'rel_pos', None) is not None:           # (objects pickled before the option existed have no such attribute)
+            return ops.relpos_attn_branch(x, resid, self.qkv.weight, self.qkv.bias, self.proj.weight, self.proj.bias,
+                                          self.relative_position_bias_table, self.rel_pos, rowscale, heads, float(self.scale))
         return ops.attn_branch(x, resid, self.qkv.weight, self.qkv.bias, self.proj.weight, self.proj.bias, gate, rowscale,
                                heads, float(self.scale))
 

@@ -16,17 +16,35 @@ class LabelSmoothingCrossEntropy(nn.Module):
         return ops.LabelSmoothingCE.apply(x.float(), target, float(self.smoothing))
 
 
+class TopLogitsDistillation(nn.Module):
+    """Distillation from a teacher of whom only the `k` largest logits of each row are kept.  `store(teacher_logits)` -> (values, classes, rest) is what a
+    teacher's pass leaves (on disk, from another job, or a line above); forward(student_logits, values, classes, rest) is temperature^2 times the
+    Kullback-Leibler divergence from it, averaged over the rows.  Without `rest` the stored probabilities are renormalised (ops.distill_top_logits)."""
+
+    def __init__(self, k, temperature=1.0, reduction='mean'):
+        super().__init__()
+        self.k, self.temperature, self.reduction = int(k), float(temperature), reduction
+
+    def store(self, logits):
+        return ops.top_logits(logits, min(self.k, logits.shape[1]), self.temperature)
+
+    def forward(self, logits, values, classes, rest=None):
+        return ops.distill_top_logits(logits, values, classes, rest, temperature=self.temperature, reduction=self.reduction)
+
+
 class DistillationLoss(nn.Module):
     """reference losses.py:10-64.  distillation_type='none' is the OFB workflow (search.py:624-631) and runs on the fused CE
     kernel; 'soft' / 'hard' follow the reference expressions on the (B, classes) logits of a model that returns
     (outputs, outputs_kd) - a handful of row-wise ATen ops on a tensor of a few hundred KB, off the search path (the OFB models
-    have no distillation head, so like the reference they raise ValueError there)."""
+    have no distillation head, so like the reference they raise ValueError there).  'top' (not in the reference): the fused loss against the
+    teacher's `top_k` largest logits (TopLogitsDistillation), on outputs_kd, or on the class logits of a model without a distillation head."""
 
-    def __init__(self, base_criterion, teacher_model, distillation_type, alpha, tau):
+    def __init__(self, base_criterion, teacher_model, distillation_type, alpha, tau, top_k=16):
         super().__init__()
-        assert distillation_type in ['none', 'soft', 'hard']
+        assert distillation_type in ['none', 'soft', 'hard', 'top']
         self.base_criterion, self.teacher_model = base_criterion, teacher_model
         self.distillation_type, self.alpha, self.tau = distillation_type, alpha, tau
+        self.top = TopLogitsDistillation(top_k, tau) if distillation_type == 'top' else None
 
     def forward(self, inputs, outputs, labels):
         outputs_kd = None
@@ -35,6 +53,8 @@ class DistillationLoss(nn.Module):
         base_loss = self.base_criterion(outputs, labels)
         if self.distillation_type == 'none':
             return base_loss
+        if outputs_kd is None and self.distillation_type == 'top':
+            outputs_kd = outputs
         if outputs_kd is None:
             raise ValueError('When knowledge distillation is enabled, the model is expected to return a Tuple[Tensor, Tensor] with the '
                              'output of the class_token and the dist_token')
@@ -42,7 +62,9 @@ class DistillationLoss(nn.Module):
             teacher_outputs = self.teacher_model(inputs)
             if isinstance(teacher_outputs, tuple):
                 teacher_outputs = teacher_outputs[0]
-        if self.distillation_type == 'soft':                             # losses.py:50-59
+        if self.distillation_type == 'top':
+            distillation_loss = self.top(outputs_kd, *self.top.store(teacher_outputs.to(outputs_kd.dtype)))
+        elif self.distillation_type == 'soft':                           # losses.py:50-59
             T = self.tau
             log_s = torch.log_softmax(outputs_kd.float() / T, dim=1)
             log_t = torch.log_softmax(teacher_outputs.float() / T, dim=1)

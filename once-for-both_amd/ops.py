@@ -1084,6 +1084,21 @@ def relpos_attention_qkv(qkv, table, buckets, scale=None, causal=False, key_lens
     return call.forward(*(_att_operand(t) for t in qkv.unbind(2)), _c(table), key_lens, False)[0]
 
 
+def relpos_attn_branch(x, resid, wqkv, bqkv, wproj, bproj, table, buckets, rowscale, heads, scale):
+    """resid + rowscale[token] * proj(relpos_attention(qkv(x))): the attention branch of a block with a relative position bias"""
+    B, N, D = x.shape
+    x2d = _c(x).reshape(B * N, D)
+    pm = getattr(x, '_ofb_p', None)                        # the LayerNorm's planes are the qkv product's operand as they are
+    if pm is not None:
+        x2d._ofb_p = pm
+    qkv = Linear.apply(x2d, wqkv, bqkv)
+    o = relpos_attention_qkv(qkv.view(B, N, 3, heads, wqkv.shape[0] // 3 // heads), table, buckets, scale=scale)
+    y = Linear.apply(o.reshape(B * N, -1), wproj, bproj)
+    if rowscale is not None:                               # one factor per token, or per sample
+        y = (y.view(rowscale.numel(), -1) * rowscale.reshape(-1, 1)).view(B * N, D)
+    return resid + y.view(B, N, D)
+
+
 # ---------------------------------------------------------------------------------------------------
 # distillation from a teacher's top logits (csrc/distill.hip)
 # ---------------------------------------------------------------------------------------------------

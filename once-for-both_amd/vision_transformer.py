@@ -9,6 +9,7 @@ import torch
 import torch.nn as nn
 
 from . import hip, ops
+from .relpos import RelPosBuckets
 from .layers import (Attention, DropPath, drop_path_scale, LayerNorm, MAEPatchEmbed, MAESparseAttention, MAESparseMlp, Mlp, ModuleInjection,
                      PatchEmbed, reduce_tensor, trunc_normal_)
 
@@ -111,10 +112,10 @@ class Block(nn.Module):
     fused into the branch GEMMs / LayerNorm backward."""
 
     def __init__(self, dim, num_heads, mlp_ratio=4., qkv_bias=False, qk_scale=None, drop=0., attn_drop=0., drop_path=0.,
-                 act_layer=nn.GELU, norm_layer=LayerNorm):
+                 act_layer=nn.GELU, norm_layer=LayerNorm, rel_pos=None):
         super().__init__()
         self.norm1 = norm_layer(dim)
-        self.attn = Attention(dim, num_heads=num_heads, qkv_bias=qkv_bias, qk_scale=qk_scale, attn_drop=attn_drop, proj_drop=drop)
+        self.attn = Attention(dim, num_heads=num_heads, qkv_bias=qkv_bias, qk_scale=qk_scale, attn_drop=attn_drop, proj_drop=drop, rel_pos=rel_pos)
         self.drop_path = DropPath(drop_path) if drop_path > 0. else nn.Identity()
         self.norm2 = norm_layer(dim)
         self.mlp = Mlp(in_features=dim, hidden_features=int(dim * mlp_ratio), act_layer=act_layer, drop=drop)
@@ -123,7 +124,10 @@ class Block(nn.Module):
         return drop_path_scale(self.drop_path, x.shape[0], x.device, u, tokens=x.shape[1])
 
     def forward(self, x):
-        y, xr = ops.layer_norm_fork(x, self.norm1.weight, self.norm1.bias, self.norm1.eps)
+        if getattr(self.attn, 'rel_pos', None) is not None:      # that branch reads the LayerNorm's rows, which the fork does not write
+            y, xr = ops.layer_norm(x, self.norm1.weight, self.norm1.bias, self.norm1.eps), x
+        else:
+            y, xr = ops.layer_norm_fork(x, self.norm1.weight, self.norm1.bias, self.norm1.eps)
         x = self.attn._branch(y, xr, None, self._row_scale(x), self.attn.num_heads)
         y, xr = ops.layer_norm_fork(x, self.norm2.weight, self.norm2.bias, self.norm2.eps)
         return self.mlp._branch(y, xr, None, self._row_scale(x))
@@ -193,11 +197,13 @@ class MAEBlock(nn.Module):
 
 
 class VisionTransformer(nn.Module):
-    """pruned-subnet / plain ViT of the finetune path (reference :222-377)."""
+    """pruned-subnet / plain ViT of the finetune path (reference :222-377).  rel_pos_bias: every block's attention also learns a bias per head
+    and relative position on the patch grid (class token: buckets of its own)."""
 
     def __init__(self, img_size=224, patch_size=16, in_chans=3, num_classes=1000, embed_dim=768, depth=12, num_heads=12,
                  mlp_ratio=4., qkv_bias=True, qk_scale=None, representation_size=None, distilled=False, drop_rate=0.,
-                 attn_drop_rate=0., drop_path_rate=0., embed_layer=PatchEmbed, norm_layer=None, act_layer=None, weight_init=''):
+                 attn_drop_rate=0., drop_path_rate=0., embed_layer=PatchEmbed, norm_layer=None, act_layer=None, weight_init='',
+                 rel_pos_bias=False):
         super().__init__()
         if distilled or representation_size:
             raise NotImplementedError('distilled / representation_size variants are not on the OFB path')
@@ -211,10 +217,13 @@ class VisionTransformer(nn.Module):
         self.dist_token = None
         self.pos_embed = nn.Parameter(torch.zeros(1, num_patches + 1, embed_dim))
         self.pos_drop = nn.Dropout(p=drop_rate)
+        rel_pos = None
+        if rel_pos_bias:
+            rel_pos = RelPosBuckets.grid(*self.patch_embed.grid_size, cls_token=True)
         dpr = [x.item() for x in torch.linspace(0, drop_path_rate, depth)]
         self.blocks = nn.Sequential(*[
             Block(dim=embed_dim, num_heads=num_heads, mlp_ratio=mlp_ratio, qkv_bias=qkv_bias, qk_scale=qk_scale, drop=drop_rate,
-                  attn_drop=attn_drop_rate, drop_path=dpr[i], norm_layer=norm_layer, act_layer=act_layer or nn.GELU)
+                  attn_drop=attn_drop_rate, drop_path=dpr[i], norm_layer=norm_layer, act_layer=act_layer or nn.GELU, rel_pos=rel_pos)
             for i in range(depth)])
         self.norm = norm_layer(embed_dim)
         self.pre_logits = nn.Identity()
