@@ -247,7 +247,7 @@ __device__ __forceinline__ int rp_bias4(int w_first, int d0, int width, float (&
 // A workgroup owns 128 queries of one head (a wave 32 of them, query on the lane), keys stream through two LDS stages.  S^T = K Q^T has
 // keys along the registers, so the softmax of a row is register-local but for one exchange between lane halves, and P^T is the B operand of
 // O^T = V^T P^T as it stands.
-template <int DT, int DP, bool SPLIT>
+template <int DT, int DP, bool POS, bool SPLIT>
 __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 2)) void relpos_fwd_kernel(ofb_relpos_args a) {
   using G = rp_geo<DT, DP>;
   constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
@@ -279,7 +279,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 
   auto fetch = [&](int kb) {
     ks_.load(kp, a.k_st * ES, kb * KB, kend, a.d);
     vs_.load(vp, a.v_st * ES, kb * KB, kend, a.d);
-    if (a.pos_k && threadIdx.x < KB) { const int j = kb * KB + threadIdx.x; pk_next = j < kend ? 4 * a.pos_k[j] : 0; }
+    if (POS && threadIdx.x < KB) { const int j = kb * KB + threadIdx.x; pk_next = j < kend ? 4 * a.pos_k[j] : 0; }
   };
   if (kb0 < kb1) fetch(kb0);
   rp_bias_vector(a, head, w);
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 
 
   const int q0 = qt * RP_TILE + wv * 32, qi = q0 + (lane & 31);
   const bool active = q0 < a.Nq, qok = qi < a.Nq;
-  const int pq = a.pos_q ? (qok ? a.pos_q[qi] : 0) : qi + a.q_offset;
+  const int pq = POS ? (qok ? a.pos_q[qi] : 0) : qi + a.q_offset;
   const int seen = a.causal ? min(kend, max(0, qi + a.q_offset + 1)) : kend;      // this query sees keys 0 .. seen - 1
   rp_frag qf[DP / 16][NP];
 #pragma unroll
@@ -314,7 +314,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 
   auto commit = [&](int buf) {
     ks_.store(tiles + buf * G::STAGE, hk);
     vs_.store(tiles + buf * G::STAGE + G::TENSOR, hv);
-    if (a.pos_k && threadIdx.x < KB) pk[buf * KB + threadIdx.x] = pk_next;
+    if (POS && threadIdx.x < KB) pk[buf * KB + threadIdx.x] = pk_next;
   };
   if (kb0 < kb1) commit(0);
   __syncthreads();
@@ -342,10 +342,10 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 
       float bt = 0.f, c_t = 1.f;
       const float wc = w[RP_PAD + (dmax <= lo ? 0 : width - 1)];
       // (a bias that swallows the scores, and a scale that is not positive, take the general form)
-      if (!a.pos_k && (dmax <= lo || dmin >= hi) && fabsf(wc) < 1e30f && c_s > 0.f) {
+      if (!POS && (dmax <= lo || dmin >= hi) && fabsf(wc) < 1e30f && c_s > 0.f) {
         bt = wc;
         c_t = c_s;
-      } else if (a.pos_k) {
+      } else if constexpr (POS) {
 #pragma unroll
         for (int t = 0; t < KB / 32; ++t)
 #pragma unroll
@@ -509,7 +509,7 @@ __device__ __forceinline__ rp_scales rp_all_scales(const ofb_relpos_args& a, flo
 // only known when a row is done (see below): the tiles with pairs between the ends are then visited once more, for S and dP alone.  (A pass of its own
 // that summed dS over the batch first, one histogram per pair of tiles, took 170 us beside 98 us of this kernel for the 14 x 14 grid, B 128, 6 x 64
 // f32, where this takes 124 us.)
-template <int DT, int DP>
+template <int DT, int DP, bool POS>
 __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 || DT == RP_F32 ? 2 : RP_OQ)) void relpos_dq_kernel(ofb_relpos_args a) {
   using G = rp_geo<DT, DP>;
   constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
@@ -537,7 +537,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
   auto fetch = [&](int kb) {
     ks_.load(kp, a.k_st * ES, kb * KB, kend, a.d);
     vs_.load(vp, a.v_st * ES, kb * KB, kend, a.d);
-    if (a.pos_k && threadIdx.x < KB) { const int j = kb * KB + threadIdx.x; pk_next = j < kend ? 4 * a.pos_k[j] : 0; }
+    if (POS && threadIdx.x < KB) { const int j = kb * KB + threadIdx.x; pk_next = j < kend ? 4 * a.pos_k[j] : 0; }
   };
   if (kb1 > 0) fetch(0);
   rp_bias_vector(a, head, w);
@@ -550,7 +550,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
 
   const int q0 = qt * RP_TILE + wv * 32, qi = q0 + (lane & 31);
   const bool active = q0 < a.Nq, qok = qi < a.Nq;
-  const int pq = a.pos_q ? (qok ? a.pos_q[qi] : 0) : qi + a.q_offset;
+  const int pq = POS ? (qok ? a.pos_q[qi] : 0) : qi + a.q_offset;
   const int seen = a.causal ? min(kend, max(0, qi + a.q_offset + 1)) : kend;
   rp_frag qf[DP / 16][NP], df[DP / 16][NP];
   float D = 0.f, m = 0.f, linv = 0.f;
@@ -586,7 +586,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
   auto commit = [&](int buf) {
     ks_.store(tiles + buf * G::STAGE, hk);
     vs_.store(tiles + buf * G::STAGE + G::TENSOR, hv);
-    if (a.pos_k && threadIdx.x < KB) pk[buf * KB + threadIdx.x] = pk_next;
+    if (POS && threadIdx.x < KB) pk[buf * KB + threadIdx.x] = pk_next;
   };
   if (kb1 > 0) commit(0);
   __syncthreads();
@@ -610,7 +610,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
   // at: the LDS addresses of the pairs' biases.
   auto general = [&](f32x16& S, f32x16& dP, int buf, int t0, int j0, bool whole, float (&ds)[16], int (&at)[16]) {
     float t[16];
-    if (a.pos_k) {
+    if constexpr (POS) {
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
         const int4 pj = *reinterpret_cast<const int4*>(&pk[buf * KB + 32 * t0 + rp_row(r, hh)]);
@@ -654,7 +654,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
   auto is_whole = [&](int j0, int n, int first) { return j0 + n <= kend && (!a.causal || j0 + n - 1 <= first + a.q_offset); };
   // the whole tile of keys j0 .. j0 + n - 1 and queries first .. last lies beyond an end: -1, 1 or 0
   auto beyond = [&](int j0, int n, int first, int last) {
-    return a.pos_k ? 0 : j0 + n - 1 - first - a.q_offset <= lo ? -1 : j0 - last - a.q_offset >= hi ? 1 : 0;
+    return POS ? 0 : j0 + n - 1 - first - a.q_offset <= lo ? -1 : j0 - last - a.q_offset >= hi ? 1 : 0;
   };
   float most = 0.f;                                            // the largest |ds| that goes to a bin
   for (int kb = 0; kb < kb1; ++kb) {
@@ -671,7 +671,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
       const bool whole = is_whole(j0, 32, q0);
       const int side = beyond(j0, 32, q0, q0 + 31);
       float ds[16], sum = 0.f;
-      if (whole && side) {
+      if (!POS && whole && side) {
         const float tb = w[RP_PAD + (side < 0 ? 0 : width - 1)] - mk;
         float psum = 0.f;
 #pragma unroll
@@ -794,7 +794,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
 
 // a query tile's row statistics for LDS: the maximum (with the sum's logarithm and the operand's scale 2^pe in it, or for f32 apart), the factor,
 // -D in dP's scale 2^de; a row without keys or behind the last query gets P = 0
-template <int DT, int KB>
+template <int DT, int KB, bool POS>
 __device__ __forceinline__ void rp_row_stats(const ofb_relpos_args& a, int64_t bh, int row0, int pe, int de, f32x4& v, int& pos) {
   const int i = row0 + threadIdx.x;
   v = f32x4{DT == RP_F32 ? 0.f : INFINITY, 0.f, 0.f, 0.f};
@@ -805,14 +805,14 @@ __device__ __forceinline__ void rp_row_stats(const ofb_relpos_args& a, int64_t b
     if constexpr (DT == RP_F32) { v[0] = m; v[1] = __builtin_ldexpf(l, pe); }
     else v[0] = l > 0.f ? m - __log2f(l) - (float)pe : l == 0.f ? INFINITY : l;
     v[2] = -__builtin_ldexpf(a.delta[row], de);
-    pos = a.pos_q ? 4 * a.pos_q[i] : i + a.q_offset;
+    pos = POS ? 4 * a.pos_q[i] : i + a.q_offset;
   }
 }
 
 // P and dS of a 32 x 32 tile, rows = queries i0 .. (LDS tiles qt_ and dt_ at row tr), the wave's key on the lane.  st: row statistics m, l, -D of
 // the tile's queries, P = exp2(s - m) (times l for f32; l is in m otherwise), -D in dP's scale.  P comes out times the p_sc that is in the statistics,
 // dS = P dP times that and dP's scale.
-template <int DT, int DP>
+template <int DT, int DP, bool POS>
 __device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char* qt_, const char* dt_, int tr, const rp_frag (&kf)[DP / 16][rp_type<DT>::NP],
                                            const rp_frag (&vf)[DP / 16][rp_type<DT>::NP], const float* st, const int* ps, const float* w, int i0, int j0,
                                            int kj, int pkj, bool kok, bool kwhole, float c_s, float (&P)[16], float (&dS)[16]) {
@@ -838,11 +838,11 @@ __device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char*
   const int dmax = j0 + 31 - i0 - a.q_offset, dmin = j0 - (i0 + 31) - a.q_offset;
   const bool cut = a.causal && j0 + 31 > i0 + a.q_offset;
   float t[16];
-  if (!a.pos_q && (dmax <= lo || dmin >= hi)) {
+  if (!POS && (dmax <= lo || dmin >= hi)) {
     const float wc = w[RP_PAD + (dmax <= lo ? 0 : width - 1)];
 #pragma unroll
     for (int r = 0; r < 16; ++r) t[r] = wc;
-  } else if (a.pos_q) {
+  } else if constexpr (POS) {
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
       const int4 pi = *reinterpret_cast<const int4*>(&ps[tr + rp_row(r, hh)]);
@@ -883,7 +883,7 @@ __device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char*
 
 // dK and dV: a workgroup owns 128 keys of one head (a wave 32, key on the lane, K and V in registers), queries stream through LDS.
 // S = Q K^T and dP = dO V^T have queries along the registers: P and dS are the B operands of dV^T = dO^T P and dK^T = Q^T dS.
-template <int DT, int DP>
+template <int DT, int DP, bool POS>
 __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OK : 1)) void relpos_dkv_kernel(ofb_relpos_args a) {
   using G = rp_geo<DT, DP>;
   constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
@@ -912,7 +912,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OK : 1)) void relpos_dkv
   auto fetch = [&](int qb) {
     qs_.load(qp, a.q_st * ES, qb * KB, a.Nq, a.d);
     ds_.load(dp, a.do_st * ES, qb * KB, a.Nq, a.d);
-    rp_row_stats<DT, KB>(a, bh, qb * KB, DT == RP_BF16 ? 0 : RP_PE, e.ed + e.ev, st_next, ps_next);
+    rp_row_stats<DT, KB, POS>(a, bh, qb * KB, DT == RP_BF16 ? 0 : RP_PE, e.ed + e.ev, st_next, ps_next);
   };
   rp_bias_vector(a, head, w);
   if (qb0 < qb1) fetch(qb0);
@@ -924,7 +924,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OK : 1)) void relpos_dkv
 
   const int j0 = j_first + wv * 32, kj = j0 + (lane & 31);
   const bool active = j0 < kend, kok = kj < kend;
-  const int pkj = a.pos_k ? (kok ? a.pos_k[kj] : 0) : kj;
+  const int pkj = POS ? (kok ? a.pos_k[kj] : 0) : kj;
   rp_frag kf[DP / 16][NP], vf[DP / 16][NP];
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
@@ -961,7 +961,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OK : 1)) void relpos_dkv
       const int i0 = qb * KB + 32 * t;
       if (!active || i0 >= a.Nq || (a.causal && j0 > i0 + 31 + a.q_offset)) continue;
       float P[16], dS[16];
-      rp_tile_ds<DT, DP>(a, qt_, dt_, 32 * t, kf, vf, st + buf * 3 * KB, ps + buf * KB, w, i0, j0, kj, pkj, kok, j0 + 32 <= kend, c_s, P, dS);
+      rp_tile_ds<DT, DP, POS>(a, qt_, dt_, 32 * t, kf, vf, st + buf * 3 * KB, ps + buf * KB, w, i0, j0, kj, pkj, kok, j0 + 32 <= kend, c_s, P, dS);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         float p8[8], x8[8];
@@ -1118,30 +1118,33 @@ int rp_check(const ofb_relpos_args* a) {
   return OFB_OK;
 }
 
-template <int DT, int DP> int rp_forward(const ofb_relpos_args& a, hipStream_t s) {
+template <int DT, int DP, bool POS> int rp_forward_of(const ofb_relpos_args& a, hipStream_t s) {
   const int64_t wgs = (int64_t)a.B * a.H * ((a.Nq + RP_TILE - 1) / RP_TILE);
   const int lds = rp_lds<DT, DP>(a, 0), splits = rp_splits(a);
   if (splits > 1) {
     if (!a.split_o || !a.split_ml) return OFB_EINVAL;
-    RP_LAUNCH((relpos_fwd_kernel<DT, DP, true>), dim3((unsigned)wgs, splits), lds, s, a);
+    RP_LAUNCH((relpos_fwd_kernel<DT, DP, POS, true>), dim3((unsigned)wgs, splits), lds, s, a);
     const int64_t rows = (int64_t)a.B * a.H * a.Nq;
     hipLaunchKernelGGL((relpos_join_kernel<DT>), dim3((unsigned)((rows + 3) / 4)), dim3(RP_THREADS), 0, s, a, splits);
   } else {
-    RP_LAUNCH((relpos_fwd_kernel<DT, DP, false>), dim3((unsigned)wgs), lds, s, a);
+    RP_LAUNCH((relpos_fwd_kernel<DT, DP, POS, false>), dim3((unsigned)wgs), lds, s, a);
   }
   return ofb_launch_status();
 }
 
-template <int DT, int DP> int rp_backward(const ofb_relpos_args& a, hipStream_t s) {
+template <int DT, int DP, bool POS> int rp_backward_of(const ofb_relpos_args& a, hipStream_t s) {
   const int nqt = (a.Nq + RP_TILE - 1) / RP_TILE, nkt = (a.Nk + RP_TILE - 1) / RP_TILE;
-  RP_LAUNCH((relpos_dq_kernel<DT, DP>), dim3((unsigned)((int64_t)a.B * a.H * nqt)), (rp_lds<DT, DP>(a, 1)), s, a);
-  RP_LAUNCH((relpos_dkv_kernel<DT, DP>), dim3((unsigned)((int64_t)a.B * a.H * nkt)), (rp_lds<DT, DP>(a, 2)), s, a);
+  RP_LAUNCH((relpos_dq_kernel<DT, DP, POS>), dim3((unsigned)((int64_t)a.B * a.H * nqt)), (rp_lds<DT, DP>(a, 1)), s, a);
+  RP_LAUNCH((relpos_dkv_kernel<DT, DP, POS>), dim3((unsigned)((int64_t)a.B * a.H * nkt)), (rp_lds<DT, DP>(a, 2)), s, a);
   if (a.dtable) {
     hipLaunchKernelGGL(relpos_table_kernel, dim3((unsigned)(((int64_t)a.n_buckets * a.H + 3) / 4)), dim3(RP_THREADS), 0, s, a, rp_table_rows(a),
                        a.pos_k ? (int64_t)0 : (int64_t)a.B * nqt * 4);
   }
   return ofb_launch_status();
 }
+
+template <int DT, int DP> int rp_forward(const ofb_relpos_args& a, hipStream_t s) { return a.pos_k ? rp_forward_of<DT, DP, true>(a, s) : rp_forward_of<DT, DP, false>(a, s); }
+template <int DT, int DP> int rp_backward(const ofb_relpos_args& a, hipStream_t s) { return a.pos_k ? rp_backward_of<DT, DP, true>(a, s) : rp_backward_of<DT, DP, false>(a, s); }
 
 #define RP_BY_TYPE(fn, a, s)                                                                                          \
   switch ((a).dtype * 3 + ((a).d <= 32 ? 0 : (a).d <= 64 ? 1 : 2)) {                                                  \
