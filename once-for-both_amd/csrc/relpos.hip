@@ -189,6 +189,20 @@ __device__ __forceinline__ void rp_cols(const char* lds, int row0, int ct, int l
 
 struct rp_scales { int eq, ek, ev, ed, es; };
 
+// The workgroup's tile and head.  Neighbouring tiles of a head share an L2 (its keys or queries are streamed by all of them); causal tiles differ in
+// length, so there the longest of all heads come first, and a head stays on one XCD where the number of heads is a multiple of eight.
+__device__ __forceinline__ void rp_place(int x, int total, int tiles, bool causal, int& tile, int& bh) {
+  if (causal) {
+    const int heads = total / tiles;
+    tile = x / heads;
+    bh = x - tile * heads;
+  } else {
+    const int id = ofb_xcd_remap(x, total);
+    bh = id / tiles;
+    tile = id - bh * tiles;
+  }
+}
+
 // maxima of N tensors from their partial maxima (n of each <= RP_NBOUND), by every thread of the workgroup; red: [4][N]
 template <int N>
 __device__ __forceinline__ void rp_bounds(const float* const (&part)[N], const int (&n)[N], float (&out)[N], float* red) {
@@ -258,8 +272,10 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 
   char* tiles = reinterpret_cast<char*>(pk + 2 * KB);
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const int nqt = (a.Nq + RP_TILE - 1) / RP_TILE;
-  const int id = ofb_xcd_remap(blockIdx.x, gridDim.x);
-  const int qt = id % nqt, bh = id / nqt, head = bh % a.H, b = bh / a.H;
+  int qt, bh;
+  rp_place(blockIdx.x, gridDim.x, nqt, a.causal, qt, bh);
+  if (a.causal) qt = nqt - 1 - qt;                             // the last queries see the most keys
+  const int head = bh % a.H, b = bh / a.H;
   const char* qp = (const char*)a.q + (b * a.q_sb + head * a.q_sh) * ES;
   const char* kp = (const char*)a.k + (b * a.k_sb + head * a.k_sh) * ES;
   const char* vp = (const char*)a.v + (b * a.v_sb + head * a.v_sh) * ES;
@@ -522,8 +538,10 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
   char* tiles = reinterpret_cast<char*>(pk + 2 * KB);
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const int nqt = (a.Nq + RP_TILE - 1) / RP_TILE;
-  const int id = ofb_xcd_remap(blockIdx.x, gridDim.x);
-  const int qt = id % nqt, bh = id / nqt, head = bh % a.H, b = bh / a.H;
+  int qt, bh;
+  rp_place(blockIdx.x, gridDim.x, nqt, a.causal, qt, bh);
+  if (a.causal) qt = nqt - 1 - qt;                             // the last queries see the most keys
+  const int head = bh % a.H, b = bh / a.H;
   const char* qp = (const char*)a.q + (b * a.q_sb + head * a.q_sh) * ES;
   const char* kp = (const char*)a.k + (b * a.k_sb + head * a.k_sh) * ES;
   const char* vp = (const char*)a.v + (b * a.v_sb + head * a.v_sh) * ES;
@@ -895,8 +913,9 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OK : 1)) void relpos_dkv
   char* tiles = reinterpret_cast<char*>(ps + 2 * KB);
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const int nkt = (a.Nk + RP_TILE - 1) / RP_TILE;
-  const int id = ofb_xcd_remap(blockIdx.x, gridDim.x);
-  const int kt = id % nkt, bh = id / nkt, head = bh % a.H, b = bh / a.H;
+  int kt, bh;
+  rp_place(blockIdx.x, gridDim.x, nkt, a.causal, kt, bh);
+  const int head = bh % a.H, b = bh / a.H;
   const char* qp = (const char*)a.q + (b * a.q_sb + head * a.q_sh) * ES;
   const char* kp = (const char*)a.k + (b * a.k_sb + head * a.k_sh) * ES;
   const char* vp = (const char*)a.v + (b * a.v_sb + head * a.v_sh) * ES;
