@@ -24,13 +24,6 @@
 #define RP_F16 2
 #define RP_THREADS 256
 #define RP_TILE 128              /* queries (forward, dQ) or keys (dK dV, table gradient) of a workgroup: four waves of 32 */
-#ifndef RP_UN_Q
-#define RP_UN_Q 2
-#define RP_UN_K 2
-#define RP_OQ 2
-#define RP_OK 2
-#define RP_OF 3
-#endif
 #define RP_PAD 4                 /* entries of w on either side, so that four consecutive differences need one clamp */
 #define RP_WMAX 4096
 #define RP_PE 14                 /* f16 planes hold P 2^14 */
@@ -47,10 +40,17 @@ typedef rp_s16x8 rp_frag;
 template <int DT> struct rp_type { static constexpr int NP = 1, ES = 2; };
 template <> struct rp_type<RP_F32> { static constexpr int NP = 2, ES = 4; };
 
-// rows of a streamed tile: 64, or 32 where two planes or wide heads would take the LDS of a second workgroup
-template <int DT, int DP> struct rp_geo {
+// Rows of a streamed tile of kernel 0 forward, 1 dQ, 2 dK dV.  More rows are fewer barriers, until the staging registers or the LDS cost a workgroup, or
+// they spill.  Measured both sides: 16-bit, d 64 (6007 tokens, 16 heads): forward 128 rows 246, 64 rows 213 us; dK dV 64 rows 553, 128 rows 521 us;
+// dQ alike.  16-bit, d 128 (4 x 1025 causal, 8 heads): forward 32 rows 47, 64 rows 41 us; dK dV 87 and 68 us; dQ 89 and 119 us.  f32, d 64 (14 x 14 grid,
+// B 128): 32 rows 59 / 113 / 101 us, 64 rows 87 / 165 / 101 us.
+template <int DT, int DP> constexpr int rp_rows_of(int kernel) {
+  constexpr int f32[3] = {32, 32, 32}, narrow[3] = {64, 64, 128}, wide[3] = {64, 32, 64};
+  return DT == RP_F32 ? f32[kernel] : DP <= 64 ? narrow[kernel] : wide[kernel];
+}
+template <int DT, int DP, int ROWS> struct rp_geo {
   static constexpr int NP = rp_type<DT>::NP;
-  static constexpr int KB = (rp_type<DT>::NP == 1 && DP <= 64) ? 64 : 32;
+  static constexpr int KB = ROWS;
   static constexpr int PITCH = DP * 2 + 16;                  // bytes of a row of one plane: 8 rows' 16-byte chunks fall into different banks
   static constexpr int PLANE = KB * PITCH;
   static constexpr int TENSOR = NP * PLANE;
@@ -140,9 +140,9 @@ __device__ __forceinline__ void rp_store4(char* p, float a, float b, float c, fl
 }
 
 // a [rows][DP] tile on its way from memory to LDS: one register image per thread, loaded a tile ahead
-template <int DT, int DP>
+template <int DT, int DP, int ROWS>
 struct rp_stage {
-  using G = rp_geo<DT, DP>;
+  using G = rp_geo<DT, DP, ROWS>;
   rp_chunk<DT> c[G::PER];
   __device__ __forceinline__ void load(const char* base, int64_t row_bytes, int row0, int row_end, int d) {
 #pragma unroll
@@ -166,17 +166,17 @@ struct rp_stage {
 };
 
 // A operand from an LDS tile, rows along the tile's rows: k-step ks of row0 + (l & 31)
-template <int DT, int DP>
+template <int DT, int DP, int ROWS>
 __device__ __forceinline__ void rp_rows(const char* lds, int row0, int ks, int lane, rp_frag (&out)[rp_type<DT>::NP]) {
-  using G = rp_geo<DT, DP>;
+  using G = rp_geo<DT, DP, ROWS>;
 #pragma unroll
   for (int p = 0; p < G::NP; ++p) out[p] = *reinterpret_cast<const rp_frag*>(lds + p * G::PLANE + (row0 + (lane & 31)) * G::PITCH + (2 * ks + (lane >> 5)) * 16);
 }
 // A operand from an LDS tile, rows along the tile's columns (channels 32 ct ..), k-slots = tile rows row0 + 8 (j >> 2) + 4 hh + (j & 3).
 // ds_read_b64_tr_b16: in each group of 16 lanes, lane 4 e + q addresses four channels of row e, lane i receives four rows of channel i.
-template <int DT, int DP>
+template <int DT, int DP, int ROWS>
 __device__ __forceinline__ void rp_cols(const char* lds, int row0, int ct, int lane, rp_frag (&out)[rp_type<DT>::NP]) {
-  using G = rp_geo<DT, DP>;
+  using G = rp_geo<DT, DP, ROWS>;
   const int off = (row0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * G::PITCH + (32 * ct + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
 #pragma unroll
   for (int p = 0; p < G::NP; ++p) {
@@ -262,8 +262,8 @@ __device__ __forceinline__ int rp_bias4(int w_first, int d0, int width, float (&
 // keys along the registers, so the softmax of a row is register-local but for one exchange between lane halves, and P^T is the B operand of
 // O^T = V^T P^T as it stands.
 template <int DT, int DP, bool POS, bool SPLIT>
-__global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 2)) void relpos_fwd_kernel(ofb_relpos_args a) {
-  using G = rp_geo<DT, DP>;
+__global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 3 : DT == RP_F32 ? 1 : 2)) void relpos_fwd_kernel(ofb_relpos_args a) {
+  using G = rp_geo<DT, DP, rp_rows_of<DT, DP>(0)>;
   constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float red[16];
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 
     kb1 = min(kb1, kb0 + per);
   }
 
-  rp_stage<DT, DP> ks_, vs_;
+  rp_stage<DT, DP, KB> ks_, vs_;
   int pk_next = 0;
   auto fetch = [&](int kb) {
     ks_.load(kp, a.k_st * ES, kb * KB, kend, a.d);
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) {
           rp_frag kf[NP];
-          rp_rows<DT, DP>(kt_, 32 * t, s, lane, kf);
+          rp_rows<DT, DP, KB>(kt_, 32 * t, s, lane, kf);
           S[t] = rp_mm<DT, NP>(kf, qf[s], S[t]);
         }
       }
@@ -422,7 +422,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OF : DT == RP_F32 ? 1 : 
 #pragma unroll
           for (int ct = 0; ct < DP / 32; ++ct) {
             rp_frag vf[NP];
-            rp_cols<DT, DP>(vt_, 32 * t + 16 * s, ct, lane, vf);
+            rp_cols<DT, DP, KB>(vt_, 32 * t + 16 * s, ct, lane, vf);
             O[ct] = rp_mm<DT, NP>(vf, pf, O[ct]);
           }
         }
@@ -526,8 +526,8 @@ __device__ __forceinline__ rp_scales rp_all_scales(const ofb_relpos_args& a, flo
 // that summed dS over the batch first, one histogram per pair of tiles, took 170 us beside 98 us of this kernel for the 14 x 14 grid, B 128, 6 x 64
 // f32, where this takes 124 us.)
 template <int DT, int DP, bool POS>
-__global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 || DT == RP_F32 ? 2 : RP_OQ)) void relpos_dq_kernel(ofb_relpos_args a) {
-  using G = rp_geo<DT, DP>;
+__global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : 2)) void relpos_dq_kernel(ofb_relpos_args a) {
+  using G = rp_geo<DT, DP, rp_rows_of<DT, DP>(1)>;
   constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float red[16];
@@ -550,7 +550,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
   const int q_last = min(a.Nq, (qt + 1) * RP_TILE) - 1;
   if (a.causal) kend = min(kend, max(0, q_last + a.q_offset + 1));
   const int kb1 = (kend + KB - 1) / KB;
-  rp_stage<DT, DP> ks_, vs_;
+  rp_stage<DT, DP, KB> ks_, vs_;
   int pk_next = 0;
   auto fetch = [&](int kb) {
     ks_.load(kp, a.k_st * ES, kb * KB, kend, a.d);
@@ -617,8 +617,8 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
       rp_frag kf[NP], vf[NP];
-      rp_rows<DT, DP>(kt_, 32 * t0, s, lane, kf);
-      rp_rows<DT, DP>(vt_, 32 * t0, s, lane, vf);
+      rp_rows<DT, DP, KB>(kt_, 32 * t0, s, lane, kf);
+      rp_rows<DT, DP, KB>(vt_, 32 * t0, s, lane, vf);
       S = rp_mm<DT, NP>(kf, qf[s], S);
       dP = rp_mm<DT, NP>(vf, df[s], dP);
     }
@@ -680,7 +680,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
     const char* kt_ = tiles + buf * G::STAGE;
     const char* vt_ = kt_ + G::TENSOR;
     if (kb + 1 < kb1) fetch(kb + 1);
-#pragma unroll RP_UN_Q
+#pragma unroll 2
     for (int t0 = 0; t0 < KB / 32; ++t0) {
       const int j0 = kb * KB + 32 * t0;
       if (!visible(j0)) continue;
@@ -724,7 +724,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : DP > 64 
 #pragma unroll
         for (int ct = 0; ct < DP / 32; ++ct) {
           rp_frag kf[NP];
-          rp_cols<DT, DP>(kt_, 32 * t0 + 16 * s, ct, lane, kf);
+          rp_cols<DT, DP, KB>(kt_, 32 * t0 + 16 * s, ct, lane, kf);
           dQ[ct] = rp_mm<DT, NP>(kf, xf, dQ[ct]);
         }
       }
@@ -830,11 +830,11 @@ __device__ __forceinline__ void rp_row_stats(const ofb_relpos_args& a, int64_t b
 // P and dS of a 32 x 32 tile, rows = queries i0 .. (LDS tiles qt_ and dt_ at row tr), the wave's key on the lane.  st: row statistics m, l, -D of
 // the tile's queries, P = exp2(s - m) (times l for f32; l is in m otherwise), -D in dP's scale.  P comes out times the p_sc that is in the statistics,
 // dS = P dP times that and dP's scale.
-template <int DT, int DP, bool POS>
+template <int DT, int DP, int ROWS, bool POS>
 __device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char* qt_, const char* dt_, int tr, const rp_frag (&kf)[DP / 16][rp_type<DT>::NP],
                                            const rp_frag (&vf)[DP / 16][rp_type<DT>::NP], const float* st, const int* ps, const float* w, int i0, int j0,
                                            int kj, int pkj, bool kok, bool kwhole, float c_s, float (&P)[16], float (&dS)[16]) {
-  using G = rp_geo<DT, DP>;
+  using G = rp_geo<DT, DP, ROWS>;
   constexpr int NP = G::NP, KB = G::KB;
   const int lane = threadIdx.x & 63, hh = lane >> 5, lo = a.lo, width = a.width, hi = lo + width - 1, w_first = rp_lds_base(w),
             w_last = w_first + 4 * (width - 1), pk4 = 4 * (pkj - lo) + w_first;
@@ -848,8 +848,8 @@ __device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char*
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
     rp_frag qa[NP], da[NP];
-    rp_rows<DT, DP>(qt_, tr, s, lane, qa);
-    rp_rows<DT, DP>(dt_, tr, s, lane, da);
+    rp_rows<DT, DP, KB>(qt_, tr, s, lane, qa);
+    rp_rows<DT, DP, KB>(dt_, tr, s, lane, da);
     S = rp_mm<DT, NP>(qa, kf[s], S);
     dP = rp_mm<DT, NP>(da, vf[s], dP);
   }
@@ -902,8 +902,8 @@ __device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char*
 // dK and dV: a workgroup owns 128 keys of one head (a wave 32, key on the lane, K and V in registers), queries stream through LDS.
 // S = Q K^T and dP = dO V^T have queries along the registers: P and dS are the B operands of dV^T = dO^T P and dK^T = Q^T dS.
 template <int DT, int DP, bool POS>
-__global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OK : 1)) void relpos_dkv_kernel(ofb_relpos_args a) {
-  using G = rp_geo<DT, DP>;
+__global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 2 : 1)) void relpos_dkv_kernel(ofb_relpos_args a) {
+  using G = rp_geo<DT, DP, rp_rows_of<DT, DP>(2)>;
   constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float red[16];
@@ -925,7 +925,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OK : 1)) void relpos_dkv
   if (a.causal) qb0 = min(qb1, max(0, j_first - a.q_offset) / KB);
   if (j_first >= kend) qb0 = qb1;                              // nobody sees these keys: their gradients are zeros
   const rp_scales e = rp_all_scales<DT>(a, red);
-  rp_stage<DT, DP> qs_, ds_;
+  rp_stage<DT, DP, KB> qs_, ds_;
   f32x4 st_next;
   int ps_next;
   auto fetch = [&](int qb) {
@@ -975,12 +975,12 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OK : 1)) void relpos_dkv
     const char* qt_ = tiles + buf * G::STAGE;
     const char* dt_ = qt_ + G::TENSOR;
     if (qb + 1 < qb1) fetch(qb + 1);
-#pragma unroll RP_UN_K
+#pragma unroll 2
     for (int t = 0; t < KB / 32; ++t) {
       const int i0 = qb * KB + 32 * t;
       if (!active || i0 >= a.Nq || (a.causal && j0 > i0 + 31 + a.q_offset)) continue;
       float P[16], dS[16];
-      rp_tile_ds<DT, DP, POS>(a, qt_, dt_, 32 * t, kf, vf, st + buf * 3 * KB, ps + buf * KB, w, i0, j0, kj, pkj, kok, j0 + 32 <= kend, c_s, P, dS);
+      rp_tile_ds<DT, DP, KB, POS>(a, qt_, dt_, 32 * t, kf, vf, st + buf * 3 * KB, ps + buf * KB, w, i0, j0, kj, pkj, kok, j0 + 32 <= kend, c_s, P, dS);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         float p8[8], x8[8];
@@ -992,8 +992,8 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OK : 1)) void relpos_dkv
 #pragma unroll
         for (int ct = 0; ct < DP / 32; ++ct) {
           rp_frag df[NP], qf[NP];
-          rp_cols<DT, DP>(dt_, 32 * t + 16 * s, ct, lane, df);
-          rp_cols<DT, DP>(qt_, 32 * t + 16 * s, ct, lane, qf);
+          rp_cols<DT, DP, KB>(dt_, 32 * t + 16 * s, ct, lane, df);
+          rp_cols<DT, DP, KB>(qt_, 32 * t + 16 * s, ct, lane, qf);
           dV[ct] = rp_mm<DT, NP>(df, pf, dV[ct]);
           dK[ct] = rp_mm<DT, NP>(qf, xf, dK[ct]);
         }
@@ -1017,26 +1017,30 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? RP_OK : 1)) void relpos_dkv
     }
 }
 
-// table gradient: one wave per (bucket, head) adds up the differences of its bucket over all workgroups, in a fixed order and in 64 bits
+// table gradient: one workgroup per (bucket, head) adds up the differences of its bucket over all workgroups of the dQ kernel, in a fixed order and in
+// 64 bits.  (difference, workgroup) pairs are dealt out together: buckets hold from one difference to dozens.
 __global__ __launch_bounds__(RP_THREADS) void relpos_table_kernel(ofb_relpos_args a, int64_t rows, int64_t nsat) {
-  const int lane = threadIdx.x & 63, id = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (id >= a.n_buckets * a.H) return;
-  const int c = id / a.H, head = id % a.H;
+  __shared__ double red[4];
+  const int c = blockIdx.x / a.H, head = blockIdx.x % a.H, e0 = a.bucket_start[c];
+  const int64_t items = (a.bucket_start[c + 1] - e0) * rows;
   double sum = 0.0;
-  for (int e = a.bucket_start[c]; e < a.bucket_start[c + 1]; ++e) {
-    const int i = a.bucket_order[e];
-    if (nsat > 0) {                                            // beyond the ends (a single difference takes both sides)
-      for (int side = i == 0 ? 0 : 1; side < (i == a.width - 1 ? 2 : i == 0 ? 1 : 0); ++side) {
-        const float* p = a.sat + (2 * (int64_t)head + side) * nsat;
-        for (int64_t r = lane; r < nsat; r += 64) sum += (double)p[r];
-      }
+#pragma unroll 4
+  for (int64_t it = threadIdx.x; it < items; it += RP_THREADS) {
+    const int64_t e = it / rows;
+    sum += (double)a.partial[((int64_t)head * a.width + a.bucket_order[e0 + e]) * rows + (it - e * rows)];
+  }
+  if (nsat > 0) {                                              // the sums beyond the ends belong to the ends' buckets
+    for (int side = 0; side < 2; ++side) {
+      if (a.lut[side ? a.width - 1 : 0] != c) continue;
+      const float* p = a.sat + (2 * (int64_t)head + side) * nsat;
+      for (int64_t r = threadIdx.x; r < nsat; r += RP_THREADS) sum += (double)p[r];
     }
-    const float* p = a.partial + ((int64_t)head * a.width + i) * rows;
-    for (int64_t r = lane; r < rows; r += 64) sum += (double)p[r];
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-  if (lane == 0) a.dtable[(int64_t)c * a.H + head] = (float)sum;
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) a.dtable[(int64_t)c * a.H + head] = (float)(red[0] + red[1] + red[2] + red[3]);
 }
 
 // partial maxima of |x| of up to three tensors (blockIdx.y), over the tokens that can be seen: what lies behind them may hold anything
@@ -1092,10 +1096,10 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_amax_kernel(ofb_relpos_args
   if (threadIdx.x == 0) out[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
-template <int DT, int DP> int rp_lds(const ofb_relpos_args& a, int kind) {       // 0 forward, 1 dQ, 2 dK dV
-  using G = rp_geo<DT, DP>;
+template <int DT, int DP, int KERNEL> int rp_lds(const ofb_relpos_args& a) {
+  using G = rp_geo<DT, DP, rp_rows_of<DT, DP>(KERNEL)>;
   const int w = ((a.width + 2 * RP_PAD + 3) & ~3) * 4;
-  return w * (kind == 1 ? 3 : 1) + (kind == 2 ? 8 : 2) * G::KB * 4 + 2 * G::STAGE;
+  return w * (KERNEL == 1 ? 3 : 1) + (KERNEL == 2 ? 8 : 2) * G::KB * 4 + 2 * G::STAGE;
 }
 
 template <typename F> int rp_allow(F* f, int bytes) {
@@ -1107,7 +1111,7 @@ template <typename F> int rp_allow(F* f, int bytes) {
     hipLaunchKernelGGL(kernel, grid, dim3(RP_THREADS), lds, stream, __VA_ARGS__);                                    \
   } while (0)
 
-int rp_kb(const ofb_relpos_args& a) { return a.dtype != RP_F32 && a.d <= 64 ? 64 : 32; }
+int rp_kb(const ofb_relpos_args& a) { return a.dtype == RP_F32 ? rp_rows_of<RP_F32, 64>(0) : a.d <= 64 ? rp_rows_of<RP_BF16, 64>(0) : rp_rows_of<RP_BF16, 128>(0); }
 // workgroups per head that leave a part of the table's gradient
 int64_t rp_table_rows(const ofb_relpos_args& a) { return (int64_t)a.B * ((a.Nq + RP_TILE - 1) / RP_TILE); }
 
@@ -1139,7 +1143,7 @@ int rp_check(const ofb_relpos_args* a) {
 
 template <int DT, int DP, bool POS> int rp_forward_of(const ofb_relpos_args& a, hipStream_t s) {
   const int64_t wgs = (int64_t)a.B * a.H * ((a.Nq + RP_TILE - 1) / RP_TILE);
-  const int lds = rp_lds<DT, DP>(a, 0), splits = rp_splits(a);
+  const int lds = rp_lds<DT, DP, 0>(a), splits = rp_splits(a);
   if (splits > 1) {
     if (!a.split_o || !a.split_ml) return OFB_EINVAL;
     RP_LAUNCH((relpos_fwd_kernel<DT, DP, POS, true>), dim3((unsigned)wgs, splits), lds, s, a);
@@ -1153,10 +1157,10 @@ template <int DT, int DP, bool POS> int rp_forward_of(const ofb_relpos_args& a, 
 
 template <int DT, int DP, bool POS> int rp_backward_of(const ofb_relpos_args& a, hipStream_t s) {
   const int nqt = (a.Nq + RP_TILE - 1) / RP_TILE, nkt = (a.Nk + RP_TILE - 1) / RP_TILE;
-  RP_LAUNCH((relpos_dq_kernel<DT, DP, POS>), dim3((unsigned)((int64_t)a.B * a.H * nqt)), (rp_lds<DT, DP>(a, 1)), s, a);
-  RP_LAUNCH((relpos_dkv_kernel<DT, DP, POS>), dim3((unsigned)((int64_t)a.B * a.H * nkt)), (rp_lds<DT, DP>(a, 2)), s, a);
+  RP_LAUNCH((relpos_dq_kernel<DT, DP, POS>), dim3((unsigned)((int64_t)a.B * a.H * nqt)), (rp_lds<DT, DP, 1>(a)), s, a);
+  RP_LAUNCH((relpos_dkv_kernel<DT, DP, POS>), dim3((unsigned)((int64_t)a.B * a.H * nkt)), (rp_lds<DT, DP, 2>(a)), s, a);
   if (a.dtable) {
-    hipLaunchKernelGGL(relpos_table_kernel, dim3((unsigned)(((int64_t)a.n_buckets * a.H + 3) / 4)), dim3(RP_THREADS), 0, s, a, rp_table_rows(a),
+    hipLaunchKernelGGL(relpos_table_kernel, dim3((unsigned)((int64_t)a.n_buckets * a.H)), dim3(RP_THREADS), 0, s, a, rp_table_rows(a),
                        a.pos_k ? (int64_t)0 : (int64_t)a.B * nqt * 4);
   }
   return ofb_launch_status();
