@@ -4,6 +4,7 @@ PyTorch is used only as plumbing here: device buffers (`data_ptr()`), the curren
 and the caching allocator.  All arithmetic happens inside the library's kernels.
 """
 import ctypes as C
+import functools
 import os
 import threading
 
@@ -1254,31 +1255,52 @@ def relpos_bwd(args):
 
 
 def _vp(t):
-    return None if t is None else _void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
+_P, _I, _L, _F = C.c_void_p, C.c_int32, C.c_int64, C.c_float
+_ARGTYPES = {
+    'ofb_distill_segments': (_L, _I),
+    'ofb_distill_fwd': (_P, _P, _P, _I, _P, _L, _I, _I, _F, _I, _P, _P, _P, C.c_double, _P, _P),
+    'ofb_distill_bwd': (_P, _P, _P, _I, _L, _I, _I, _F, _I, _P, _P, _I, _F, _P, _P),
+    'ofb_top_logits_segments': (_L, _I, _I),
+    'ofb_top_logits': (_P, _L, _I, _I, _F, _I, _P, _P, _P, _P, _P, _P),
+}
+_typed = {}
+
+
+def _entry_typed(name):
+    """an entry point with its argument types declared: calls convert plain numbers and addresses"""
+    f = _typed.get(name)
+    if f is None:
+        f = C.CFUNCTYPE(C.c_int, *_ARGTYPES[name])((name, lib()))
+        _typed[name] = f
+    return f
+
+
+@functools.lru_cache(maxsize=256)
 def distill_segments(R, V):
-    return int(lib().ofb_distill_segments(C.c_int64(R), _i(V)))
+    return int(_entry_typed('ofb_distill_segments')(R, V))
 
 
 def distill_fwd(z, values, indices, rest, tau, stats, part, row_loss, loss_scale, loss):
     R, V = z.shape
-    check(lib().ofb_distill_fwd(_vp(z), _vp(values), _vp(indices), _i(indices.dtype == torch.int64), _vp(rest), C.c_int64(R), _i(V), _i(values.shape[1]),
-                                _f(tau), _i(DTYPE_CODE[z.dtype]), _vp(stats), _vp(part), _vp(row_loss), C.c_double(loss_scale), _vp(loss), stream()),
-          'ofb_distill_fwd')
+    check(_entry_typed('ofb_distill_fwd')(z.data_ptr(), values.data_ptr(), indices.data_ptr(), indices.dtype == torch.int64, _vp(rest), R, V, values.shape[1], tau,
+                                          DTYPE_CODE[z.dtype], stats.data_ptr(), _vp(part), row_loss.data_ptr(), loss_scale, _vp(loss), stream()), 'ofb_distill_fwd')
 
 
 def distill_bwd(z, values, indices, tau, stats, up, grad_scale, dz):
     R, V = z.shape
-    check(lib().ofb_distill_bwd(_vp(z), _vp(values), _vp(indices), _i(indices.dtype == torch.int64), C.c_int64(R), _i(V), _i(values.shape[1]), _f(tau),
-                                _i(DTYPE_CODE[z.dtype]), _vp(stats), _vp(up), _i(up.numel() > 1), _f(grad_scale), _vp(dz), stream()), 'ofb_distill_bwd')
+    check(_entry_typed('ofb_distill_bwd')(z.data_ptr(), values.data_ptr(), indices.data_ptr(), indices.dtype == torch.int64, R, V, values.shape[1], tau,
+                                          DTYPE_CODE[z.dtype], stats.data_ptr(), up.data_ptr(), up.dim() > 0, grad_scale, dz.data_ptr(), stream()), 'ofb_distill_bwd')
 
 
+@functools.lru_cache(maxsize=256)
 def top_logits_segments(R, V, K):
-    return int(lib().ofb_top_logits_segments(C.c_int64(R), _i(V), _i(K)))
+    return int(_entry_typed('ofb_top_logits_segments')(R, V, K))
 
 
 def top_logits(z, K, tau, values, indices, rest, cand, part):
     R, V = z.shape
-    check(lib().ofb_top_logits(_vp(z), C.c_int64(R), _i(V), _i(K), _f(tau), _i(DTYPE_CODE[z.dtype]), _vp(values), _vp(indices), _vp(rest), _vp(cand),
-                               _vp(part), stream()), 'ofb_top_logits')
+    check(_entry_typed('ofb_top_logits')(z.data_ptr(), R, V, K, tau, DTYPE_CODE[z.dtype], values.data_ptr(), indices.data_ptr(), rest.data_ptr(), _vp(cand), _vp(part),
+                                         stream()), 'ofb_top_logits')

@@ -1147,11 +1147,11 @@ class DistillTopLogits(torch.autograd.Function):
             R, V = z.shape
             segs = hip.distill_segments(R, V)
             stats, rows = _new(z, R, 8), _new(z, R)
-            loss = _new(z, 1) if reduction != 'none' else None
+            loss = _new(z) if reduction != 'none' else None
             hip.distill_fwd(z, values, indices, rest, tau, stats, _new(z, R, segs, 2) if segs > 1 else None, rows, 1.0 / R if reduction == 'mean' else 1.0, loss)
             ctx.save_for_backward(z, values, indices, stats)
             ctx.tau, ctx.scale = tau, tau / R if reduction == 'mean' else tau
-            return rows if loss is None else loss[0]
+            return rows if loss is None else loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -1159,8 +1159,7 @@ class DistillTopLogits(torch.autograd.Function):
         z, values, indices, stats = ctx.saved_tensors
         with hip.on_device(z):
             dz = torch.empty(z.shape, device=z.device, dtype=z.dtype)
-            up = _c(up).reshape(-1)
-            hip.distill_bwd(z, values, indices, ctx.tau, stats, up, ctx.scale, dz)
+            hip.distill_bwd(z, values, indices, ctx.tau, stats, _c(up), ctx.scale, dz)
         return dz, None, None, None, None, None
 
 

@@ -66,9 +66,10 @@ class RelPosBuckets:
                 start[c + 1] += 1
             for c in range(self.num_buckets):
                 start[c + 1] += start[c]
-            up = lambda x: torch.tensor(x, dtype=torch.int32, device=device)
-            pq, pk = (up(self.positions[0]), up(self.positions[1])) if self.positions else (None, None)
-            got = self._on[device] = (up(self.lut), up(start), up(order), pq, pk)
+            parts = [self.lut, start, order] + (list(self.positions) if self.positions else [])
+            flat = torch.tensor([x for p in parts for x in p], dtype=torch.int32, device=device)
+            parts = list(flat.split([len(p) for p in parts]))
+            got = self._on[device] = tuple(parts) if self.positions else (*parts, None, None)
             if device.type == 'cuda':
                 torch.cuda.current_stream(device).synchronize()      # any stream may read the plan from here on
         return got
