@@ -233,6 +233,8 @@ __device__ __forceinline__ int rp_keys_of(const ofb_relpos_args& a, int b) {
 }
 
 typedef __attribute__((address_space(3))) const float rp_lds_float;
+// the same value in every lane, as a scalar
+__device__ __forceinline__ float rp_uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
 // LDS address of w[RP_PAD]: the entry of difference lo
 __device__ __forceinline__ int rp_lds_base(const float* w) { return (int)(uintptr_t)(rp_lds_float*)(w + RP_PAD); }
 // the bias at an LDS address, clamped to the head's vector: one instruction (the compiler makes two of min and max), and a read
@@ -308,7 +310,10 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 3 : DT == RP_F32 ? 1 : 2)) 
     c_s = c_s * ofb_h_pow2(-eq) * ofb_h_pow2(-ek);
     c_o = ofb_h_pow2(-ev);
   }
-  constexpr float p_exp = DT == RP_BF16 ? 0.f : (float)RP_PE;  // P and its sum are held times 2^p_exp
+  // f32: P's planes hold it times 2^14.  (Not by way of the exponent, where a maximum like -1e9 would swallow it; f16 needs no scale here: P is at
+  // most 1 and its row's sum at least 1, what falls below the subnormal step 2^-24 is nothing beside f16's own 2^-11.)
+  const float p_sc = DT == RP_F32 ? ofb_h_pow2(RP_PE) : 1.f;
+  if constexpr (DT == RP_F32) c_o *= ofb_h_pow2(-RP_PE);
 
   const int q0 = qt * RP_TILE + wv * 32, qi = q0 + (lane & 31);
   const bool active = q0 < a.Nq, qok = qi < a.Nq;
@@ -356,7 +361,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 3 : DT == RP_F32 ? 1 : 2)) 
       // scores in log2 units with the bias: s = c_t S + bt, where beyond the table's ends (the whole tile has one bias) S stays as it is
       const int dmax = j0 + KB - 1 - q0 - a.q_offset, dmin = j0 - (q0 + 31) - a.q_offset;
       float bt = 0.f, c_t = 1.f;
-      const float wc = w[RP_PAD + (dmax <= lo ? 0 : width - 1)];
+      const float wc = rp_uniform(w[RP_PAD + (dmax <= lo ? 0 : width - 1)]);
       // (a bias that swallows the scores, and a scale that is not positive, take the general form)
       if (!POS && (dmax <= lo || dmin >= hi) && fabsf(wc) < 1e30f && c_s > 0.f) {
         bt = wc;
@@ -405,7 +410,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 3 : DT == RP_F32 ? 1 : 2)) 
         for (int t = 0; t < DP / 32; ++t) O[t] *= alpha;
         m = m_new;
       }
-      const float tb = bt - (m > -INFINITY ? m : 0.f) + p_exp;         // a row that has seen nothing yet: exp2(-inf - 0) = 0
+      const float tb = bt - (m > -INFINITY ? m : 0.f);         // a row that has seen nothing yet: exp2(-inf - 0) = 0
 #pragma unroll
       for (int t = 0; t < KB / 32; ++t) {
 #pragma unroll
@@ -415,7 +420,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 3 : DT == RP_F32 ? 1 : 2)) 
           for (int j = 0; j < 8; ++j) {
             const float p = __builtin_amdgcn_exp2f(fmaf(S[t][8 * s + j], c_t, tb));
             l += p;
-            p8[j] = p;
+            p8[j] = DT == RP_F32 ? p * p_sc : p;
           }
           rp_frag pf[NP];
           rp_pack8<DT>(p8, pf);
@@ -435,7 +440,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 3 : DT == RP_F32 ? 1 : 2)) 
   if (!qok) return;
   if constexpr (SPLIT) {                                       // partial sums in units of exp2(m), joined by relpos_join_kernel
     const int64_t row = ((int64_t)blockIdx.y * a.B * a.H + bh) * a.Nq + qi;
-    if (hh == 0) { a.split_ml[2 * row] = m - p_exp; a.split_ml[2 * row + 1] = l; }
+    if (hh == 0) { a.split_ml[2 * row] = m; a.split_ml[2 * row + 1] = l; }
 #pragma unroll
     for (int ct = 0; ct < DP / 32; ++ct)
 #pragma unroll
@@ -448,7 +453,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 3 : DT == RP_F32 ? 1 : 2)) 
     if (a.stats && hh == 0) {
       float* st = a.stats + 2 * ((int64_t)bh * a.Nq + qi);
       st[0] = m > -INFINITY ? m : 0.f;
-      st[1] = __builtin_ldexpf(linv, (int)p_exp);
+      st[1] = linv;
     }
     const float f = linv * c_o;
     char* op = (char*)a.out + (b * a.o_sb + qi * a.o_st + head * a.o_sh) * ES;
@@ -593,10 +598,9 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : 2)) void
     m = a.stats[2 * row];
     linv = a.stats[2 * row + 1];
   }
-  // P 2^ek_ = exp2(s - mk) lk; a row without keys has 1 / sum = 0
-  const float mk = NP == 2 ? m : linv > 0.f ? m - __log2f(linv) - (float)ek_ : linv == 0.f ? INFINITY : linv;
-  const float lk = NP == 2 ? __builtin_ldexpf(linv, ek_) : 1.f;
-  const float nD = -__builtin_ldexpf(D, e.ed + e.ev);
+  // Inside the loop P lacks its factor 1 / sum, a constant of the lane that the row's results take at the end, and is held times kk.  (Neither goes
+  // into the exponent: a maximum like -1e9 would swallow it.)
+  const float kk = DT == RP_BF16 ? 1.f : ofb_h_pow2(max(-126, min(126, ek_))), nD = -__builtin_ldexpf(D, e.ed + e.ev);
   f32x16 dQ[DP / 32];
 #pragma unroll
   for (int t = 0; t < DP / 32; ++t) dQ[t] = rp_zero16();
@@ -623,8 +627,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : 2)) void
       dP = rp_mm<DT, NP>(vf, df[s], dP);
     }
   };
-  // ds: dS in units of 1 / k, k = the power of two that makes it the second product's operand (dP's own scale is in it too).  P's maximum and
-  // sum are one exponent (bf16, f16) or, for f32, the maximum and a factor: the rounding of a logarithm of the size of 10 would show.
+  // ds: dS over 1 / sum, in units of 1 / k, k = the power of two that makes it the second product's operand (dP's own scale is in it too).
   // at: the LDS addresses of the pairs' biases.
   auto general = [&](f32x16& S, f32x16& dP, int buf, int t0, int j0, bool whole, float (&ds)[16], int (&at)[16]) {
     float t[16];
@@ -654,9 +657,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : 2)) void
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      float p = __builtin_amdgcn_exp2f(fmaf(S[r], c_s, t[r]) - mk);
-      if constexpr (NP == 2) p *= lk;
-      ds[r] = p * dP[r];
+      ds[r] = __builtin_amdgcn_exp2f(fmaf(S[r], c_s, t[r]) - m) * kk * dP[r];
     }
   };
   // adds the pairs to their bins as whole numbers of 2^-32 / mul: high word floor(mul ds), low word the rest
@@ -671,9 +672,10 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : 2)) void
   auto visible = [&](int j0) { return active && j0 < kend && !(a.causal && j0 > q0 + 31 + a.q_offset); };
   auto is_whole = [&](int j0, int n, int first) { return j0 + n <= kend && (!a.causal || j0 + n - 1 <= first + a.q_offset); };
   // the whole tile of keys j0 .. j0 + n - 1 and queries first .. last lies beyond an end: -1, 1 or 0
-  auto beyond = [&](int j0, int n, int first, int last) {
-    return POS ? 0 : j0 + n - 1 - first - a.q_offset <= lo ? -1 : j0 - last - a.q_offset >= hi ? 1 : 0;
-  };
+  // (a bias that swallows the scores takes the general form, as in the forward)
+  const float w_lo = rp_uniform(w[RP_PAD]), w_hi = rp_uniform(w[RP_PAD + width - 1]);
+  const int below = fabsf(w_lo) < 1e30f ? lo + a.q_offset : -0x7fffffff, above = fabsf(w_hi) < 1e30f ? hi + a.q_offset : 0x7fffffff;
+  auto beyond = [&](int j0, int n, int first, int last) { return POS ? 0 : j0 + n - 1 - first <= below ? -1 : j0 - last >= above ? 1 : 0; };
   float most = 0.f;                                            // the largest |ds| that goes to a bin
   for (int kb = 0; kb < kb1; ++kb) {
     const int buf = kb & 1;
@@ -690,12 +692,11 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : 2)) void
       const int side = beyond(j0, 32, q0, q0 + 31);
       float ds[16], sum = 0.f;
       if (!POS && whole && side) {
-        const float tb = w[RP_PAD + (side < 0 ? 0 : width - 1)] - mk;
+        const float tb = (side < 0 ? w_lo : w_hi) - m;
         float psum = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          float p = __builtin_amdgcn_exp2f(fmaf(S[r], c_s, tb));
-          if constexpr (NP == 2) p *= lk;
+          const float p = __builtin_amdgcn_exp2f(fmaf(S[r], c_s, tb)) * kk;
           ds[r] = p * dP[r];
           sum += ds[r];
           psum += p;
@@ -707,7 +708,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : 2)) void
 #pragma unroll
         for (int r = 0; r < 16; ++r) sum += ds[r];
         if constexpr (DT == RP_F32) {                          // |ds| < 2^15, and a row's |ds| sum to less than that: 128 rows stay below 2^60
-          if (a.dtable) { asm volatile(""); bins(ds, at, 64.f); }
+          if (a.dtable) { asm volatile(""); bins(ds, at, 64.f * linv); }
         } else {
 #pragma unroll
           for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(ds[r]));
@@ -732,6 +733,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : 2)) void
     if (kb + 1 < kb1) commit(buf ^ 1);
     __syncthreads();
   }
+  const float c_out = c_dq * linv;
   if (qok) {
     char* op = (char*)a.dq + (b * a.dq_sb + qi * a.dq_st + head * a.dq_sh) * ES;
 #pragma unroll
@@ -739,19 +741,20 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : 2)) void
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
         const int ch = 32 * ct + rp_row(r, hh);
-        if (ch < a.d) rp_store4<DT>(op + ch * ES, dQ[ct][r] * c_dq, dQ[ct][r + 1] * c_dq, dQ[ct][r + 2] * c_dq, dQ[ct][r + 3] * c_dq);
+        if (ch < a.d) rp_store4<DT>(op + ch * ES, dQ[ct][r] * c_out, dQ[ct][r + 1] * c_out, dQ[ct][r + 2] * c_out, dQ[ct][r + 3] * c_out);
       }
   }
   // D came from an output whose P was rounded for the product.  A row of dS sums to zero, so what this row's sum is off by is D's error: the
   // kernels that follow read D without it, and the sums above lose it times their share of P.  (The table's gradient is f32 and sums whole rows'
   // parts, where an error that a row's terms share does not average out: without this it was 1e-3 off for bf16.)
   OFB_XOR_STEP(left, ofb_add_, 32)
+  left *= linv;
   if (qok && hh == 0) a.delta[(int64_t)bh * a.Nq + qi] = D + __builtin_ldexpf(left, -e.es);
   if (!a.dtable) return;
   if (a.sat) {
-    const float k = __builtin_ldexpf(left, -ek_);              // (P is held times 2^ek_)
-    sat_lo = ofb_wave_sum(sat_lo - k * pat_lo);
-    sat_hi = ofb_wave_sum(sat_hi - k * pat_hi);
+    const float k = __builtin_ldexpf(left, -ek_);              // (P is held times 2^ek_ and without 1 / sum)
+    sat_lo = ofb_wave_sum((sat_lo - k * pat_lo) * linv);
+    sat_hi = ofb_wave_sum((sat_hi - k * pat_hi) * linv);
     if (lane == 0) {
       const int64_t n = (int64_t)a.B * nqt * 4, at = ((int64_t)b * nqt + qt) * 4 + wv;
       a.sat[(2 * (int64_t)head) * n + at] = __builtin_ldexpf(sat_lo, -e.es);
@@ -763,14 +766,14 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : 2)) void
   if constexpr (DT != RP_F32) {
     // once more over the tiles with pairs between the ends, with the D that is known now; bins of 2^-unit, such that all pairs of the
     // workgroup could be as large as the largest
-    most = ofb_wave_max(most + fabsf(left));
+    most = ofb_wave_max(most * linv + fabsf(left));
     if (lane == 0) red[wv] = most;
     __syncthreads();
     most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     int ex = 0;
     if (most > 0.f) frexpf(most, &ex);
     unit = 62 - max(ex, -60) - (7 + 32 - __clz(a.Nk));
-    const float mul = __builtin_ldexpf(1.f, unit - 32), nd = nD - __builtin_ldexpf(left, e.ed + e.ev - e.es);
+    const float mul = __builtin_ldexpf(linv, unit - 32), nd = nD - __builtin_ldexpf(left, e.ed + e.ev - e.es);
     auto next = [&](int kb) {
       while (kb < kb1 && is_whole(kb * KB, KB, qt * RP_TILE) && beyond(kb * KB, KB, qt * RP_TILE, q_last)) ++kb;
       return kb;
@@ -810,26 +813,25 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : 2)) void
   }
 }
 
-// a query tile's row statistics for LDS: the maximum (with the sum's logarithm and the operand's scale 2^pe in it, or for f32 apart), the factor,
-// -D in dP's scale 2^de; a row without keys or behind the last query gets P = 0
-template <int DT, int KB, bool POS>
+// a query tile's row statistics for LDS: the maximum, 1 / sum times the operand's scale 2^pe, -D in dP's scale 2^de; a row without keys or behind the
+// last query gets P = 0
+template <int KB, bool POS>
 __device__ __forceinline__ void rp_row_stats(const ofb_relpos_args& a, int64_t bh, int row0, int pe, int de, f32x4& v, int& pos) {
   const int i = row0 + threadIdx.x;
-  v = f32x4{DT == RP_F32 ? 0.f : INFINITY, 0.f, 0.f, 0.f};
+  v = f32x4{0.f, 0.f, 0.f, 0.f};
   pos = 0;
   if (threadIdx.x < KB && i < a.Nq) {
     const int64_t row = bh * a.Nq + i;
-    const float m = a.stats[2 * row], l = a.stats[2 * row + 1];
-    if constexpr (DT == RP_F32) { v[0] = m; v[1] = __builtin_ldexpf(l, pe); }
-    else v[0] = l > 0.f ? m - __log2f(l) - (float)pe : l == 0.f ? INFINITY : l;
+    v[0] = a.stats[2 * row];
+    v[1] = __builtin_ldexpf(a.stats[2 * row + 1], pe);
     v[2] = -__builtin_ldexpf(a.delta[row], de);
     pos = POS ? 4 * a.pos_q[i] : i + a.q_offset;
   }
 }
 
 // P and dS of a 32 x 32 tile, rows = queries i0 .. (LDS tiles qt_ and dt_ at row tr), the wave's key on the lane.  st: row statistics m, l, -D of
-// the tile's queries, P = exp2(s - m) (times l for f32; l is in m otherwise), -D in dP's scale.  P comes out times the p_sc that is in the statistics,
-// dS = P dP times that and dP's scale.
+// the tile's queries, -D in dP's scale.  P = exp2(s - m) l comes out times the scale that is in l, dS = P (dP - D) times that and dP's scale.  (1 / sum stays
+// apart: its logarithm does not survive beside a maximum like -1e9.)
 template <int DT, int DP, int ROWS, bool POS>
 __device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char* qt_, const char* dt_, int tr, const rp_frag (&kf)[DP / 16][rp_type<DT>::NP],
                                            const rp_frag (&vf)[DP / 16][rp_type<DT>::NP], const float* st, const int* ps, const float* w, int i0, int j0,
@@ -887,13 +889,10 @@ __device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char*
 #pragma unroll
   for (int r = 0; r < 16; r += 4) {
     const int rr = rp_row(r, hh);
-    const f32x4 m4 = *reinterpret_cast<const f32x4*>(&st[tr + rr]);
-    f32x4 l4 = {1.f, 1.f, 1.f, 1.f};
-    if constexpr (NP == 2) l4 = *reinterpret_cast<const f32x4*>(&st[KB + tr + rr]);
+    const f32x4 m4 = *reinterpret_cast<const f32x4*>(&st[tr + rr]), l4 = *reinterpret_cast<const f32x4*>(&st[KB + tr + rr]);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      P[r + u] = __builtin_amdgcn_exp2f(fmaf(S[r + u], c_s, t[r + u] - m4[u]));
-      if constexpr (NP == 2) P[r + u] *= l4[u];
+      P[r + u] = __builtin_amdgcn_exp2f(fmaf(S[r + u], c_s, t[r + u]) - m4[u]) * l4[u];
       dS[r + u] = P[r + u] * dP[r + u];
     }
   }
@@ -931,7 +930,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 2 : 1)) void relpos_dkv_ker
   auto fetch = [&](int qb) {
     qs_.load(qp, a.q_st * ES, qb * KB, a.Nq, a.d);
     ds_.load(dp, a.do_st * ES, qb * KB, a.Nq, a.d);
-    rp_row_stats<DT, KB, POS>(a, bh, qb * KB, DT == RP_BF16 ? 0 : RP_PE, e.ed + e.ev, st_next, ps_next);
+    rp_row_stats<KB, POS>(a, bh, qb * KB, DT == RP_BF16 ? 0 : RP_PE, e.ed + e.ev, st_next, ps_next);
   };
   rp_bias_vector(a, head, w);
   if (qb0 < qb1) fetch(qb0);
@@ -1129,7 +1128,7 @@ int rp_check(const ofb_relpos_args* a) {
   if (!a || !a->q || !a->k || !a->v || !a->table || !a->lut) return OFB_EINVAL;
   if (a->B < 1 || a->H < 1 || a->Nq < 1 || a->Nk < 1 || a->d < 8 || a->d % 8 || a->dtype < 0 || a->dtype > 2) return OFB_EINVAL;
   if (a->width < 1 || a->n_buckets < 1 || (!a->pos_q) != (!a->pos_k) || (a->pos_q && a->causal)) return OFB_EINVAL;
-  if (a->d > 128 || a->width > RP_WMAX || a->Nq > (1 << 26) || a->Nk > (1 << 26)) return OFB_ELIMIT;
+  if (a->d > 128 || a->width > RP_WMAX || a->n_buckets > (1 << 20) || a->Nq > (1 << 26) || a->Nk > (1 << 26)) return OFB_ELIMIT;
   if (a->q_offset > (1 << 26) || a->q_offset < -(1 << 26) || a->lo > (1 << 26) || a->lo < -(1 << 26)) return OFB_ELIMIT;
   const int64_t tiles = (int64_t)a->B * a->H * (((int64_t)(a->Nq > a->Nk ? a->Nq : a->Nk) + 31) / 32);
   if (tiles > 0x3fffffff) return OFB_ELIMIT;

@@ -10,6 +10,7 @@ import torch
 
 from . import hip
 from .dp import grad_slot
+from .relpos import RelPosBuckets
 
 
 def _new(like, *shape):
@@ -898,6 +899,8 @@ class _RelposCall:
                 raise hip.OfbError(f'relpos_attention: q, k and v must share one of the types float32, bfloat16, float16; {name} is {t.dtype}')
             if t.device != q.device:
                 raise hip.OfbError('relpos_attention: q, k and v must be on one device')
+        if not isinstance(buckets, RelPosBuckets) or not isinstance(table, torch.Tensor):
+            raise hip.OfbError('relpos_attention: buckets must be a RelPosBuckets and table a tensor')
         B, Nq, H, d = q.shape
         if k.shape != v.shape or k.shape[0] != B or k.shape[2:] != q.shape[2:]:
             raise hip.OfbError(f'relpos_attention: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}: k and v must have the same number of tokens, '

@@ -26,6 +26,8 @@ class RelPosBuckets:
         lo, self.num_buckets = int(lo), int(num_buckets) if num_buckets is not None else max(lut) + 1
         if max(lut) >= self.num_buckets:
             raise OfbError(f'RelPosBuckets: bucket {max(lut)} of a table of {self.num_buckets} rows')
+        if self.num_buckets > 1 << 20:
+            raise OfbError('RelPosBuckets: tables of more than 2^20 rows are not supported')
         first, last = 0, len(lut) - 1                          # runs of one bucket at the ends say nothing that the clamp does not
         while first < last and lut[first + 1] == lut[0]:
             first += 1

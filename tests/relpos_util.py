@@ -4,7 +4,8 @@ Bounds.  u = eps / 2 of the tensors' type.  The first products are exact in f32 
 the absolute terms; f32: two f16 planes, 2^-21 a product more), exp2's argument and result are rounded once each: a probability is off by at most
 e_P = e (1 + scale sum |q||k| + |bias| + |S - max|) relative, e = (d + 16) 2^-24, counted at the row's largest, and twice (the row's sum).  P and dS are rounded to the type
 once more (u; f32: 2^-22), sums over n terms add n 2^-24.  f16 and f32 planes have an absolute floor of 2^-39 of their bound (half a subnormal step),
-one plane of f16 of 2^-39 for P (a step of 2^-24 below 2^-14, half of it, over the 2^14 of its scale) and 2^-39 of the bound for dS.  Rounding the result to f16
+one plane of f16 of 2^-25 of the row's largest P in the forward (half a step of 2^-24 below 2^-14),
+2^-39 for P in the backward (the same over the 2^14 of its scale) and 2^-39 of the bound for dS.  A bias beyond 1e30 swallows the score exactly.  Rounding the result to f16
 is off by u of the value where it is a normal number and by half the subnormal step, 2^-25, below 2^-14: both are counted."""
 import math
 
@@ -45,12 +46,15 @@ def reference(q, k, v, table, plan, scale=None, causal=False, key_lens=None, q_o
     o = p @ v
     c = 2.0 ** -24
     sub = 2.0 ** -25 if dtype == torch.float16 else 0.0
-    spread = scale * (q.abs() @ k.abs().transpose(2, 3)) + bias.abs().clamp(max=1e6) + torch.where(seen, (s - top).abs(), 0.0).clamp(max=100)
-    e_p = 2 * (d + 16) * c * (1 + (spread * seen).amax(-1, keepdim=True)) + 8 * c
+    size = abs(scale)
+    near = seen & (s - top > -200)                           # beyond, P is 0 in f32 whatever the score's rounding
+    spread = size * (q.abs() @ k.abs().transpose(2, 3)) + torch.where(bias.abs() < 1e30, bias.abs(), 0.0) + torch.where(near, (s - top).abs(), 0.0).clamp(max=100)
+    e_p = 2 * (d + 16) * c * (1 + (spread * near).amax(-1, keepdim=True)) + 8 * c
     floor_p = 2.0 ** -39 if dtype == torch.float16 else 0.0
     floor_x = 2.0 ** -39 if dtype == torch.float32 else 0.0
     pv = p @ v.abs()
-    e_o = (e_p + r + (Nk + 8) * c) * pv + floor_p * v.abs().sum(2, keepdim=True) + floor_x * v.abs().amax()
+    floor_f = 2.0 ** -25 * p.amax(-1, keepdim=True) if dtype == torch.float16 else 0.0
+    e_o = (e_p + r + (Nk + 8) * c) * pv + floor_f * v.abs().sum(2, keepdim=True) + floor_x * v.abs().amax()
     got = {'out': (o.transpose(1, 2), (e_o + u * (o.abs() + e_o) + sub).transpose(1, 2))}
     if dout is None:
         return got
@@ -59,7 +63,7 @@ def reference(q, k, v, table, plan, scale=None, causal=False, key_lens=None, q_o
     dp = do @ v.transpose(2, 3)
     ds = p * (dp - D)
     e32 = (e_p + (Nk + 8) * c) * pv + floor_x * v.abs().amax()                      # the unrounded output; for bf16 / f16 P's rounding is in it too
-    e_D = (do.abs() * (e32 + r * pv + floor_p * v.abs().sum(2, keepdim=True))).sum(-1, keepdim=True) + (d + 8) * c * (do.abs() * pv).sum(-1, keepdim=True)
+    e_D = (do.abs() * (e32 + r * pv + floor_f * v.abs().sum(2, keepdim=True))).sum(-1, keepdim=True) + (d + 8) * c * (do.abs() * pv).sum(-1, keepdim=True)
     e_dp = (d + 16) * c * (do.abs() @ v.abs().transpose(2, 3)) + floor_x * d * do.abs().amax() * v.abs().amax()
     e_ds = e_p * ds.abs() + p * (1 + e_p) * (e_dp + e_D) + 4 * c * ds.abs()
     top_ds = 2 * d * do.abs().amax() * v.abs().amax()
@@ -67,8 +71,8 @@ def reference(q, k, v, table, plan, scale=None, causal=False, key_lens=None, q_o
     def second(a, e_a, b, n, fl):
         """bound of a^T-like product already laid out: a (.., i, j), b (.., j, ch)"""
         return (e_a + r * a.abs() + n * c * a.abs()) @ b.abs() + fl * b.abs().sum(-2, keepdim=True) + floor_x * a.abs().sum(-1, keepdim=True) * b.abs().amax()
-    dq, e_dq = scale * (ds @ k), scale * second(ds, e_ds, k, Nk + 8, floor_ds)
-    dk, e_dk = scale * (ds.transpose(2, 3) @ q), scale * second(ds.transpose(2, 3), e_ds.transpose(2, 3), q, Nq + 8, floor_ds)
+    dq, e_dq = scale * (ds @ k), size * second(ds, e_ds, k, Nk + 8, floor_ds)
+    dk, e_dk = scale * (ds.transpose(2, 3) @ q), size * second(ds.transpose(2, 3), e_ds.transpose(2, 3), q, Nq + 8, floor_ds)
     dv, e_dv = p.transpose(2, 3) @ do, second(p.transpose(2, 3), (e_p * p).transpose(2, 3), do, Nq + 8, floor_p)
     for name, x, ex in (('dq', dq, e_dq), ('dk', dk, e_dk), ('dv', dv, e_dv)):
         got[name] = (x.transpose(1, 2), (ex + u * (x.abs() + ex) + sub).transpose(1, 2))

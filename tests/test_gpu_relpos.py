@@ -104,9 +104,28 @@ def test_a_bias_of_the_lowest_value_masks_and_a_row_of_it_is_even(dtype):
     even = v.float().mean(1, keepdim=True).expand(2, 70, 2, 32)
     tol = 2 * torch.finfo(DT[dtype]).eps * v.float().abs().mean(1, keepdim=True) + 1e-6
     assert bool(((got['out'].float() - even).abs() <= tol).all())
+    for plan, masked in ((RelPosBuckets([0, 1], 0), 1), (RelPosBuckets.clipped(3), 0)):
+        # a long run of masked keys beside visible ones, and rows that are masked throughout: even, with the gradients of an even row
+        q, k, v, table, dout = make(10, 1, 70, 300, 2, 64, DT[dtype], plan)
+        table[masked] = low
+        for off in (0, 2000, -2000):
+            U.check(step(q, k, v, table, plan, dout, q_offset=off), U.reference(q, k, v, table, plan, q_offset=off, dout=dout))
+    plan = RelPosBuckets([0, 1, 2], -1)
+    q, k, v, table, dout = make(9, 2, 70, 70, 2, 32, DT[dtype], plan)
     table[:] = -math.inf                                      # nothing is seen
     got = step(q, k, v, table, plan, dout)
     assert not got['out'].any() and not got['dq'].any() and not got['dv'].any()
+
+
+@pytest.mark.parametrize('dtype', list(DT))
+@pytest.mark.parametrize('scale', [-0.3, 0.0, 1.0])
+def test_scales(scale, dtype):
+    """a scale of any sign: beyond the ends too"""
+    for name, off in (('clip', 0), ('log8', 100), ('causal', -5)):
+        plan = PLANS[name]()
+        q, k, v, table, dout = make(14, 2, 70, 200, 1, 32, DT[dtype], plan)
+        got, want = step(q, k, v, table, plan, dout, scale=scale, q_offset=off), U.reference(q, k, v, table, plan, scale=scale, q_offset=off, dout=dout)
+        U.check(got, want)
 
 
 @pytest.mark.parametrize('dtype', list(DT))

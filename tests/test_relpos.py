@@ -59,7 +59,7 @@ def test_clipped_trimming_and_copies():
 
 @pytest.mark.parametrize('make', [
     lambda: RelPosBuckets([], 0), lambda: RelPosBuckets([0, -1], 0), lambda: RelPosBuckets([0, 3], 0, num_buckets=3), lambda: RelPosBuckets(range(4097), 0),
-    lambda: RelPosBuckets([0], 1 << 30), lambda: RelPosBuckets([0], 0, positions=([1 << 30], [0])), lambda: RelPosBuckets.log_spaced(7, 20), lambda: RelPosBuckets.log_spaced(0, 20),
+    lambda: RelPosBuckets([0], 1 << 30), lambda: RelPosBuckets([0], 0, num_buckets=1 << 21), lambda: RelPosBuckets([0], 0, positions=([1 << 30], [0])), lambda: RelPosBuckets.log_spaced(7, 20), lambda: RelPosBuckets.log_spaced(0, 20),
     lambda: RelPosBuckets.log_spaced(32, 8), lambda: RelPosBuckets.clipped(-1), lambda: RelPosBuckets.clipped(2048), lambda: RelPosBuckets.grid(0, 3), lambda: RelPosBuckets.grid(40, 40),
     lambda: RelPosBuckets.log_spaced(1000, 100000)])
 def test_plans_that_are_refused(make):
@@ -76,7 +76,7 @@ def test_refusals():
         dict(q=t(2, 5, 48)), dict(q=t(2, 5, 3, 16, dtype=torch.float64)), dict(k=t(2, 7, 3, 16, dtype=torch.bfloat16)), dict(k=t(2, 7, 1, 16), v=t(2, 7, 1, 16)),
         dict(v=t(2, 6, 3, 16)), dict(k=t(1, 7, 3, 16), v=t(1, 7, 3, 16)), dict(q=t(2, 5, 3, 12), k=t(2, 7, 3, 12), v=t(2, 7, 3, 12)),
         dict(q=t(2, 5, 3, 136), k=t(2, 7, 3, 136), v=t(2, 7, 3, 136)), dict(table=t(7, 3)), dict(table=t(8, 3, dtype=torch.bfloat16)), dict(key_lens=torch.zeros(2, dtype=torch.int64)),
-        dict(key_lens=torch.zeros(3, dtype=torch.int32)), dict(q_offset=1 << 30), dict(buckets=grid, table=t(12, 3)), dict(q=t(2, 5, 0, 16), k=t(2, 7, 0, 16), v=t(2, 7, 0, 16), table=t(8, 0)),
+        dict(key_lens=torch.zeros(3, dtype=torch.int32)), dict(buckets=[0, 1]), dict(table=None), dict(q_offset=1 << 30), dict(buckets=grid, table=t(12, 3)), dict(q=t(2, 5, 0, 16), k=t(2, 7, 0, 16), v=t(2, 7, 0, 16), table=t(8, 0)),
         dict(buckets=grid, table=t(12, 3), k=t(2, 5, 3, 16), v=t(2, 5, 3, 16), causal=True), dict(buckets=grid, table=t(12, 3), k=t(2, 5, 3, 16), v=t(2, 5, 3, 16), q_offset=1),
         dict(),                                                # CPU tensors: there is no fallback
     ]
@@ -103,6 +103,6 @@ def test_entry_refuses_what_the_kernels_cannot_take():
     bad = [dict(q=None), dict(q=8), dict(d=12), dict(d=0), dict(B=0), dict(Nq=0), dict(dtype=3), dict(width=0), dict(q_st=44), dict(v_sb=-8), dict(o_st=2), dict(pos_q=16),
            dict(pos_q=16, pos_k=16, causal=1), dict(out=8), dict(dtype=0)]
     assert [run(**b) for b in bad] == [-1] * len(bad)
-    limit = [dict(d=136), dict(width=4097), dict(q_offset=1 << 30), dict(B=1 << 20, H=1 << 10, Nk=1 << 12)]
+    limit = [dict(d=136), dict(width=4097), dict(n_buckets=1 << 21), dict(q_offset=1 << 30), dict(B=1 << 20, H=1 << 10, Nk=1 << 12)]
     assert [run(**b) for b in limit] == [-2] * len(limit)
     assert lib.ofb_relpos_fwd(None, None) == -1 and lib.ofb_relpos_bwd(None, None) == -1 and lib.ofb_relpos_sizes(None, None) == -1 and lib.ofb_relpos_amax(None, 0, 1, None) == -1
