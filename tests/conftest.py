@@ -21,6 +21,9 @@ _OFF = {
 
 
 def pytest_collection_modifyitems(items):
+    absent = not os.path.isfile('/root/reference/engine.py')
     for item in items:
+        if absent and item.nodeid.startswith('tests/test_reference_conformance.py'):
+            item.add_marker(pytest.mark.skip(reason='the reference is not here'))      # (the folder alone may be)
         if item.nodeid in _OFF:
             item.add_marker(pytest.mark.skip(reason=_OFF[item.nodeid]))
