@@ -23,7 +23,7 @@
 #define DS_STATS 8                /* floats kept per row: m_t, kappa, m, 1/s, m_teacher, 1/s_teacher, used, 0 */
 #define TL_CAP 4096               /* candidates of a row or segment that are ranked at once */
 #define TL_THREADS 1024
-#define TL_SMALL 256              /* threads for lists of up to TL_SMALL / 2: 1024 x 100003 bf16, 64 kept: 90 us, 512 threads 103 us, 1024 threads 99 us */
+#define TL_SMALL 256              /* threads for lists of up to TL_SMALL / 2: 1024 x 100003 bf16, 64 kept: 75 us, 1024 threads 99 us */
 
 namespace {
 
@@ -476,10 +476,13 @@ __device__ __forceinline__ ds_sum tl_rank(unsigned long long* list, float* left,
 }
 
 template <int DT, int THREADS, bool WHOLE>
-__global__ __launch_bounds__(THREADS) void top_logits_kernel(tl_args a) {
+__global__ __launch_bounds__(THREADS, 4) void top_logits_kernel(tl_args a) {
   constexpr int CH = ds_type<DT>::CH;
-  __shared__ __attribute__((aligned(16))) unsigned long long list[TL_CAP + 2];
-  __shared__ float left[TL_CAP];
+  // Small workgroups: half the list and at most 128 registers, so that four share a CU (1024 rows are then one round of the chip: 1024 x 100003
+  // bf16, 64 kept, 75 us; 90 us with the whole list and as many registers as the compiler likes).
+  constexpr int CAP = THREADS == TL_SMALL ? TL_CAP / 2 : TL_CAP;
+  __shared__ __attribute__((aligned(16))) unsigned long long list[CAP + 2];
+  __shared__ float left[CAP];
   __shared__ float redm[THREADS / 64], reds[THREADS / 64];
   __shared__ int count;
   __shared__ unsigned bound;
@@ -530,7 +533,7 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(tl_args a) {
         const int at_c = c + i / CH * THREADS;
         if (!(x[i] < least) && r.has(at_c, i % CH)) {
           const int at = atomicAdd(&count, 1);
-          if (at < TL_CAP) list[at] = ((unsigned long long)tl_key(x[i]) << 32) | (unsigned)~(unsigned)(at_c * CH + i % CH - r.mis);
+          if (at < CAP) list[at] = ((unsigned long long)tl_key(x[i]) << 32) | (unsigned)~(unsigned)(at_c * CH + i % CH - r.mis);
           x[i] = -INFINITY;
         }
       }
@@ -539,7 +542,7 @@ __global__ __launch_bounds__(THREADS) void top_logits_kernel(tl_args a) {
   });
   __syncthreads();
   int n = count;
-  if (n > TL_CAP) {
+  if (n > CAP) {
     // many equal elements, or a sorted run: the K-th largest key itself, bit by bit from the top
     unsigned long long floor_key = 0ull;
     for (int bit = 63; bit >= 0; --bit) {

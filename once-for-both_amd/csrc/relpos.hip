@@ -10,8 +10,8 @@
 //
 // Matrix products: v_mfma_f32_32x32x16.  bf16 and f16 operands as they are; f32 operands as two f16 planes of a power-of-two scaled copy and
 // three products (hformat.h), with the exponents from device-side maxima.  Scores, softmax statistics, dS and all sums are f32 (the
-// table's gradient sums in 64 bits); P and dS are rounded to the operand type for the second product - bf16, or f16 times 2^14 and a power
-// of two that keeps |dS| < 2^15, in two planes again for f32.
+// table's gradient sums in 64 bits); P and dS are rounded to the operand type for the second product: bf16 as they are,
+// f16 with dS times a power of two that keeps it below 2^15 (and P times 2^14 for dV), f32 likewise in two f16 planes.
 //
 // Operand conventions (lane l, hh = l >> 5): A[row = l & 31][k = 8 hh + j], B[k = 8 hh + j][col = l & 31], accumulator register r holds
 // row 8 (r >> 2) + 4 hh + (r & 3) of column l & 31.  A reduction may run over its index in any order that both operands share, so an
@@ -26,7 +26,7 @@
 #define RP_TILE 128              /* queries (forward, dQ) or keys (dK dV, table gradient) of a workgroup: four waves of 32 */
 #define RP_PAD 4                 /* entries of w on either side, so that four consecutive differences need one clamp */
 #define RP_WMAX 4096
-#define RP_PE 14                 /* f16 planes hold P 2^14 */
+#define RP_PE 14                 /* f32's planes, and the backward's f16, hold P 2^14 */
 #define RP_NBOUND 256            /* partial maxima of a tensor */
 
 namespace {

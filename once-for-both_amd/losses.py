@@ -102,7 +102,7 @@ class OFBSearchLOSS(nn.Module):
             # the three module terms are the slots of ONE device vector (the gate kernel's output): w1 a + w2 m + w4 e as one weighted
             # sum - 4 launches forward and 2 backward instead of 7 and ~12 (three select-backward fills and their accumulation)
             if ops._scalar_ok(loss_flops) and sp.is_cuda and sp.dtype == torch.float32 and sp.is_contiguous():
-                # one launch forward, one backward (round 6; the weights are plain attributes: read at every call)
+                # one launch forward, one backward (the weights are plain attributes: read at every call)
                 arch = ops.ArchLoss.apply(sp, loss_flops, float(self.w1), float(self.w2), float(self.w4), float(self.w5))
             else:
                 key = (float(self.w1), float(self.w2), float(self.w4), sp.device, sp.dtype)

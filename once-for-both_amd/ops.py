@@ -621,7 +621,7 @@ class TokenTaps(torch.autograd.Function):
     @staticmethod
     def forward(ctx, latent, patch_ids):
         """patch_ids: int32 global patch ids b * L + l of the masked patches (ofb_patch_mask's list); their token rows are computed in
-        the kernel.  One launch forward (ofb_token_taps_fwd), a memset node + one launch backward (round 6: they were five and three)."""
+        the kernel.  One launch forward (ofb_token_taps_fwd), a fill and one launch backward (they were five and three)."""
         B, T, D = latent.shape
         latent = _c(latent)
         n = int(patch_ids.numel())
