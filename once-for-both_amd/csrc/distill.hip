@@ -644,7 +644,7 @@ int tl_segments(int64_t R, int V, int K) {
 }
 int ds_check(const void* z, const void* values, const void* indices, int64_t R, int32_t V, int32_t K, float tau, int32_t dtype) {
   if (!z || !values || !indices || R < 1 || V < 1 || K < 1 || dtype < 0 || dtype > 2 || !(tau > 0.f) || !(tau < 3.0e38f)) return OFB_EINVAL;
-  if (K > DS_KMAX || K > V || V > (1 << 30) || R > (1 << 24)) return OFB_ELIMIT;
+  if (K > DS_KMAX || K > V || V > (1 << 30) || R >= (1 << 22)) return OFB_ELIMIT;      // (threads of a launch count in 32 bits)
   if (!ofb_aligned16(z)) return OFB_EINVAL;
   return OFB_OK;
 }
@@ -662,7 +662,7 @@ extern "C" int ofb_distill_fwd(const void* z, const void* values, const void* in
   a.z = z; a.values = values; a.indices = indices; a.rest = rest; a.stats = stats; a.part = part; a.row_loss = row_loss;
   a.R = R; a.V = V; a.K = K; a.segs = ds_segments(R, V); a.idx64 = idx64; a.c = (float)(1.4426950408889634074 / (double)tau); a.tau = tau;
   if (a.segs > 1 && !part) return OFB_EINVAL;
-  if (R * a.segs > 0x7fffffff) return OFB_ELIMIT;
+  if (R * a.segs >= (1 << 22)) return OFB_ELIMIT;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)(R * a.segs)), block(DS_THREADS);
   // (a row spans one chunk more than V classes take where it starts inside one; the last word is only cleared)
@@ -685,7 +685,7 @@ extern "C" int ofb_distill_bwd(const void* z, const void* values, const void* in
   ds_args a = {};
   a.z = z; a.values = values; a.indices = indices; a.stats = (float*)stats; a.dz = dz; a.up = up; a.up_rows = up_rows; a.grad_scale = grad_scale;
   a.R = R; a.V = V; a.K = K; a.segs = ds_segments(R, V); a.idx64 = idx64; a.c = (float)(1.4426950408889634074 / (double)tau); a.tau = tau;
-  if (R * a.segs > 0x7fffffff) return OFB_ELIMIT;
+  if (R * a.segs >= (1 << 22)) return OFB_ELIMIT;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)(R * a.segs)), block(DS_THREADS);
   if (dtype == DS_F32) hipLaunchKernelGGL((distill_bwd_kernel<DS_F32>), grid, block, 0, s, a);
@@ -700,7 +700,7 @@ extern "C" int ofb_top_logits(const void* z, int64_t R, int32_t V, int32_t K, fl
   if (!rest) return OFB_EINVAL;
   tl_args a = {z, values, indices, rest, (unsigned long long*)cand, part, R, V, K, tl_segments(R, V, K), (float)(1.4426950408889634074 / (double)tau)};
   if (a.segs > 1 && (!cand || !part)) return OFB_EINVAL;
-  if (R * a.segs > 0x7fffffff) return OFB_ELIMIT;
+  if (R * a.segs >= (1 << 22)) return OFB_ELIMIT;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)(R * a.segs));
 #define TL_RUN(DT)                                                                                                        \

@@ -1042,7 +1042,8 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_table_kernel(ofb_relpos_arg
   if (threadIdx.x == 0) a.dtable[(int64_t)c * a.H + head] = (float)(red[0] + red[1] + red[2] + red[3]);
 }
 
-// partial maxima of |x| of up to three tensors (blockIdx.y), over the tokens that can be seen: what lies behind them may hold anything
+// partial maxima of |x| of up to three tensors (blockIdx.y), over the tokens that can be seen: what lies behind them may hold anything.
+// Infinities and NaN do not count: they pass the planes at any exponent, and the rows that do not meet them keep theirs
 template <int DT>
 __global__ __launch_bounds__(RP_THREADS) void relpos_amax_kernel(ofb_relpos_args a, int first) {
   constexpr int ES = rp_type<DT>::ES;
@@ -1084,7 +1085,10 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_amax_kernel(ofb_relpos_args
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v = fmaxf(v, fabsf(rp_chunk_at<DT>(q[u], j)));
+          for (int j = 0; j < 8; ++j) {
+            const float y = fabsf(rp_chunk_at<DT>(q[u], j));
+            v = fmaxf(v, y < INFINITY ? y : 0.f);
+          }
       }
     }
   }
@@ -1130,8 +1134,8 @@ int rp_check(const ofb_relpos_args* a) {
   if (a->width < 1 || a->n_buckets < 1 || (!a->pos_q) != (!a->pos_k) || (a->pos_q && a->causal)) return OFB_EINVAL;
   if (a->d > 128 || a->width > RP_WMAX || a->n_buckets > (1 << 20) || a->Nq > (1 << 26) || a->Nk > (1 << 26)) return OFB_ELIMIT;
   if (a->q_offset > (1 << 26) || a->q_offset < -(1 << 26) || a->lo > (1 << 26) || a->lo < -(1 << 26)) return OFB_ELIMIT;
-  const int64_t tiles = (int64_t)a->B * a->H * (((int64_t)(a->Nq > a->Nk ? a->Nq : a->Nk) + 31) / 32);
-  if (tiles > 0x3fffffff) return OFB_ELIMIT;
+  const int64_t tiles = (int64_t)a->B * a->H * (((int64_t)(a->Nq > a->Nk ? a->Nq : a->Nk) + RP_TILE - 1) / RP_TILE);
+  if (tiles >= (1 << 24)) return OFB_ELIMIT;                   // threads of a launch count in 32 bits
   const int64_t unit = a->dtype == RP_F32 ? 4 : 8;             // 16-byte loads
   if (!ofb_aligned16(a->q) || !ofb_aligned16(a->k) || !ofb_aligned16(a->v)) return OFB_EINVAL;
   for (int64_t s : {a->q_sb, a->q_st, a->q_sh, a->k_sb, a->k_st, a->k_sh, a->v_sb, a->v_st, a->v_sh})
@@ -1198,8 +1202,13 @@ extern "C" int ofb_relpos_amax(const ofb_relpos_args* a, int32_t first, int32_t 
   if (a->B < 1 || a->H < 1 || a->Nq < 1 || a->Nk < 1 || a->d < 8 || a->d % 8 || a->dtype < 0 || a->dtype > 2) return OFB_EINVAL;
   const void* x[4] = {a->q, a->k, a->v, a->dout};
   const float* o[4] = {a->bound_q, a->bound_k, a->bound_v, a->bound_do};
-  for (int i = first; i < first + count; ++i)
+  const int64_t t[4][3] = {{a->q_sb, a->q_st, a->q_sh}, {a->k_sb, a->k_st, a->k_sh}, {a->v_sb, a->v_st, a->v_sh}, {a->do_sb, a->do_st, a->do_sh}};
+  const int64_t unit = a->dtype == RP_F32 ? 4 : 8;
+  for (int i = first; i < first + count; ++i) {
     if (!x[i] || !o[i] || !ofb_aligned16(x[i])) return OFB_EINVAL;
+    for (int64_t s : t[i])
+      if (s % unit || s < 0) return OFB_EINVAL;
+  }
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid(RP_NBOUND, count);
   if (a->dtype == RP_F32) hipLaunchKernelGGL((relpos_amax_kernel<RP_F32>), grid, dim3(RP_THREADS), 0, s, *a, first);
@@ -1219,6 +1228,7 @@ extern "C" int ofb_relpos_fwd(const ofb_relpos_args* a, void* stream) {
 extern "C" int ofb_relpos_bwd(const ofb_relpos_args* a, void* stream) {
   if (const int rc = rp_check(a)) return rc;
   if (!a->dout || !a->out32 || !a->stats || !a->delta || !a->dq || !a->dk || !a->dv) return OFB_EINVAL;
+  if (a->dtable && (int64_t)a->n_buckets * a->H >= (1 << 24)) return OFB_ELIMIT;
   if (a->dtable && (!a->partial || !a->bucket_start || !a->bucket_order || (!a->pos_k && !a->sat))) return OFB_EINVAL;
   if (a->dtype != RP_BF16 && (!a->bound_v || !a->bound_do || a->n_bound < 1 || a->n_bound > RP_NBOUND || a->n_bound_do < 1 || a->n_bound_do > RP_NBOUND)) return OFB_EINVAL;
   for (const void* p : {(const void*)a->dout, (const void*)a->out32, (const void*)a->dq, (const void*)a->dk, (const void*)a->dv})

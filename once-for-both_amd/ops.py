@@ -1063,7 +1063,8 @@ def relpos_attention(q, k, v, table, buckets, scale=None, causal=False, key_lens
     Key j stands at position j and query i at i + q_offset (new tokens behind a cache: q_offset = Nk - Nq), unless the plan has positions of its own.
     causal: a query sees the keys at or before its position.  key_lens (B,) int32: keys from there on are padding - they are not read, and
     their gradients are zero; a length beyond Nk counts as Nk, one below 0 as 0.  A query that sees no key has output and gradients 0.
-    Returns (B, Nq, H, d) of q's type.  Differentiable once, in q, k, v and the table; the same inputs give the same bits."""
+    Returns (B, Nq, H, d) of q's type.  Differentiable once, in q, k, v and the table; the same inputs give the same bits.  A NaN or infinity makes the rows,
+    and the gradients, that meet it NaN, and the table's gradient of its head."""
     call = _RelposCall(q, k, v, table, buckets, scale, causal, key_lens, q_offset)
     if key_lens is not None:
         key_lens = _c(key_lens)
@@ -1116,8 +1117,8 @@ def _check_logits(what, z, K, temperature):
         raise hip.OfbError(f'{what}: temperature must be positive and finite, got {temperature}')
     if not 1 <= K <= min(z.shape[1], 1024):
         raise hip.OfbError(f'{what}: {K} of {z.shape[1]} classes: 1 to 1024 can be stored, at most all')
-    if z.shape[1] > 1 << 30 or z.shape[0] > 1 << 24:
-        raise hip.OfbError(f'{what}: at most 2^24 rows of 2^30 classes are supported')
+    if z.shape[1] > 1 << 30 or z.shape[0] >= 1 << 22:
+        raise hip.OfbError(f'{what}: fewer than 2^22 rows of at most 2^30 classes are supported')
     if not z.is_cuda:
         raise hip.OfbError('once-for-both_amd kernels need device tensors (no CPU fallback); got a CPU tensor')
 

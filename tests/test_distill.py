@@ -35,3 +35,11 @@ def test_entries_refuse_what_the_kernels_cannot_take():
     top = lambda rest, V: lib.ofb_top_logits(p(16), L(1), i(V), i(3), f(1.0), i(0), p(16), p(16), p(rest), None, None, None)
     assert top(None, 9) == -1 and top(16, 1 << 20) == -1
     assert lib.ofb_distill_segments(L(0), i(5)) == 0 and lib.ofb_top_logits_segments(L(5), i(5), i(0)) == 0
+
+
+def test_too_many_rows():
+    z = torch.zeros(1, 1).expand(1 << 22, 1)
+    with pytest.raises(hip.OfbError, match='2.22'):
+        ops.top_logits(z, 1)
+    with pytest.raises(hip.OfbError, match='2.22'):
+        ops.distill_top_logits(z, z, z.int())

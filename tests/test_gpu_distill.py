@@ -211,3 +211,13 @@ def test_no_rows():
     loss = ops.distill_top_logits(z, values, indices, reduction='sum')
     loss.backward()
     assert float(loss) == 0 and z.grad.shape == (0, 5)
+
+
+def test_as_many_rows_as_there_can_be():
+    R = (1 << 22) - 1
+    z = torch.randn(R, 3, generator=torch.Generator().manual_seed(3)).cuda()
+    values, indices, rest = ops.top_logits(z, 2)
+    v, i = z.sort(dim=1, descending=True, stable=True)              # (a few of the rows have ties: the lowest class first)
+    assert torch.equal(values, v[:, :2]) and torch.equal(indices.long(), i[:, :2]) and torch.allclose(rest, v[:, 2], rtol=0, atol=1e-5)
+    loss, g = run(z.flip(0), values.flip(0), indices.flip(0), rest.flip(0), 1.0, torch.ones((), device='cuda'), 'sum')
+    assert float(loss) <= R * 1e-6 and float(g.abs().max()) <= 1e-5

@@ -270,3 +270,109 @@ def test_only_some_gradients_and_twice_through_one_graph():
     g = torch.autograd.grad(out.sum(), t, create_graph=True)[0]
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.parametrize('dtype', list(DT))
+def test_positions_with_lengths_and_other_orders(dtype):
+    """given positions in any order, more keys than queries, lengths, and one query over many keys"""
+    g = torch.Generator().manual_seed(12)
+    for Nq, Nk, d in ((70, 200, 64), (1, 1400, 40), (130, 33, 128)):
+        plan = RelPosBuckets(range(41), -20, positions=(torch.randint(-30, 30, (Nq,), generator=g), torch.randint(-30, 30, (Nk,), generator=g)))
+        q, k, v, table, dout = make(13 + Nq, 3, Nq, Nk, 2, d, DT[dtype], plan)
+        lens = torch.tensor([Nk, 0, Nk // 2 + 1], dtype=torch.int32, device='cuda')
+        U.check(step(q, k, v, table, plan, dout, key_lens=lens), U.reference(q, k, v, table, plan, key_lens=lens, dout=dout))
+
+
+@pytest.mark.parametrize('dtype', list(DT))
+def test_the_widest_plan(dtype):
+    """4095 differences and heads of 128: the most LDS that a call can ask for"""
+    plan = RelPosBuckets.clipped(2047)
+    q, k, v, table, dout = make(31, 1, 150, 2300, 2, 128, DT[dtype], plan)
+    for off in (0, 2200):
+        U.check(step(q, k, v, table, plan, dout, q_offset=off), U.reference(q, k, v, table, plan, q_offset=off, dout=dout))
+
+
+@pytest.mark.parametrize('dtype', list(DT))
+def test_zeros(dtype):
+    plan = PLANS['clip']()
+    q, k, v, table, dout = make(1, 2, 40, 40, 1, 32, DT[dtype], plan)
+    for zero in (q, k, v, dout):
+        ins = [torch.zeros_like(x) if x is zero else x for x in (q, k, v)]
+        do = torch.zeros_like(dout) if zero is dout else dout
+        U.check(step(*ins, table, plan, do), U.reference(*ins, table, plan, dout=do))
+    ins = [torch.zeros_like(x) for x in (q, k, v)]
+    got = step(*ins, torch.zeros_like(table), plan, torch.zeros_like(dout))
+    assert not any(bool(x.any()) for x in got.values())
+
+
+@pytest.mark.parametrize('dtype', list(DT))
+@pytest.mark.parametrize('value', [math.inf, -math.inf, math.nan])
+def test_what_is_not_finite_stays_where_it_is(value, dtype):
+    """in one batch item: the others are as without it, the rows that meet it are NaN, and the table's gradient is"""
+    plan = PLANS['clip']()
+    q, k, v, table, dout = make(15, 3, 70, 70, 2, 64, DT[dtype], plan)
+    want = U.reference(q, k, v, table, plan, dout=dout)
+    for at in range(4):
+        ins = [q.clone(), k.clone(), v.clone(), dout.clone()]
+        ins[at][1, 20, 0, 5] = value
+        got = step(*ins[:3], table, plan, ins[3])
+        others = {n: got[n][[0, 2]] for n in ('out', 'dq', 'dk', 'dv')}
+        U.check(others, {n: tuple(x[[0, 2]] for x in want[n]) for n in others})
+        U.check({n: x[:, :, 1] for n, x in ((n, got[n][1:2]) for n in others)}, {n: tuple(x[1:2, :, 1] for x in want[n]) for n in others})      # the other head
+        if at < 3:
+            assert bool((~torch.isfinite(got['out'][1, :, 0])).any())
+        assert not bool(torch.isfinite(got['dq'][1, :, 0]).all()) and not bool(torch.isfinite(got['dtable'][:, 0]).all())
+        assert torch.isfinite(got['dtable'][:, 1]).all()
+
+
+@pytest.mark.parametrize('dtype', list(DT))
+def test_strides_beyond_32_bits(dtype):
+    """batch, token and head strides whose offsets pass 2^32 bytes and 2^31 elements: the bits of contiguous copies"""
+    plan = PLANS['log8']()
+    room = torch.empty(5_000_000_000, dtype=DT[dtype], device='cuda')
+    for shape, stride in (((3, 70, 2, 64), (2_200_000_000, 128, 64, 1)), ((1, 300, 2, 64), (0, 16_000_000, 64, 1)), ((2, 70, 2, 64), (128, 256, 4_400_000_000, 1))):
+        q, k, v, table, dout = make(17, *shape[:2], *shape[1:], DT[dtype], plan)
+        want = step(q, k, v, table, plan, dout)
+        for i, x in enumerate((q, k, v, dout)):
+            far = room.as_strided(shape, stride)
+            far.copy_(x)
+            ins = [q, k, v, dout]
+            ins[i] = far
+            got = step(*ins[:3], table, plan, ins[3])
+            for n in want:
+                assert torch.equal(want[n], got[n]), (shape, i, n)
+
+
+def test_gradients_beyond_32_bits():
+    """2^31 + key elements of a long cache, of which eight queries at its end see the last ones: those and their gradients as in the slice alone, none for the others"""
+    N, H, d, last = 530_000, 32, 128, 1024
+    plan = RelPosBuckets.clipped(100)
+    g = torch.Generator(device='cuda').manual_seed(3)
+    k, v = (torch.randn(1, N, H, d, generator=g, device='cuda', dtype=torch.bfloat16) for _ in range(2))
+    q, dout = (torch.randn(1, 8, H, d, generator=g, device='cuda', dtype=torch.bfloat16) for _ in range(2))
+    table = torch.randn(201, H, generator=g, device='cuda')
+    table[0] = -math.inf                                      # nothing from 100 tokens back on
+    got = step(q, k, v, table, plan, dout, q_offset=N - 8)
+    ks, vs = k[:, -last:].clone(), v[:, -last:].clone()
+    want = U.reference(q, ks, vs, table, plan, q_offset=last - 8, dout=dout)
+    want.pop('dtable')
+    U.check({n: got[n][:, -last:] if n in ('dk', 'dv') else got[n] for n in want}, want)
+    assert not got['dk'][:, :-last].any() and not got['dv'][:, :-last].any()
+
+
+def test_queries_beyond_32_bits():
+    """2^31 + query elements over few keys: the last rows' output and gradient are those of the rows alone"""
+    N, H, d = 530_000, 32, 128
+    plan = RelPosBuckets.clipped(20)
+    g = torch.Generator(device='cuda').manual_seed(4)
+    q = torch.randn(1, N, H, d, generator=g, device='cuda', dtype=torch.bfloat16)
+    k, v = (torch.randn(1, 16, H, d, generator=g, device='cuda', dtype=torch.bfloat16) for _ in range(2))
+    table = torch.randn(41, H, generator=g, device='cuda')
+    got = step(q, k, v, table, plan, q)
+    rows = slice(N - 80, N)
+    part = q[:, rows].clone()
+    alone = step(part, k, v, table, plan, part, q_offset=N - 80)
+    for n in ('out', 'dq'):
+        assert torch.equal(got[n][:, rows], alone[n]), n
+    for n in ('dk', 'dv', 'dtable'):
+        assert torch.isfinite(got[n]).all() and bool(got[n].any())

@@ -106,3 +106,20 @@ def test_entry_refuses_what_the_kernels_cannot_take():
     limit = [dict(d=136), dict(width=4097), dict(n_buckets=1 << 21), dict(q_offset=1 << 30), dict(B=1 << 20, H=1 << 10, Nk=1 << 12)]
     assert [run(**b) for b in limit] == [-2] * len(limit)
     assert lib.ofb_relpos_fwd(None, None) == -1 and lib.ofb_relpos_bwd(None, None) == -1 and lib.ofb_relpos_sizes(None, None) == -1 and lib.ofb_relpos_amax(None, 0, 1, None) == -1
+
+
+def test_entries_refuse_launches_that_are_too_large():
+    """threads of a launch count in 32 bits; strides that the loads of 16 bytes cannot take"""
+    import ctypes as C
+    lib = hip.lib()
+    def args(**kw):
+        a = hip.RelposArgs()
+        for n, x in {**dict(q=16, k=16, v=16, table=16, lut=16, out=16, width=3, n_buckets=3, lo=-1, B=2, H=3, Nq=5, Nk=7, d=16, scale=1.0, dtype=1), **kw}.items():
+            setattr(a, n, x)
+        return C.byref(a)
+    assert lib.ofb_relpos_fwd(args(B=1 << 14, H=1 << 10, Nk=1), None) == -2
+    grads = dict(dout=16, out32=16, stats=16, delta=16, dq=16, dk=16, dv=16, dtable=16)
+    assert lib.ofb_relpos_bwd(args(B=1, H=1 << 10, n_buckets=1 << 14, **grads), None) == -2
+    assert lib.ofb_relpos_bwd(args(**grads), None) == -1      # no room for the table's parts
+    bounds = dict(bound_q=16, bound_k=16, bound_v=16)
+    assert lib.ofb_relpos_amax(args(q_st=12, **bounds), 0, 1, None) == -1 and lib.ofb_relpos_amax(args(v_sb=-8, **bounds), 0, 3, None) == -1
