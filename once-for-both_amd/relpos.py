@@ -3,6 +3,7 @@
 A query at position p and a key at position r share the bias table[bucket(r - p), head].  `RelPosBuckets` holds the bucket of every difference
 lo .. lo + width - 1 (differences beyond the ends take the end's bucket) and, where the positions are not simply the tokens' numbers, the
 positions themselves."""
+import numpy as np
 import torch
 
 from .hip import OfbError
@@ -62,15 +63,12 @@ class RelPosBuckets:
             device = torch.device('cuda', torch.cuda.current_device())
         got = self._on.get(device)
         if got is None:
-            order = sorted(range(self.width), key=lambda i: (self.lut[i], i))
-            start = [0] * (self.num_buckets + 1)
-            for c in self.lut:
-                start[c + 1] += 1
-            for c in range(self.num_buckets):
-                start[c + 1] += start[c]
-            parts = [self.lut, start, order] + (list(self.positions) if self.positions else [])
-            flat = torch.tensor([x for p in parts for x in p], dtype=torch.int32, device=device)
-            parts = list(flat.split([len(p) for p in parts]))
+            lut = np.asarray(self.lut)
+            start = np.cumsum(np.bincount(lut, minlength=self.num_buckets))
+            parts = [lut, [0], start, np.argsort(lut, kind='stable'), *(self.positions or ())]
+            flat = torch.from_numpy(np.concatenate(parts).astype(np.int32)).to(device)
+            sizes = [self.width, self.num_buckets + 1, self.width, *(len(p) for p in self.positions or ())]
+            parts = list(flat.split(sizes))
             got = self._on[device] = tuple(parts) if self.positions else (*parts, None, None)
             if device.type == 'cuda':
                 torch.cuda.current_stream(device).synchronize()      # any stream may read the plan from here on

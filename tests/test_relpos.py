@@ -123,3 +123,12 @@ def test_entries_refuse_launches_that_are_too_large():
     assert lib.ofb_relpos_bwd(args(**grads), None) == -1      # no room for the table's parts
     bounds = dict(bound_q=16, bound_k=16, bound_v=16)
     assert lib.ofb_relpos_amax(args(q_st=12, **bounds), 0, 1, None) == -1 and lib.ofb_relpos_amax(args(v_sb=-8, **bounds), 0, 3, None) == -1
+
+
+def test_what_a_plan_uploads():
+    for plan in (RelPosBuckets.grid(3, 2), RelPosBuckets([5, 0, 5, 2], -1, 9), RelPosBuckets.grid(1, 1), RelPosBuckets([0], 0, positions=([], []))):
+        lut, start, order, pq, pk = plan.on('cpu')
+        assert lut.tolist() == plan.lut and order.tolist() == sorted(range(plan.width), key=lambda i: (plan.lut[i], i))
+        assert start.tolist() == [sum(x < c for x in plan.lut) for c in range(plan.num_buckets + 1)]
+        assert all(t.dtype == torch.int32 for t in (lut, start, order))
+        assert (pq.tolist(), pk.tolist()) == tuple(plan.positions) if plan.positions else pq is None and pk is None
