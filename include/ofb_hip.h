@@ -540,8 +540,9 @@ int ofb_jpeg_decode_pixels(const ofb_jpeg_job* jobs_dev, int32_t n_images, int32
  * strides multiples of 4 elements).  d: a multiple of 8, at most 128.  lut[width]: bucket of each difference lo .. lo + width - 1 (differences are clamped; width <= 4096);
  * bucket_start[n_buckets + 1] / bucket_order[width]: the lut inverted (dtable only).  pos_q / pos_k: positions of the queries and keys, or
  * both NULL: i + q_offset and j.  Only index ranges are checked: lut entries must be < n_buckets.
- * f32 (forward and backward) and f16 (backward) read upper bounds of the tensors from bound_*: n_bound (n_bound_do) partial maxima each
- * (1 .. 256; ofb_relpos_amax writes 256). */
+ * f32 (forward and backward) and f16 (backward, v alone) scale by upper bounds of |k| and |v|: n_bound (1 .. 256) partial maxima each, for head
+ * b * H + h from bound_step * (b * H + h) on (ofb_relpos_amax writes 256 for all heads: step 0).  n_bound 0, where ofb_relpos_sizes allows it: the forward finds
+ * them by itself and leaves one a head in bound_k / bound_v [B * H] (or NULL), for the backward with n_bound = bound_step = 1. */
 typedef struct {
   const void *q, *k, *v;
   int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
@@ -554,8 +555,8 @@ typedef struct {
   int32_t lo, width, n_buckets, q_offset, causal, dtype;
   int32_t B, H, Nq, Nk, d;
   float scale;
-  const float *bound_q, *bound_k, *bound_v, *bound_do;
-  int32_t n_bound, n_bound_do;
+  float *bound_q, *bound_k, *bound_v, *bound_do;      /* bound_q (f32) and bound_do (f32, f16): workspaces of the backward */
+  int32_t n_bound, bound_step;
   float *split_o, *split_ml;    /* workspaces of ofb_relpos_sizes floats */
   const void* dout;
   int64_t do_sb, do_st, do_sh;
@@ -564,9 +565,9 @@ typedef struct {
   float* dtable;                /* [n_buckets][H], or NULL */
   float *delta, *partial, *sat; /* delta: [B][H][Nq]; the others of ofb_relpos_sizes floats */
 } ofb_relpos_args;
-/* out4[0..3]: floats of split_o, split_ml, partial, sat (0: not needed) */
-int ofb_relpos_sizes(const ofb_relpos_args* a, int64_t* out4);
-/* 256 partial maxima of |x| for `count` of q, k, v, dout (0 .. 3) from `first` on, into bound_*; tokens nobody sees are left out */
+/* out6[0..3]: floats of split_o, split_ml, partial, sat (0: not needed); [4]: of bound_q and of bound_do; [5]: 1 if the forward may have n_bound 0 */
+int ofb_relpos_sizes(const ofb_relpos_args* a, int64_t* out6);
+/* 256 partial maxima of |x| for `count` of k, v (0, 1) from `first` on, into bound_*; keys nobody sees, infinities and NaN are left out */
 int ofb_relpos_amax(const ofb_relpos_args* a, int32_t first, int32_t count, void* stream);
 int ofb_relpos_fwd(const ofb_relpos_args* a, void* stream);
 int ofb_relpos_bwd(const ofb_relpos_args* a, void* stream);

@@ -9,9 +9,10 @@
 // are j and i + q_offset, or come from two int32 arrays (a patch grid: y (2 w - 1) + x makes one number of two coordinates).
 //
 // Matrix products: v_mfma_f32_32x32x16.  bf16 and f16 operands as they are; f32 operands as two f16 planes of a power-of-two scaled copy and
-// three products (hformat.h), with the exponents from device-side maxima.  Scores, softmax statistics, dS and all sums are f32 (the
-// table's gradient sums in 64 bits); P and dS are rounded to the operand type for the second product: bf16 as they are,
-// f16 with dS times a power of two that keeps it below 2^15 (and P times 2^14 for dV), f32 likewise in two f16 planes.
+// three products (hformat.h), with exponents from the maxima of the tile (Q, dO, dS) or of the head (K, V; of all heads where a pass of its own
+// finds them).  Scores, softmax statistics, dS and all sums are f32 (the table's gradient sums in 64 bits); P and dS are rounded to the operand
+// type for the second product: bf16 as they are, f16 with dS times a power of two that keeps it below 2^15 (and P times 2^14 for dV), f32 likewise
+// in two f16 planes.
 //
 // Operand conventions (lane l, hh = l >> 5): A[row = l & 31][k = 8 hh + j], B[k = 8 hh + j][col = l & 31], accumulator register r holds
 // row 8 (r >> 2) + 4 hh + (r & 3) of column l & 31.  A reduction may run over its index in any order that both operands share, so an
@@ -28,6 +29,9 @@
 #define RP_WMAX 4096
 #define RP_PE 14                 /* f32's planes, and the backward's f16, hold P 2^14 */
 #define RP_NBOUND 256            /* partial maxima of a tensor */
+// Keys up to which a workgroup of the f32 forward reads its head's K and V once more for their maxima; a pass of its own over both otherwise.  Both, heads
+// of 64: 128 x 197 keys, 6 heads 68 and 73 us; 32 x 256, 6 heads 26 and 31; 16 x 512, 12 heads 65.5 and 67.5; 8 x 768 75.7 and 76.6; 8 x 1024 111 and 108.
+#define RP_OWN 512
 
 namespace {
 
@@ -203,12 +207,17 @@ __device__ __forceinline__ void rp_place(int x, int total, int tiles, bool causa
   }
 }
 
-// maxima of N tensors from their partial maxima (n of each <= RP_NBOUND), by every thread of the workgroup; red: [4][N]
-template <int N>
-__device__ __forceinline__ void rp_bounds(const float* const (&part)[N], const int (&n)[N], float (&out)[N], float* red) {
-  float v[N];
+// |x| for a maximum.  Infinities and NaN do not count: they pass the planes at any exponent, and the rows that do not meet them keep theirs
+__device__ __forceinline__ float rp_size(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; }
+template <int DT>
+__device__ __forceinline__ float rp_size8(const rp_chunk<DT>& c, float top) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = (int)threadIdx.x < n[i] ? part[i][threadIdx.x] : 0.f;
+  for (int j = 0; j < 8; ++j) top = fmaxf(top, rp_size(rp_chunk_at<DT>(c, j)));
+  return top;
+}
+// the maxima of N values over the workgroup, in every thread; red: [4][N]
+template <int N>
+__device__ __forceinline__ void rp_tops(float (&v)[N], float* red) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = ofb_wave_max(v[i]);
   if ((threadIdx.x & 63) == 0)
@@ -216,7 +225,36 @@ __device__ __forceinline__ void rp_bounds(const float* const (&part)[N], const i
     for (int i = 0; i < N; ++i) red[(threadIdx.x >> 6) * N + i] = v[i];
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < N; ++i) out[i] = fmaxf(fmaxf(red[i], red[N + i]), fmaxf(red[2 * N + i], red[3 * N + i]));
+  for (int i = 0; i < N; ++i) v[i] = fmaxf(fmaxf(red[i], red[N + i]), fmaxf(red[2 * N + i], red[3 * N + i]));
+}
+// this thread's share of the maxima over a tensor that are stored for head bh: n of them, step apart from head to head
+__device__ __forceinline__ float rp_part(const float* part, int64_t bh, int step, int n) {
+  float top = 0.f;
+  for (int i = threadIdx.x; i < n; i += RP_THREADS) top = fmaxf(top, part[bh * step + i]);
+  return top;
+}
+// this thread's share of the maxima of one head's first `keys` rows of k and v, eight chunks in flight
+template <int DT>
+__device__ __forceinline__ void rp_rows_top(const char* k, int64_t k_row, const char* v, int64_t v_row, int keys, int d, float& top_k, float& top_v) {
+  const int per = d / 8, groups = RP_THREADS / per, g = threadIdx.x / per, ch = threadIdx.x - g * per;
+  top_k = top_v = 0.f;
+  if (g >= groups) return;
+  k += 8 * ch * rp_type<DT>::ES;
+  v += 8 * ch * rp_type<DT>::ES;
+  for (int row = g; row < keys; row += 4 * groups) {
+    rp_chunk<DT> c[8];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t at = min(row + u * groups, keys - 1);
+      c[2 * u] = rp_load_chunk<DT>(k + at * k_row);
+      c[2 * u + 1] = rp_load_chunk<DT>(v + at * v_row);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      top_k = rp_size8<DT>(c[2 * u], top_k);
+      top_v = rp_size8<DT>(c[2 * u + 1], top_v);
+    }
+  }
 }
 
 // the head's bias by difference, times log2 e, padded by RP_PAD copies of its ends
@@ -302,9 +340,33 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 3 : DT == RP_F32 ? 1 : 2)) 
   if (kb0 < kb1) fetch(kb0);
   rp_bias_vector(a, head, w);
   float hq = 1.f, hk = 1.f, hv = 1.f, c_s = a.scale * 1.44269504088896340736f, c_o = 1.f;
+  const int q0 = qt * RP_TILE + wv * 32, qi = q0 + (lane & 31);
+  const bool active = q0 < a.Nq, qok = qi < a.Nq;
+  const int seen = a.causal ? min(kend, max(0, qi + a.q_offset + 1)) : kend;      // this query sees keys 0 .. seen - 1
+  rp_chunk<DT> qc[DP / 16];
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const int ch = 16 * s + 8 * hh;
+    qc[s] = rp_zero_chunk<DT>();
+    if (qok && ch < a.d) qc[s] = rp_load_chunk<DT>(qp + (int64_t)qi * a.q_st * ES + ch * ES);
+  }
   if constexpr (DT == RP_F32) {
-    float top[3];
-    rp_bounds<3>({a.bound_q, a.bound_k, a.bound_v}, {a.n_bound, a.n_bound, a.n_bound}, top, red);
+    // exponents of the planes: this tile's for Q, the head's for K and V
+    float top[3] = {0.f, 0.f, 0.f};
+    if (seen > 0)
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) top[0] = rp_size8<DT>(qc[s], top[0]);
+    if (a.n_bound) {
+      top[1] = rp_part(a.bound_k, bh, a.bound_step, a.n_bound);
+      top[2] = rp_part(a.bound_v, bh, a.bound_step, a.n_bound);
+    } else {
+      rp_rows_top<DT>(kp, a.k_st * ES, vp, a.v_st * ES, rp_keys_of(a, b), a.d, top[1], top[2]);
+    }
+    rp_tops(top, red);
+    if (!a.n_bound && a.bound_k && qt == 0 && threadIdx.x == 0) {
+      a.bound_k[bh] = top[1];
+      a.bound_v[bh] = top[2];
+    }
     const int eq = ofb_h_exp(top[0]), ek = ofb_h_exp(top[1]), ev = ofb_h_exp(top[2]);
     hq = ofb_h_pow2(eq); hk = ofb_h_pow2(ek); hv = ofb_h_pow2(ev);
     c_s = c_s * ofb_h_pow2(-eq) * ofb_h_pow2(-ek);
@@ -315,18 +377,10 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 3 : DT == RP_F32 ? 1 : 2)) 
   const float p_sc = DT == RP_F32 ? ofb_h_pow2(RP_PE) : 1.f;
   if constexpr (DT == RP_F32) c_o *= ofb_h_pow2(-RP_PE);
 
-  const int q0 = qt * RP_TILE + wv * 32, qi = q0 + (lane & 31);
-  const bool active = q0 < a.Nq, qok = qi < a.Nq;
   const int pq = POS ? (qok ? a.pos_q[qi] : 0) : qi + a.q_offset;
-  const int seen = a.causal ? min(kend, max(0, qi + a.q_offset + 1)) : kend;      // this query sees keys 0 .. seen - 1
   rp_frag qf[DP / 16][NP];
 #pragma unroll
-  for (int s = 0; s < DP / 16; ++s) {
-    const int ch = 16 * s + 8 * hh;
-    rp_chunk<DT> c = rp_zero_chunk<DT>();
-    if (qok && ch < a.d) c = rp_load_chunk<DT>(qp + (int64_t)qi * a.q_st * ES + ch * ES);
-    rp_planes<DT>(c, hq, qf[s]);
-  }
+  for (int s = 0; s < DP / 16; ++s) rp_planes<DT>(qc[s], hq, qf[s]);
   f32x16 O[DP / 32];
 #pragma unroll
   for (int t = 0; t < DP / 32; ++t) O[t] = rp_zero16();
@@ -502,24 +556,19 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_join_kernel(ofb_relpos_args
 // ------------------------------------------------------------------------------------------------------------------
 // backward
 // ------------------------------------------------------------------------------------------------------------------
+// top: this thread's share of the maxima of q, k, v and dout (f16: only the last two count)
 template <int DT>
-__device__ __forceinline__ rp_scales rp_all_scales(const ofb_relpos_args& a, float* red) {
+__device__ __forceinline__ rp_scales rp_all_scales(float (&top)[4], int d, float* red) {
   rp_scales e = {0, 0, 0, 0, 0};
   if constexpr (DT != RP_BF16) {
-    float top[4] = {0.f, 0.f, 0.f, 0.f};
+    rp_tops(top, red);
     if constexpr (DT == RP_F32) {
-      rp_bounds<4>({a.bound_q, a.bound_k, a.bound_v, a.bound_do}, {a.n_bound, a.n_bound, a.n_bound, a.n_bound_do}, top, red);
       e.eq = ofb_h_exp(top[0]);
       e.ek = ofb_h_exp(top[1]);
       e.ev = ofb_h_exp(top[2]);
       e.ed = ofb_h_exp(top[3]);
-    } else {
-      float two[2];
-      rp_bounds<2>({a.bound_v, a.bound_do}, {a.n_bound, a.n_bound_do}, two, red);
-      top[2] = two[0];
-      top[3] = two[1];
     }
-    e.es = ofb_h_exp(2.f * a.d * top[2] * top[3]);             // |dS| <= P (|dP| + |D|) <= 2 d max|dO| max|V|
+    e.es = ofb_h_exp(2.f * d * top[2] * top[3]);               // |dS| <= P (|dP| + |D|) <= 2 d max|dO| max|V|
   }
   return e;
 }
@@ -529,7 +578,7 @@ __device__ __forceinline__ rp_scales rp_all_scales(const ofb_relpos_args& a, flo
 // difference in LDS, as whole numbers, so that the order of the additions does not matter.  For f32 that happens on the way.  For bf16 and f16 D is
 // only known when a row is done (see below): the tiles with pairs between the ends are then visited once more, for S and dP alone.  (A pass of its own
 // that summed dS over the batch first, one histogram per pair of tiles, took 170 us beside 98 us of this kernel for the 14 x 14 grid, B 128, 6 x 64
-// f32, where this takes 124 us.)
+// f32, where this takes 110 us.)
 template <int DT, int DP, bool POS>
 __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : 2)) void relpos_dq_kernel(ofb_relpos_args a) {
   using G = rp_geo<DT, DP, rp_rows_of<DT, DP>(1)>;
@@ -565,32 +614,51 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : 2)) void
   if (kb1 > 0) fetch(0);
   rp_bias_vector(a, head, w);
   for (int i = threadIdx.x; i < wpad; i += RP_THREADS) hist[i] = 0ull;
-  const rp_scales e = rp_all_scales<DT>(a, red);
-  const float hq = ofb_h_pow2(e.eq), hk = ofb_h_pow2(e.ek), hv = ofb_h_pow2(e.ev), hd = ofb_h_pow2(e.ed);
-  const float c_s = a.scale * 1.44269504088896340736f * ofb_h_pow2(-e.eq) * ofb_h_pow2(-e.ek);
-  const int ek_ = e.es - e.ed - e.ev;                          // dP's accumulators times 2^ek_ are in dS's scale
-  const float c_dq = a.scale * ofb_h_pow2(-e.es) * ofb_h_pow2(-e.ek);
-
   const int q0 = qt * RP_TILE + wv * 32, qi = q0 + (lane & 31);
   const bool active = q0 < a.Nq, qok = qi < a.Nq;
   const int pq = POS ? (qok ? a.pos_q[qi] : 0) : qi + a.q_offset;
   const int seen = a.causal ? min(kend, max(0, qi + a.q_offset + 1)) : kend;
-  rp_frag qf[DP / 16][NP], df[DP / 16][NP];
+  rp_chunk<DT> qc[DP / 16], dc[DP / 16];
   float D = 0.f, m = 0.f, linv = 0.f;
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
     const int ch = 16 * s + 8 * hh;
-    rp_chunk<DT> c = rp_zero_chunk<DT>(), g = rp_zero_chunk<DT>();
+    qc[s] = dc[s] = rp_zero_chunk<DT>();
     if (qok && ch < a.d) {
-      c = rp_load_chunk<DT>(qp + (int64_t)qi * a.q_st * ES + ch * ES);
-      g = rp_load_chunk<DT>(dp + (int64_t)qi * a.do_st * ES + ch * ES);
+      qc[s] = rp_load_chunk<DT>(qp + (int64_t)qi * a.q_st * ES + ch * ES);
+      dc[s] = rp_load_chunk<DT>(dp + (int64_t)qi * a.do_st * ES + ch * ES);
       const float* o32 = a.out32 + (((int64_t)b * a.Nq + qi) * a.H + head) * a.d + ch;
       const f32x4 oa = *reinterpret_cast<const f32x4*>(o32), ob = *reinterpret_cast<const f32x4*>(o32 + 4);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) D = fmaf(rp_chunk_at<DT>(g, j), j < 4 ? oa[j & 3] : ob[j & 3], D);
+      for (int j = 0; j < 8; ++j) D = fmaf(rp_chunk_at<DT>(dc[s], j), j < 4 ? oa[j & 3] : ob[j & 3], D);
     }
-    rp_planes<DT>(c, hq, qf[s]);
-    rp_planes<DT>(g, hd, df[s]);
+  }
+  // exponents: this tile's for Q, dO and dS, the head's for K and V.  The dK dV kernel reads the tiles' maxima of Q and dO.
+  float top[4] = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (DT != RP_BF16) {
+    if (seen > 0)
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) {
+        if constexpr (DT == RP_F32) top[0] = rp_size8<DT>(qc[s], top[0]);
+        top[3] = rp_size8<DT>(dc[s], top[3]);
+      }
+    if constexpr (DT == RP_F32) top[1] = rp_part(a.bound_k, bh, a.bound_step, a.n_bound);
+    top[2] = rp_part(a.bound_v, bh, a.bound_step, a.n_bound);
+  }
+  const rp_scales e = rp_all_scales<DT>(top, a.d, red);
+  if (DT != RP_BF16 && threadIdx.x == 0) {
+    if constexpr (DT == RP_F32) a.bound_q[(int64_t)bh * nqt + qt] = top[0];
+    a.bound_do[(int64_t)bh * nqt + qt] = top[3];
+  }
+  const float hq = ofb_h_pow2(e.eq), hk = ofb_h_pow2(e.ek), hv = ofb_h_pow2(e.ev), hd = ofb_h_pow2(e.ed);
+  const float c_s = a.scale * 1.44269504088896340736f * ofb_h_pow2(-e.eq) * ofb_h_pow2(-e.ek);
+  const int ek_ = e.es - e.ed - e.ev;                          // dP's accumulators times 2^ek_ are in dS's scale
+  const float c_dq = a.scale * ofb_h_pow2(-e.es) * ofb_h_pow2(-e.ek);
+  rp_frag qf[DP / 16][NP], df[DP / 16][NP];
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    rp_planes<DT>(qc[s], hq, qf[s]);
+    rp_planes<DT>(dc[s], hd, df[s]);
   }
   OFB_XOR_STEP(D, ofb_add_, 32)
   if (qok) {
@@ -923,7 +991,17 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 2 : 1)) void relpos_dkv_ker
   int qb0 = 0, qb1 = (a.Nq + KB - 1) / KB;
   if (a.causal) qb0 = min(qb1, max(0, j_first - a.q_offset) / KB);
   if (j_first >= kend) qb0 = qb1;                              // nobody sees these keys: their gradients are zeros
-  const rp_scales e = rp_all_scales<DT>(a, red);
+  float top[4] = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (DT != RP_BF16) {
+    const int nqt = (a.Nq + RP_TILE - 1) / RP_TILE;
+    if constexpr (DT == RP_F32) {
+      top[0] = rp_part(a.bound_q, bh, nqt, nqt);
+      top[1] = rp_part(a.bound_k, bh, a.bound_step, a.n_bound);
+    }
+    top[2] = rp_part(a.bound_v, bh, a.bound_step, a.n_bound);
+    top[3] = rp_part(a.bound_do, bh, nqt, nqt);
+  }
+  const rp_scales e = rp_all_scales<DT>(top, a.d, red);
   rp_stage<DT, DP, KB> qs_, ds_;
   f32x4 st_next;
   int ps_next;
@@ -1042,20 +1120,16 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_table_kernel(ofb_relpos_arg
   if (threadIdx.x == 0) a.dtable[(int64_t)c * a.H + head] = (float)(red[0] + red[1] + red[2] + red[3]);
 }
 
-// partial maxima of |x| of up to three tensors (blockIdx.y), over the tokens that can be seen: what lies behind them may hold anything.
-// Infinities and NaN do not count: they pass the planes at any exponent, and the rows that do not meet them keep theirs
+// partial maxima of |x| of k and / or v (blockIdx.y), over the keys that can be seen: what lies behind them may hold anything
 template <int DT>
 __global__ __launch_bounds__(RP_THREADS) void relpos_amax_kernel(ofb_relpos_args a, int first) {
   constexpr int ES = rp_type<DT>::ES;
   __shared__ float red[4];
-  const int which = first + blockIdx.y;                        // 0 q, 1 k, 2 v, 3 dout
-  const char* x = (const char*)(which == 0 ? a.q : which == 1 ? a.k : which == 2 ? a.v : a.dout);
-  const int64_t sb = which == 0 ? a.q_sb : which == 1 ? a.k_sb : which == 2 ? a.v_sb : a.do_sb;
-  const int64_t st = which == 0 ? a.q_st : which == 1 ? a.k_st : which == 2 ? a.v_st : a.do_st;
-  const int64_t sh = which == 0 ? a.q_sh : which == 1 ? a.k_sh : which == 2 ? a.v_sh : a.do_sh;
-  const bool key = which == 1 || which == 2;
+  const bool is_k = first + blockIdx.y == 0;
+  const char* x = (const char*)(is_k ? a.k : a.v);
+  const int64_t sb = is_k ? a.k_sb : a.v_sb, st = is_k ? a.k_st : a.v_st, sh = is_k ? a.k_sh : a.v_sh;
   const int per = a.H * (a.d / 8);                             // chunks of a token
-  const int tokens = key ? a.Nk : a.Nq;
+  const int tokens = a.Nk;
   float v = 0.f;
   const int64_t rows = (int64_t)a.B * tokens;
   // a group of threads per token (`per` chunks each), four tokens' loads in flight
@@ -1071,8 +1145,7 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_amax_kernel(ofb_relpos_args
         p[u] = nullptr;
         if (at >= rows) continue;
         const int end = rp_keys_of(a, b);
-        const bool seen = key ? i < (a.causal ? min(end, max(0, a.Nq + a.q_offset)) : end) : end > 0 && !(a.causal && i + a.q_offset < 0);
-        if (seen) p[u] = x + (b * sb + (int64_t)i * st) * ES;
+        if (i < (a.causal ? min(end, max(0, a.Nq + a.q_offset)) : end)) p[u] = x + (b * sb + (int64_t)i * st) * ES;
       }
       for (int c = t0; c < per; c += group) {
         const int64_t off = ((c / (a.d / 8)) * sh + (c % (a.d / 8)) * 8) * ES;
@@ -1083,20 +1156,13 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_amax_kernel(ofb_relpos_args
           if (p[u]) q[u] = rp_load_chunk<DT>(p[u] + off);
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float y = fabsf(rp_chunk_at<DT>(q[u], j));
-            v = fmaxf(v, y < INFINITY ? y : 0.f);
-          }
+        for (int u = 0; u < 4; ++u) v = rp_size8<DT>(q[u], v);
       }
     }
   }
-  v = ofb_wave_max(v);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float* out = (float*)(which == 0 ? a.bound_q : which == 1 ? a.bound_k : which == 2 ? a.bound_v : a.bound_do);
-  if (threadIdx.x == 0) out[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  float top[1] = {v};
+  rp_tops(top, red);
+  if (threadIdx.x == 0) (is_k ? a.bound_k : a.bound_v)[blockIdx.x] = top[0];
 }
 
 template <int DT, int DP, int KERNEL> int rp_lds(const ofb_relpos_args& a) {
@@ -1128,6 +1194,9 @@ int rp_splits(const ofb_relpos_args& a) {
   return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 
+// f32: a workgroup of the forward finds its head's maxima of K and V by itself where that is little to read once more
+bool rp_own_bounds(const ofb_relpos_args& a) { return a.dtype == RP_F32 && a.Nk <= RP_OWN && rp_splits(a) == 1; }
+
 int rp_check(const ofb_relpos_args* a) {
   if (!a || !a->q || !a->k || !a->v || !a->table || !a->lut) return OFB_EINVAL;
   if (a->B < 1 || a->H < 1 || a->Nq < 1 || a->Nk < 1 || a->d < 8 || a->d % 8 || a->dtype < 0 || a->dtype > 2) return OFB_EINVAL;
@@ -1140,7 +1209,7 @@ int rp_check(const ofb_relpos_args* a) {
   if (!ofb_aligned16(a->q) || !ofb_aligned16(a->k) || !ofb_aligned16(a->v)) return OFB_EINVAL;
   for (int64_t s : {a->q_sb, a->q_st, a->q_sh, a->k_sb, a->k_st, a->k_sh, a->v_sb, a->v_st, a->v_sh})
     if (s % unit || s < 0) return OFB_EINVAL;
-  if (a->dtype == RP_F32 && (!a->bound_q || !a->bound_k || !a->bound_v || a->n_bound < 1 || a->n_bound > RP_NBOUND)) return OFB_EINVAL;
+  if (a->n_bound < 0 || a->n_bound > RP_NBOUND || a->bound_step < 0 || a->bound_step > RP_NBOUND) return OFB_EINVAL;
   return OFB_OK;
 }
 
@@ -1187,38 +1256,38 @@ template <int DT, int DP> int rp_backward(const ofb_relpos_args& a, hipStream_t 
 
 }  // namespace
 
-extern "C" int ofb_relpos_sizes(const ofb_relpos_args* a, int64_t* out4) {
-  if (!a || !out4 || a->B < 1 || a->H < 1 || a->Nq < 1 || a->Nk < 1 || a->width < 1) return OFB_EINVAL;
+extern "C" int ofb_relpos_sizes(const ofb_relpos_args* a, int64_t* out6) {
+  if (!a || !out6 || a->B < 1 || a->H < 1 || a->Nq < 1 || a->Nk < 1 || a->width < 1) return OFB_EINVAL;
   const int64_t rows = (int64_t)a->B * a->H * a->Nq, splits = rp_splits(*a);
-  out4[0] = splits > 1 ? splits * rows * a->d : 0;             // split_o
-  out4[1] = splits > 1 ? splits * rows * 2 : 0;                // split_ml
-  out4[2] = (int64_t)a->H * a->width * rp_table_rows(*a);      // partial
-  out4[3] = a->pos_k ? 0 : (int64_t)a->H * 2 * a->B * ((a->Nq + RP_TILE - 1) / RP_TILE) * 4;        // sat
+  out6[0] = splits > 1 ? splits * rows * a->d : 0;             // split_o
+  out6[1] = splits > 1 ? splits * rows * 2 : 0;                // split_ml
+  out6[2] = (int64_t)a->H * a->width * rp_table_rows(*a);      // partial
+  out6[3] = a->pos_k ? 0 : (int64_t)a->H * 2 * a->B * ((a->Nq + RP_TILE - 1) / RP_TILE) * 4;        // sat
+  out6[4] = (int64_t)a->B * a->H * ((a->Nq + RP_TILE - 1) / RP_TILE);        // bound_q, bound_do
+  out6[5] = rp_own_bounds(*a);
   return OFB_OK;
 }
 
 extern "C" int ofb_relpos_amax(const ofb_relpos_args* a, int32_t first, int32_t count, void* stream) {
-  if (!a || first < 0 || count < 1 || first + count > 4) return OFB_EINVAL;
-  if (a->B < 1 || a->H < 1 || a->Nq < 1 || a->Nk < 1 || a->d < 8 || a->d % 8 || a->dtype < 0 || a->dtype > 2) return OFB_EINVAL;
-  const void* x[4] = {a->q, a->k, a->v, a->dout};
-  const float* o[4] = {a->bound_q, a->bound_k, a->bound_v, a->bound_do};
-  const int64_t t[4][3] = {{a->q_sb, a->q_st, a->q_sh}, {a->k_sb, a->k_st, a->k_sh}, {a->v_sb, a->v_st, a->v_sh}, {a->do_sb, a->do_st, a->do_sh}};
-  const int64_t unit = a->dtype == RP_F32 ? 4 : 8;
+  if (!a || first < 0 || count < 1 || first + count > 2) return OFB_EINVAL;
+  if (a->B < 1 || a->H < 1 || a->Nq < 1 || a->Nk < 1 || a->d < 8 || a->d % 8 || (a->dtype != RP_F32 && a->dtype != RP_F16)) return OFB_EINVAL;
+  const int64_t t[2][3] = {{a->k_sb, a->k_st, a->k_sh}, {a->v_sb, a->v_st, a->v_sh}}, unit = a->dtype == RP_F32 ? 4 : 8;
   for (int i = first; i < first + count; ++i) {
-    if (!x[i] || !o[i] || !ofb_aligned16(x[i])) return OFB_EINVAL;
+    const void* x = i ? a->v : a->k;
+    if (!x || !(i ? a->bound_v : a->bound_k) || !ofb_aligned16(x)) return OFB_EINVAL;
     for (int64_t s : t[i])
       if (s % unit || s < 0) return OFB_EINVAL;
   }
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid(RP_NBOUND, count);
   if (a->dtype == RP_F32) hipLaunchKernelGGL((relpos_amax_kernel<RP_F32>), grid, dim3(RP_THREADS), 0, s, *a, first);
-  else if (a->dtype == RP_BF16) hipLaunchKernelGGL((relpos_amax_kernel<RP_BF16>), grid, dim3(RP_THREADS), 0, s, *a, first);
   else hipLaunchKernelGGL((relpos_amax_kernel<RP_F16>), grid, dim3(RP_THREADS), 0, s, *a, first);
   return ofb_launch_status();
 }
 
 extern "C" int ofb_relpos_fwd(const ofb_relpos_args* a, void* stream) {
   if (const int rc = rp_check(a)) return rc;
+  if (a->dtype == RP_F32 && (a->n_bound ? !a->bound_k || !a->bound_v : !rp_own_bounds(*a) || !a->bound_k != !a->bound_v)) return OFB_EINVAL;
   if (!a->out || !ofb_aligned16(a->out) || (a->out32 && !ofb_aligned16(a->out32))) return OFB_EINVAL;
   for (int64_t s : {a->o_sb, a->o_st, a->o_sh})
     if (s % 4 || s < 0) return OFB_EINVAL;
@@ -1230,7 +1299,8 @@ extern "C" int ofb_relpos_bwd(const ofb_relpos_args* a, void* stream) {
   if (!a->dout || !a->out32 || !a->stats || !a->delta || !a->dq || !a->dk || !a->dv) return OFB_EINVAL;
   if (a->dtable && (int64_t)a->n_buckets * a->H >= (1 << 24)) return OFB_ELIMIT;
   if (a->dtable && (!a->partial || !a->bucket_start || !a->bucket_order || (!a->pos_k && !a->sat))) return OFB_EINVAL;
-  if (a->dtype != RP_BF16 && (!a->bound_v || !a->bound_do || a->n_bound < 1 || a->n_bound > RP_NBOUND || a->n_bound_do < 1 || a->n_bound_do > RP_NBOUND)) return OFB_EINVAL;
+  if (a->dtype != RP_BF16 && (!a->bound_v || !a->bound_do || a->n_bound < 1)) return OFB_EINVAL;
+  if (a->dtype == RP_F32 && (!a->bound_q || !a->bound_k)) return OFB_EINVAL;
   for (const void* p : {(const void*)a->dout, (const void*)a->out32, (const void*)a->dq, (const void*)a->dk, (const void*)a->dv})
     if (!ofb_aligned16(p)) return OFB_EINVAL;
   const int64_t unit = a->dtype == RP_F32 ? 4 : 8;

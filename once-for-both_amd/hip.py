@@ -1216,7 +1216,7 @@ class RelposArgs(C.Structure):
         + [(n, C.c_int32) for n in ('lo', 'width', 'n_buckets', 'q_offset', 'causal', 'dtype', 'B', 'H', 'Nq', 'Nk', 'd')]
         + [('scale', C.c_float)]
         + [(n, C.c_void_p) for n in ('bound_q', 'bound_k', 'bound_v', 'bound_do')]
-        + [('n_bound', C.c_int32), ('n_bound_do', C.c_int32), ('split_o', C.c_void_p), ('split_ml', C.c_void_p), ('dout', C.c_void_p)]
+        + [('n_bound', C.c_int32), ('bound_step', C.c_int32), ('split_o', C.c_void_p), ('split_ml', C.c_void_p), ('dout', C.c_void_p)]
         + [(f'do_{s}', C.c_int64) for s in ('sb', 'st', 'sh')]
         + [(n, C.c_void_p) for n in ('dq', 'dk', 'dv')]
         + [(f'{t}_{s}', C.c_int64) for t in ('dq', 'dk', 'dv') for s in ('sb', 'st', 'sh')]
@@ -1236,8 +1236,8 @@ def relpos_tensor(args, name, t):
 
 
 def relpos_sizes(args):
-    """floats of the workspaces (split_o, split_ml, partial, sat)"""
-    out = (C.c_int64 * 4)()
+    """floats of the workspaces (split_o, split_ml, partial, sat, bound_q and bound_do each), and whether the forward finds its bounds by itself"""
+    out = (C.c_int64 * 6)()
     check(lib().ofb_relpos_sizes(C.byref(args), out), 'ofb_relpos_sizes')
     return list(out)
 

@@ -940,15 +940,19 @@ class _RelposCall:
         a.Nk, a.scale = k.shape[1], self.scale
         return a
 
-    def bounds(self, a, like):
-        """f32: upper bounds of |q|, |k|, |v| for the split into f16 planes - the caller's scalar, or the tensors' own maxima"""
+    def bounds(self, a, like, own, keep):
+        """f32: upper bounds of |k| and |v| for the split into f16 planes - the caller's scalar, the tensors' own maxima, or what the forward finds"""
         if self.bound is not None:
-            a.bound_q = a.bound_k = a.bound_v = self.bound.data_ptr()
+            a.bound_k = a.bound_v = self.bound.data_ptr()
             a.n_bound = 1
             return self.bound
-        part = torch.empty(3, hip.RELPOS_BOUNDS, device=like.device, dtype=torch.float32)
-        a.bound_q, a.bound_k, a.bound_v = (part.data_ptr() + 4 * hip.RELPOS_BOUNDS * i for i in range(3))
-        a.n_bound = hip.RELPOS_BOUNDS
+        if own and not keep:
+            return None
+        part = torch.empty(2, a.B * a.H if own else hip.RELPOS_BOUNDS, device=like.device, dtype=torch.float32)
+        a.bound_k, a.bound_v = part.data_ptr(), part.data_ptr() + 4 * part.shape[1]
+        if not own:
+            a.n_bound = hip.RELPOS_BOUNDS
+            hip.relpos_amax(a, 0, 2)
         return part
 
     def forward(self, q, k, v, table, key_lens, keep):
@@ -966,11 +970,9 @@ class _RelposCall:
                 stats = torch.empty(B, H, Nq, 2, device=q.device, dtype=torch.float32)
                 a.stats = stats.data_ptr()
                 a.out32 = None if out32 is out else out32.data_ptr()
-            if q.dtype == torch.float32:
-                bounds = self.bounds(a, q)
-                if self.bound is None:
-                    hip.relpos_amax(a, 0, 3)
             n = hip.relpos_sizes(a)
+            if q.dtype == torch.float32:
+                bounds = self.bounds(a, q, n[5], keep)
             if n[0]:
                 ws = torch.empty(n[0] + n[1], device=q.device, dtype=torch.float32)
                 a.split_o, a.split_ml = ws.data_ptr(), ws.data_ptr() + 4 * n[0]
@@ -991,24 +993,26 @@ class _RelposCall:
             for name, t in (('do', dout), ('dq', dq), ('dk', dk), ('dv', dv)):
                 hip.relpos_tensor(a, name, t)
             n = hip.relpos_sizes(a)
+            own, tiles = n[5], n[4] if q.dtype != torch.bfloat16 else 0
             n = [B * H * Nq, n[2] if want_table else 0, n[3] if want_table else 0]
-            ws = torch.empty(sum(n), device=q.device, dtype=torch.float32)
+            ws = torch.empty(sum(n) + 2 * tiles, device=q.device, dtype=torch.float32)
             a.out32, a.stats, a.delta = out32.data_ptr(), stats.data_ptr(), ws.data_ptr()
             if want_table:
                 dtable = torch.empty(table.shape, device=q.device, dtype=torch.float32)
                 a.dtable, a.partial = dtable.data_ptr(), ws.data_ptr() + 4 * n[0]
                 if n[2]:
                     a.sat = ws.data_ptr() + 4 * (n[0] + n[1])
-            if q.dtype != torch.bfloat16:                       # dS is scaled by a bound of it: maxima of v and dout
-                part = torch.empty(2, hip.RELPOS_BOUNDS, device=q.device, dtype=torch.float32)
-                if q.dtype == torch.float32:
-                    m = hip.RELPOS_BOUNDS if self.bound is None else 1
-                    a.bound_q, a.bound_k, a.bound_v = (bounds.data_ptr() + (4 * m * i if self.bound is None else 0) for i in range(3))
-                    a.n_bound = m
+            if tiles:                                           # dS is scaled by a bound of it: maxima of v and dout
+                a.bound_q, a.bound_do = ws.data_ptr() + 4 * sum(n), ws.data_ptr() + 4 * (sum(n) + tiles)
+                if q.dtype == torch.float16:
+                    bounds = torch.empty(hip.RELPOS_BOUNDS, device=q.device, dtype=torch.float32)
+                    a.bound_v, a.n_bound = bounds.data_ptr(), hip.RELPOS_BOUNDS
+                    hip.relpos_amax(a, 1, 1)
+                elif self.bound is not None:
+                    a.bound_k, a.bound_v, a.n_bound = bounds.data_ptr(), bounds.data_ptr(), 1
                 else:
-                    a.bound_v, a.n_bound = part.data_ptr(), hip.RELPOS_BOUNDS
-                a.bound_do, a.n_bound_do = part.data_ptr() + 4 * hip.RELPOS_BOUNDS, hip.RELPOS_BOUNDS
-                hip.relpos_amax(a, 3 if q.dtype == torch.float32 else 2, 1 if q.dtype == torch.float32 else 2)
+                    a.bound_k, a.bound_v = bounds.data_ptr(), bounds.data_ptr() + 4 * bounds.shape[1]
+                    a.n_bound, a.bound_step = (1, 1) if own else (hip.RELPOS_BOUNDS, 0)
             hip.relpos_bwd(a)
             return dtable
 

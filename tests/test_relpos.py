@@ -101,7 +101,7 @@ def test_entry_refuses_what_the_kernels_cannot_take():
             setattr(a, n, x)
         return lib.ofb_relpos_fwd(C.byref(a), None)
     bad = [dict(q=None), dict(q=8), dict(d=12), dict(d=0), dict(B=0), dict(Nq=0), dict(dtype=3), dict(width=0), dict(q_st=44), dict(v_sb=-8), dict(o_st=2), dict(pos_q=16),
-           dict(pos_q=16, pos_k=16, causal=1), dict(out=8), dict(dtype=0)]
+           dict(pos_q=16, pos_k=16, causal=1), dict(out=8), dict(dtype=0, n_bound=1), dict(dtype=0, Nk=5000), dict(dtype=0, bound_k=16), dict(n_bound=257), dict(n_bound=-1)]
     assert [run(**b) for b in bad] == [-1] * len(bad)
     limit = [dict(d=136), dict(width=4097), dict(n_buckets=1 << 21), dict(q_offset=1 << 30), dict(B=1 << 20, H=1 << 10, Nk=1 << 12)]
     assert [run(**b) for b in limit] == [-2] * len(limit)
