@@ -238,7 +238,8 @@ class VisionTransformer(nn.Module):
 
     @torch.jit.ignore
     def no_weight_decay(self):
-        return ['pos_embed', 'cls_token', 'dist_token']
+        tables = [n for n, _ in self.named_parameters() if n.endswith('relative_position_bias_table')]
+        return ['pos_embed', 'cls_token', 'dist_token'] + tables
 
     def get_classifier(self):
         return self.head

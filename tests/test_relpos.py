@@ -132,3 +132,16 @@ def test_what_a_plan_uploads():
         assert start.tolist() == [sum(x < c for x in plan.lut) for c in range(plan.num_buckets + 1)]
         assert all(t.dtype == torch.int32 for t in (lut, start, order))
         assert (pq.tolist(), pk.tolist()) == tuple(plan.positions) if plan.positions else pq is None and pk is None
+
+
+def test_bias_tables_are_not_decayed():
+    import ofb_amd
+    from ofb_amd.lr_decay import param_groups_lrd
+    m = ofb_amd.VisionTransformer(img_size=32, patch_size=8, embed_dim=32, depth=2, num_heads=2, num_classes=5, rel_pos_bias=True)
+    tables = [f'blocks.{i}.attn.relative_position_bias_table' for i in range(2)]
+    assert m.no_weight_decay() == ['pos_embed', 'cls_token', 'dist_token'] + tables
+    plain = ofb_amd.VisionTransformer(img_size=32, patch_size=8, embed_dim=32, depth=2, num_heads=2, num_classes=5)
+    assert plain.no_weight_decay() == ['pos_embed', 'cls_token', 'dist_token']
+    by_id = {id(p): n for n, p in m.named_parameters()}
+    kept = {by_id[id(p)] for g in param_groups_lrd(m, no_weight_decay_list=m.no_weight_decay()) if g['weight_decay'] == 0 for p in g['params']}
+    assert set(tables) <= kept
