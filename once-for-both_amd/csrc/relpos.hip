@@ -44,12 +44,12 @@ typedef rp_s16x8 rp_frag;
 template <int DT> struct rp_type { static constexpr int NP = 1, ES = 2; };
 template <> struct rp_type<RP_F32> { static constexpr int NP = 2, ES = 4; };
 
-// Rows of a streamed tile of kernel 0 forward, 1 dQ, 2 dK dV.  More rows are fewer barriers, until the staging registers or the LDS cost a workgroup, or
-// they spill.  Measured both sides: 16-bit, d 64 (6007 tokens, 16 heads): forward 128 rows 246, 64 rows 213 us; dK dV 64 rows 553, 128 rows 521 us;
+// Rows of a streamed tile of kernel 0 forward, 1 dQ, 2 dK dV, 3 dQ where workgroups are few (rp_few).  More rows are fewer barriers, until the staging
+// registers or the LDS cost a workgroup, or they spill.  Measured both sides: 16-bit, d 64 (6007 tokens, 16 heads): forward 128 rows 246, 64 rows 213 us; dK dV 64 rows 553, 128 rows 521 us;
 // dQ alike.  16-bit, d 128 (4 x 1025 causal, 8 heads): forward 32 rows 47, 64 rows 41 us; dK dV 87 and 68 us; dQ 89 and 119 us.  f32, d 64 (14 x 14 grid,
 // B 128): 32 rows 59 / 113 / 101 us, 64 rows 87 / 165 / 101 us.
 template <int DT, int DP> constexpr int rp_rows_of(int kernel) {
-  constexpr int f32[3] = {32, 32, 32}, narrow[3] = {64, 64, 128}, wide[3] = {64, 32, 64};
+  constexpr int f32[4] = {32, 32, 32, 32}, narrow[4] = {64, 64, 128, 64}, wide[4] = {64, 32, 64, 64};
   return DT == RP_F32 ? f32[kernel] : DP <= 64 ? narrow[kernel] : wide[kernel];
 }
 template <int DT, int DP, int ROWS> struct rp_geo {
@@ -579,9 +579,10 @@ __device__ __forceinline__ rp_scales rp_all_scales(float (&top)[4], int d, float
 // only known when a row is done (see below): the tiles with pairs between the ends are then visited once more, for S and dP alone.  (A pass of its own
 // that summed dS over the batch first, one histogram per pair of tiles, took 170 us beside 98 us of this kernel for the 14 x 14 grid, B 128, 6 x 64
 // f32, where this takes 110 us.)
-template <int DT, int DP, bool POS>
-__global__ __launch_bounds__(RP_THREADS, (DP > 64 && DT == RP_F32 ? 1 : 2)) void relpos_dq_kernel(ofb_relpos_args a) {
-  using G = rp_geo<DT, DP, rp_rows_of<DT, DP>(1)>;
+// FEW: see rp_few.
+template <int DT, int DP, bool POS, bool FEW>
+__global__ __launch_bounds__(RP_THREADS, (DP > 64 && (DT == RP_F32 || FEW) ? 1 : 2)) void relpos_dq_kernel(ofb_relpos_args a) {
+  using G = rp_geo<DT, DP, rp_rows_of<DT, DP>(FEW ? 3 : 1)>;
   constexpr int NP = G::NP, KB = G::KB, ES = rp_type<DT>::ES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ float red[16];
@@ -1168,7 +1169,7 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_amax_kernel(ofb_relpos_args
 template <int DT, int DP, int KERNEL> int rp_lds(const ofb_relpos_args& a) {
   using G = rp_geo<DT, DP, rp_rows_of<DT, DP>(KERNEL)>;
   const int w = ((a.width + 2 * RP_PAD + 3) & ~3) * 4;
-  return w * (KERNEL == 1 ? 3 : 1) + (KERNEL == 2 ? 8 : 2) * G::KB * 4 + 2 * G::STAGE;
+  return w * (KERNEL & 1 ? 3 : 1) + (KERNEL == 2 ? 8 : 2) * G::KB * 4 + 2 * G::STAGE;
 }
 
 template <typename F> int rp_allow(F* f, int bytes) {
@@ -1227,9 +1228,20 @@ template <int DT, int DP, bool POS> int rp_forward_of(const ofb_relpos_args& a, 
   return ofb_launch_status();
 }
 
+// 16-bit dQ with heads over 64, where there is at most one workgroup a CU (causal: half as many again, the short ones run behind each other): nothing is
+// lost if it takes more than half the registers, so nothing spills and a tile holds 64 keys, not 32.  Step with and without, heads of 128, 8 of them, causal: 2 x 1025
+// tokens 174 and 192 us, 4 x 1025 184 and 205, 6 x 1025 230 and 231, 8 x 1025 281 and 259; not causal: 2 x 1025 257 and 273, 4 x 1025 392 and 384.
+bool rp_few(const ofb_relpos_args& a) { return (int64_t)a.B * a.H * ((a.Nq + RP_TILE - 1) / RP_TILE) <= (a.causal ? 384 : 256); }
+
 template <int DT, int DP, bool POS> int rp_backward_of(const ofb_relpos_args& a, hipStream_t s) {
   const int nqt = (a.Nq + RP_TILE - 1) / RP_TILE, nkt = (a.Nk + RP_TILE - 1) / RP_TILE;
-  RP_LAUNCH((relpos_dq_kernel<DT, DP, POS>), dim3((unsigned)((int64_t)a.B * a.H * nqt)), (rp_lds<DT, DP, 1>(a)), s, a);
+  const dim3 grid((unsigned)((int64_t)a.B * a.H * nqt));
+  if constexpr (DT != RP_F32 && DP > 64) {
+    if (rp_few(a)) RP_LAUNCH((relpos_dq_kernel<DT, DP, POS, true>), grid, (rp_lds<DT, DP, 3>(a)), s, a);
+    else RP_LAUNCH((relpos_dq_kernel<DT, DP, POS, false>), grid, (rp_lds<DT, DP, 1>(a)), s, a);
+  } else {
+    RP_LAUNCH((relpos_dq_kernel<DT, DP, POS, false>), grid, (rp_lds<DT, DP, 1>(a)), s, a);
+  }
   RP_LAUNCH((relpos_dkv_kernel<DT, DP, POS>), dim3((unsigned)((int64_t)a.B * a.H * nkt)), (rp_lds<DT, DP, 2>(a)), s, a);
   if (a.dtable) {
     hipLaunchKernelGGL(relpos_table_kernel, dim3((unsigned)((int64_t)a.n_buckets * a.H)), dim3(RP_THREADS), 0, s, a, rp_table_rows(a),

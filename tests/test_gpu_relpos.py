@@ -376,3 +376,17 @@ def test_queries_beyond_32_bits():
         assert torch.equal(got[n][:, rows], alone[n]), n
     for n in ('dk', 'dv', 'dtable'):
         assert torch.isfinite(got[n]).all() and bool(got[n].any())
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'f16'])
+@pytest.mark.parametrize('d', [72, 128])
+def test_wide_heads_in_many_workgroups(d, dtype):
+    """more workgroups than the chip has CUs: causal or not, with given positions, and lengths"""
+    B, H = 5, 84
+    lens = torch.tensor([70, 1, 0, 33, 64], dtype=torch.int32, device='cuda')
+    g = torch.Generator().manual_seed(2)
+    plan = RelPosBuckets(range(21), -10, positions=(torch.randint(-15, 15, (40,), generator=g), torch.randint(-15, 15, (70,), generator=g)))
+    for plan, kw in ((PLANS['log8'](), dict(q_offset=30)), (PLANS['clip'](), dict(q_offset=25, causal=True)), (plan, {})):
+        q, k, v, table, dout = make(41 + d, B, 40, 70, H, d, DT[dtype], plan)
+        for n in (None, lens):
+            U.check(step(q, k, v, table, plan, dout, key_lens=n, **kw), U.reference(q, k, v, table, plan, key_lens=n, dout=dout, **kw))
