@@ -270,6 +270,12 @@ __device__ __forceinline__ int rp_keys_of(const ofb_relpos_args& a, int b) {
   return min(max(n, 0), a.Nk);
 }
 
+// the keys that any query of batch item b sees: what lies behind them may hold anything
+__device__ __forceinline__ int rp_seen_of(const ofb_relpos_args& a, int b) {
+  const int n = rp_keys_of(a, b);
+  return a.causal ? min(n, max(0, a.Nq + a.q_offset)) : n;
+}
+
 typedef __attribute__((address_space(3))) const float rp_lds_float;
 // the same value in every lane, as a scalar
 __device__ __forceinline__ float rp_uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
@@ -353,14 +359,13 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 3 : DT == RP_F32 ? 1 : 2)) 
   if constexpr (DT == RP_F32) {
     // exponents of the planes: this tile's for Q, the head's for K and V
     float top[3] = {0.f, 0.f, 0.f};
-    if (seen > 0)
 #pragma unroll
-      for (int s = 0; s < DP / 16; ++s) top[0] = rp_size8<DT>(qc[s], top[0]);
+    for (int s = 0; s < DP / 16; ++s) top[0] = rp_size8<DT>(qc[s], top[0]);
     if (a.n_bound) {
       top[1] = rp_part(a.bound_k, bh, a.bound_step, a.n_bound);
       top[2] = rp_part(a.bound_v, bh, a.bound_step, a.n_bound);
     } else {
-      rp_rows_top<DT>(kp, a.k_st * ES, vp, a.v_st * ES, rp_keys_of(a, b), a.d, top[1], top[2]);
+      rp_rows_top<DT>(kp, a.k_st * ES, vp, a.v_st * ES, rp_seen_of(a, b), a.d, top[1], top[2]);
     }
     rp_tops(top, red);
     if (!a.n_bound && a.bound_k && qt == 0 && threadIdx.x == 0) {
@@ -637,12 +642,12 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && (DT == RP_F32 || FEW) ? 1 :
   // exponents: this tile's for Q, dO and dS, the head's for K and V.  The dK dV kernel reads the tiles' maxima of Q and dO.
   float top[4] = {0.f, 0.f, 0.f, 0.f};
   if constexpr (DT != RP_BF16) {
-    if (seen > 0)
+    // (rows that see nothing count too: the dK dV kernel multiplies them by zeros, so they must stay finite)
 #pragma unroll
-      for (int s = 0; s < DP / 16; ++s) {
-        if constexpr (DT == RP_F32) top[0] = rp_size8<DT>(qc[s], top[0]);
-        top[3] = rp_size8<DT>(dc[s], top[3]);
-      }
+    for (int s = 0; s < DP / 16; ++s) {
+      if constexpr (DT == RP_F32) top[0] = rp_size8<DT>(qc[s], top[0]);
+      top[3] = rp_size8<DT>(dc[s], top[3]);
+    }
     if constexpr (DT == RP_F32) top[1] = rp_part(a.bound_k, bh, a.bound_step, a.n_bound);
     top[2] = rp_part(a.bound_v, bh, a.bound_step, a.n_bound);
   }
@@ -988,7 +993,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 2 : 1)) void relpos_dkv_ker
   const char* kp = (const char*)a.k + (b * a.k_sb + head * a.k_sh) * ES;
   const char* vp = (const char*)a.v + (b * a.v_sb + head * a.v_sh) * ES;
   const char* dp = (const char*)a.dout + (b * a.do_sb + head * a.do_sh) * ES;
-  const int kend = rp_keys_of(a, b), j_first = kt * RP_TILE;
+  const int kend = rp_seen_of(a, b), j_first = kt * RP_TILE;
   int qb0 = 0, qb1 = (a.Nq + KB - 1) / KB;
   if (a.causal) qb0 = min(qb1, max(0, j_first - a.q_offset) / KB);
   if (j_first >= kend) qb0 = qb1;                              // nobody sees these keys: their gradients are zeros
@@ -1145,8 +1150,7 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_amax_kernel(ofb_relpos_args
         const int b = (int)(at / tokens), i = (int)(at - (int64_t)b * tokens);
         p[u] = nullptr;
         if (at >= rows) continue;
-        const int end = rp_keys_of(a, b);
-        if (i < (a.causal ? min(end, max(0, a.Nq + a.q_offset)) : end)) p[u] = x + (b * sb + (int64_t)i * st) * ES;
+        if (i < rp_seen_of(a, b)) p[u] = x + (b * sb + (int64_t)i * st) * ES;
       }
       for (int c = t0; c < per; c += group) {
         const int64_t off = ((c / (a.d / 8)) * sh + (c % (a.d / 8)) * 8) * ES;

@@ -1065,7 +1065,7 @@ def relpos_attention(q, k, v, table, buckets, scale=None, causal=False, key_lens
     q (B, Nq, H, d), k and v (B, Nk, H, d): float32, bfloat16 or float16, any strides (channels that are not contiguous or rows that are not 16-byte aligned
     are copied first), d a multiple of 8 up to 128; table (buckets.num_buckets, H) float32; buckets a RelPosBuckets; scale d^-0.5 by default.
     Key j stands at position j and query i at i + q_offset (new tokens behind a cache: q_offset = Nk - Nq), unless the plan has positions of its own.
-    causal: a query sees the keys at or before its position.  key_lens (B,) int32: keys from there on are padding - they are not read, and
+    causal: a query sees the keys at or before its position; keys behind the last query's are not read.  key_lens (B,) int32: keys from there on are padding - they are not read, and
     their gradients are zero; a length beyond Nk counts as Nk, one below 0 as 0.  A query that sees no key has output and gradients 0.
     Returns (B, Nq, H, d) of q's type.  Differentiable once, in q, k, v and the table; the same inputs give the same bits.  A NaN or infinity makes the rows,
     and the gradients, that meet it NaN, and the table's gradient of its head."""

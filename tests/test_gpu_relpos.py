@@ -390,3 +390,25 @@ def test_wide_heads_in_many_workgroups(d, dtype):
         q, k, v, table, dout = make(41 + d, B, 40, 70, H, d, DT[dtype], plan)
         for n in (None, lens):
             U.check(step(q, k, v, table, plan, dout, key_lens=n, **kw), U.reference(q, k, v, table, plan, key_lens=n, dout=dout, **kw))
+
+
+@pytest.mark.parametrize('dtype', list(DT))
+@pytest.mark.parametrize('N', [40, 100, 600])
+def test_large_values_that_nobody_meets(dtype, N):
+    """causal: queries before the first key may be far larger than the others, and keys after the last query hold anything (unused places of a cache)"""
+    plan = PLANS['causal']()
+    big = 6e4 if dtype == 'f16' else 1e30
+    q, k, v, table, dout = make(19, 2, 70, N, 2, 64, DT[dtype], plan)
+    want = U.reference(q, k, v, table, plan, causal=True, q_offset=-30, dout=dout)      # queries 0 .. 29 see nothing, keys from 40 on are not seen
+    base = step(q, k, v, table, plan, dout, causal=True, q_offset=-30)
+    U.check(base, want)
+    far_k, far_v = k.clone(), v.clone()
+    for x in (big, math.nan):
+        far_k[:, 40:], far_v[:, 40:] = x, -x
+        got = step(q, far_k, far_v, table, plan, dout, causal=True, q_offset=-30)
+        U.check(got, want)
+        assert not got['dk'][:, 40:].any() and not got['dv'][:, 40:].any()
+    far_q, far_do = q.clone(), dout.clone()
+    far_q[:, :30], far_do[:, :30] = 1e4, -1e4
+    got = step(far_q, k, v, table, plan, far_do, causal=True, q_offset=-30)
+    U.check(got, U.reference(far_q, k, v, table, plan, causal=True, q_offset=-30, dout=far_do))
