@@ -625,7 +625,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && (DT == RP_F32 || FEW) ? 1 :
   const int pq = POS ? (qok ? a.pos_q[qi] : 0) : qi + a.q_offset;
   const int seen = a.causal ? min(kend, max(0, qi + a.q_offset + 1)) : kend;
   rp_chunk<DT> qc[DP / 16], dc[DP / 16];
-  float D = 0.f, m = 0.f, linv = 0.f;
+  float D = 0.f, m = INFINITY, linv = 0.f;                     // (a row behind the last query has P = 0 whatever its biases are)
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
     const int ch = 16 * s + 8 * hh;
@@ -887,12 +887,12 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && (DT == RP_F32 || FEW) ? 1 :
   }
 }
 
-// a query tile's row statistics for LDS: the maximum, 1 / sum times the operand's scale 2^pe, -D in dP's scale 2^de; a row without keys or behind the
-// last query gets P = 0
+// a query tile's row statistics for LDS: the maximum, 1 / sum times the operand's scale 2^pe, -D in dP's scale 2^de; a row without keys has 1 / sum 0, one
+// behind the last query a maximum of infinity: P = 0
 template <int KB, bool POS>
 __device__ __forceinline__ void rp_row_stats(const ofb_relpos_args& a, int64_t bh, int row0, int pe, int de, f32x4& v, int& pos) {
   const int i = row0 + threadIdx.x;
-  v = f32x4{0.f, 0.f, 0.f, 0.f};
+  v = f32x4{INFINITY, 0.f, 0.f, 0.f};                          // (a maximum of 0 would leave exp2 of a large bias there: infinity times 0)
   pos = 0;
   if (threadIdx.x < KB && i < a.Nq) {
     const int64_t row = bh * a.Nq + i;

@@ -412,3 +412,17 @@ def test_large_values_that_nobody_meets(dtype, N):
     far_q[:, :30], far_do[:, :30] = 1e4, -1e4
     got = step(far_q, k, v, table, plan, far_do, causal=True, q_offset=-30)
     U.check(got, U.reference(far_q, k, v, table, plan, causal=True, q_offset=-30, dout=far_do))
+
+
+@pytest.mark.parametrize('dtype', list(DT))
+@pytest.mark.parametrize('Nq', [1, 70, 161])
+def test_biases_beyond_the_exponential(dtype, Nq):
+    """buckets of +150, -200 and +1000: their exponentials are infinite or 0, the softmax is not (nor are the rows behind the last query, where such a bias meets no
+    score)"""
+    for name, causal in (('clip', False), ('log8', False), ('causal', True)):
+        plan = PLANS[name]()
+        for big, low in ((150.0, -200.0), (1000.0, 0.0)):
+            q, k, v, table, dout = make(23, 2, Nq, 170, 2, 64, DT[dtype], plan)
+            table[-1], table[1], table[2] = big, low, big - 3.0
+            kw = dict(q_offset=170 - Nq if causal else 3, causal=causal)
+            U.check(step(q, k, v, table, plan, dout, **kw), U.reference(q, k, v, table, plan, dout=dout, **kw))
