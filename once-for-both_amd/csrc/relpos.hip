@@ -12,7 +12,7 @@
 // three products (hformat.h), with exponents from the maxima of the tile (Q, dO, dS) or of the head (K, V; of all heads where a pass of its own
 // finds them).  Scores, softmax statistics, dS and all sums are f32 (the table's gradient sums in 64 bits); P and dS are rounded to the operand
 // type for the second product: bf16 as they are, f16 with dS times a power of two that keeps it below 2^15 (and P times 2^14 for dV), f32 likewise
-// in two f16 planes.
+// in two f16 planes.  (Exponents of f32 operands end at 2^60: a tensor whose maximum is below 2^-45 is held to 2^-85.)
 //
 // Operand conventions (lane l, hh = l >> 5): A[row = l & 31][k = 8 hh + j], B[k = 8 hh + j][col = l & 31], accumulator register r holds
 // row 8 (r >> 2) + 4 hh + (r & 3) of column l & 31.  A reduction may run over its index in any order that both operands share, so an
@@ -28,6 +28,7 @@
 #define RP_PAD 4                 /* entries of w on either side, so that four consecutive differences need one clamp */
 #define RP_WMAX 4096
 #define RP_PE 14                 /* f32's planes, and the backward's f16, hold P 2^14 */
+#define RP_ESMAX 100             /* dS is scaled by 2^-100 .. 2^60 */
 #define RP_NBOUND 256            /* partial maxima of a tensor */
 // Keys up to which a workgroup of the f32 forward reads its head's K and V once more for their maxima; a pass of its own over both otherwise.  Both, heads
 // of 64: 128 x 197 keys, 6 heads 68 and 73 us; 32 x 256, 6 heads 26 and 31; 16 x 512, 12 heads 65.5 and 67.5; 8 x 768 75.7 and 76.6; 8 x 1024 111 and 108.
@@ -573,7 +574,15 @@ __device__ __forceinline__ rp_scales rp_all_scales(float (&top)[4], int d, float
       e.ev = ofb_h_exp(top[2]);
       e.ed = ofb_h_exp(top[3]);
     }
-    e.es = ofb_h_exp(2.f * d * top[2] * top[3]);               // |dS| <= P (|dP| + |D|) <= 2 d max|dO| max|V|
+    // |dS| <= P (|dP| + |D|) <= 2 d max|dO| max|V| = m 2^ex, m in [0.5, 1): m 2^15 in its scale, as long as that is a power of two that f32 has room for
+    // (the factors' exponents apart: their product may leave f32)
+    int ev, ed, ec;
+    const float m = frexpf(top[2], &ev) * frexpf(top[3], &ed) * frexpf(2.f * d, &ec);
+    if (m > 0.f) {
+      int ex;
+      frexpf(m, &ex);
+      e.es = max(-RP_ESMAX, min(OFB_H_EMAX, 15 - ex - ev - ed - ec));
+    }
   }
   return e;
 }

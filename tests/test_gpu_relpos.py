@@ -426,3 +426,14 @@ def test_biases_beyond_the_exponential(dtype, Nq):
             table[-1], table[1], table[2] = big, low, big - 3.0
             kw = dict(q_offset=170 - Nq if causal else 3, causal=causal)
             U.check(step(q, k, v, table, plan, dout, **kw), U.reference(q, k, v, table, plan, dout=dout, **kw))
+
+
+@pytest.mark.parametrize('v_size,do_size', [(1e-22, 1e-25), (1e-30, 1e-30), (0.0, 1e-30), (1.0, 1e-30), (1e12, 1e12)])
+def test_gradients_whose_scale_leaves_f32(v_size, do_size):
+    """the product of the maxima of v and dout underflows, or is large.  Exponents of the planes end at 2^60: an operand whose maximum is below 2^-45 is held to 2^-85, half a
+    subnormal step of f16, so out and dv are off by N 2^-85 at most and dq, dk, dtable by the N |q| or N |k| <= 600 x 5 roundings of dS that they sum: 1e-22 in all"""
+    plan = PLANS['clip']()
+    for N in (70, 600):
+        q, k, v, table, dout = make(27, 1, N, N, 1, 64, torch.float32, plan)
+        v, dout = v * v_size, dout * do_size
+        U.check(step(q, k, v, table, plan, dout), U.reference(q, k, v, table, plan, dout=dout), tiny=1e-22)
