@@ -11,7 +11,8 @@
 //                  = tau q_j (1 - p_r / q_r) = tau exp(y_j - m_t) (q_r - p_r) / s_t   for the others
 // where m_t and s_t are the maximum of y and the sum of exp(y - m_t) over the classes that are NOT stored: they are summed apart (a bit per
 // class in LDS says which is stored), so that log q_r and the small tail gradients do not come out of a difference of nearly equal sums.
-// Exponentials are exp2 of one fma (y log2 e - m): their argument's rounding is relative to the distance from the maximum.
+// Exponentials are exp2 of (z - m) log2 e / tau with m in z's own units: exactly 0 at the maximum, and rounded relative to the distance from it, whatever the
+// logits' size is.  (One fma of z with -m log2 e / tau instead leaves the rounding of that product there: 2^103 at bf16's lowest value.)
 #include "hformat.h"
 
 #define DS_F32 0
@@ -23,7 +24,7 @@
 #define DS_STATS 8                /* floats kept per row: m_t, kappa, m, 1/s, m_teacher, 1/s_teacher, used, 0 */
 #define TL_CAP 4096               /* candidates of a row or segment that are ranked at once */
 #define TL_THREADS 1024
-#define TL_SMALL 256              /* threads for lists of up to TL_SMALL / 2: 1024 x 100003 bf16, 64 kept: 75 us, 1024 threads 99 us */
+#define TL_SMALL 256              /* threads for lists of up to TL_SMALL / 2: 1024 x 100003 bf16, 64 kept: 78 us, 1024 threads 102 us */
 
 namespace {
 
@@ -123,7 +124,7 @@ struct ds_row {
   }
 };
 
-// running maximum and sum of exp2(y - max), y = x c
+// running maximum m and sum of exp2((x - m) c)
 struct ds_sum {
   float m = -INFINITY, s = 0.f;
   template <int CH>
@@ -131,18 +132,17 @@ struct ds_sum {
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < CH; ++i) top = fmaxf(top, x[i]);
-    top *= c;
     if (top > m) {                                            // (-inf alone: nothing to add; NaN: added below, the sum becomes NaN)
-      s *= __builtin_amdgcn_exp2f(m - top);
+      s *= __builtin_amdgcn_exp2f((m - top) * c);
       m = top;
     }
     const float mu = m > -INFINITY ? m : 0.f;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) s += __builtin_amdgcn_exp2f(fmaf(x[i], c, -mu));
+    for (int i = 0; i < CH; ++i) s += __builtin_amdgcn_exp2f((x[i] - mu) * c);
   }
-  __device__ __forceinline__ void join(float m2, float s2) {
+  __device__ __forceinline__ void join(float m2, float s2, float c) {
     const float n = fmaxf(m, m2), mu = n > -INFINITY ? n : 0.f;
-    s = s * __builtin_amdgcn_exp2f(m - mu) + s2 * __builtin_amdgcn_exp2f(m2 - mu);
+    s = s * __builtin_amdgcn_exp2f((m - mu) * c) + s2 * __builtin_amdgcn_exp2f((m2 - mu) * c);
     m = n;
   }
 };
@@ -165,12 +165,12 @@ __device__ __forceinline__ double ds_total(double v, double* red) {
   return v;
 }
 template <int THREADS>
-__device__ __forceinline__ ds_sum ds_join(ds_sum a, float* redm, float* reds) {
+__device__ __forceinline__ ds_sum ds_join(ds_sum a, float c, float* redm, float* reds) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     const float m2 = __shfl_xor(a.m, o, 64), s2 = __shfl_xor(a.s, o, 64);
     const float n = fmaxf(a.m, m2), mu = n > -INFINITY ? n : 0.f;      // (symmetric: every lane computes the same)
-    const float x = a.s * __builtin_amdgcn_exp2f(a.m - mu), y = s2 * __builtin_amdgcn_exp2f(m2 - mu);
+    const float x = a.s * __builtin_amdgcn_exp2f((a.m - mu) * c), y = s2 * __builtin_amdgcn_exp2f((m2 - mu) * c);
     a.s = x + y;
     a.m = n;
   }
@@ -181,7 +181,7 @@ __device__ __forceinline__ ds_sum ds_join(ds_sum a, float* redm, float* reds) {
   r.m = redm[0];
   r.s = reds[0];
 #pragma unroll
-  for (int i = 1; i < THREADS / 64; ++i) r.join(redm[i], reds[i]);
+  for (int i = 1; i < THREADS / 64; ++i) r.join(redm[i], reds[i], c);
   return r;
 }
 
@@ -253,34 +253,34 @@ __device__ void ds_finish(const ds_args& a, int64_t row, ds_sum tail, ds_entries
   float mt = -INFINITY, m = tail.m;
   for (int k = lane; k < a.K; k += 64) {
     if (e.cls[k] < 0) continue;
-    mt = fmaxf(mt, e.t[k] * a.c);
-    m = fmaxf(m, e.y[k] * a.c);
+    mt = fmaxf(mt, e.t[k]);
+    m = fmaxf(m, e.y[k]);
   }
   mt = ofb_wave_max(mt);
   m = ofb_wave_max(m);
   const bool any = classes > 0, all = classes >= a.V;                              // every class is stored: there is no rest
-  const float r2 = (a.rest && !all) ? a.rest[row] * 1.44269504088896340736f : -INFINITY;
-  mt = fmaxf(mt, r2);
+  const double r2 = (a.rest && !all) ? (double)a.rest[row] * 1.44269504088896340736 : -INFINITY;
+  mt = fmaxf(mt, (float)(r2 / (double)a.c));
   const float mtu = mt > -INFINITY ? mt : 0.f, mu = m > -INFINITY ? m : 0.f;
   double st = 0.0, s = 0.0;
   for (int k = lane; k < a.K; k += 64) {
     if (e.cls[k] < 0) continue;
-    st += (double)__builtin_amdgcn_exp2f(fmaf(e.t[k], a.c, -mtu));
-    s += (double)__builtin_amdgcn_exp2f(fmaf(e.own[k], a.c, -mu));
+    st += (double)__builtin_amdgcn_exp2f((e.t[k] - mtu) * a.c);
+    s += (double)__builtin_amdgcn_exp2f((e.own[k] - mu) * a.c);
   }
-  const float er = __builtin_amdgcn_exp2f(r2 - mtu), et = tail.s > 0.f ? tail.s * __builtin_amdgcn_exp2f(tail.m - mu) : tail.s;
+  const float er = __builtin_amdgcn_exp2f((float)(r2 - (double)mtu * (double)a.c)), et = tail.s > 0.f ? tail.s * __builtin_amdgcn_exp2f((tail.m - mu) * a.c) : tail.s;
   st = ds_wave_sum(st) + (double)er;
   s = ds_wave_sum(s) + (double)et;
-  const double L2 = (double)mtu + log2(st), A2 = (double)mu + log2(s), ci = 1.0 / st;
+  const double c = (double)a.c, lt = log2(st), ls = log2(s), ci = 1.0 / st;      // (logarithms relative to the maxima: log V does not survive beside 1e38)
   double loss = 0.0;
   for (int k = lane; k < a.K; k += 64) {
     if (e.cls[k] < 0) continue;
-    const double p = (double)__builtin_amdgcn_exp2f(fmaf(e.t[k], a.c, -mtu)) * ci;
-    loss += p * ((double)e.t[k] * (double)a.c - L2 - (double)e.y[k] * (double)a.c + A2);
+    const double p = (double)__builtin_amdgcn_exp2f((e.t[k] - mtu) * a.c) * ci;
+    loss += p * (((double)e.t[k] - (double)mtu) * c - lt - ((double)e.y[k] - (double)mu) * c + ls);
   }
   loss = ds_wave_sum(loss);
   const double pr = (double)er * ci;
-  if (pr > 0.0) loss += pr * ((double)r2 - L2 - ((double)tail.m + log2((double)tail.s) - A2));
+  if (pr > 0.0) loss += pr * (r2 - (double)mtu * c - lt - (((double)tail.m - (double)mu) * c + log2((double)tail.s) - ls));
   if (lane == 0) {
     float* o = a.stats + row * DS_STATS;
     o[0] = tail.m > -INFINITY ? tail.m : 0.f;
@@ -334,7 +334,7 @@ __global__ __launch_bounds__(DS_THREADS) void distill_fwd_kernel(ds_args a) {
     }
     sum.add<N>(x, a.c);
   });
-  sum = ds_join<DS_THREADS>(sum, redf, redf + 4);
+  sum = ds_join<DS_THREADS>(sum, a.c, redf, redf + 4);
   if constexpr (WHOLE) {
     if (threadIdx.x < 64) ds_finish(a, row, sum, e, classes);
   } else if (threadIdx.x == 0) {
@@ -350,9 +350,9 @@ __global__ __launch_bounds__(DS_THREADS) void distill_finish_kernel(ds_args a) {
   __shared__ float redf[8];
   const int64_t row = blockIdx.x;
   ds_sum sum;
-  for (int i = threadIdx.x; i < a.segs; i += DS_THREADS) sum.join(a.part[2 * (row * a.segs + i)], a.part[2 * (row * a.segs + i) + 1]);
+  for (int i = threadIdx.x; i < a.segs; i += DS_THREADS) sum.join(a.part[2 * (row * a.segs + i)], a.part[2 * (row * a.segs + i) + 1], a.c);
   const int classes = ds_load_entries<DT>(a, row, e);
-  sum = ds_join<DS_THREADS>(sum, redf, redf + 4);
+  sum = ds_join<DS_THREADS>(sum, a.c, redf, redf + 4);
   if (threadIdx.x < 64) ds_finish(a, row, sum, e, classes);
 }
 
@@ -382,7 +382,7 @@ __global__ __launch_bounds__(DS_THREADS) void distill_bwd_kernel(ds_args a) {
   char* out = (char*)a.dz + (row * a.V - r.mis) * (int64_t)ds_type<DT>::ES;
   r.template each<DS_THREADS, false>(c0, c1, 0.f, [&](int c, float (&x)[CH]) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i) x[i] = used ? __builtin_amdgcn_exp2f(fmaf(x[i], a.c, -mt)) * kappa : 0.f;
+    for (int i = 0; i < CH; ++i) x[i] = used ? __builtin_amdgcn_exp2f((x[i] - mt) * a.c) * kappa : 0.f;
     char* p = out + (int64_t)c * 16;
     if (r.whole(c)) {
       if constexpr (DT == DS_F32) {
@@ -406,7 +406,7 @@ __global__ __launch_bounds__(DS_THREADS) void distill_bwd_kernel(ds_args a) {
   for (int k = threadIdx.x; k < ((a.K + 3) & ~3); k += DS_THREADS) {
     float v = 0.f;
     cls[k] = k < a.K ? ds_class<DT>(a, row, k, v) : -1;
-    prob[k] = cls[k] < 0 ? 0.f : __builtin_amdgcn_exp2f(fmaf(v, a.c, -mk)) * ik;
+    prob[k] = cls[k] < 0 ? 0.f : __builtin_amdgcn_exp2f((v - mk) * a.c) * ik;
   }
   __syncthreads();                                             // ... and the stores above come before those below
   for (int k = threadIdx.x; k < a.K; k += DS_THREADS) {
@@ -422,7 +422,7 @@ __global__ __launch_bounds__(DS_THREADS) void distill_bwd_kernel(ds_args a) {
       if (o.w == i && e + 3 > k) p += prob[e + 3];
     }
     const int64_t at = row * a.V + i;
-    const float q = __builtin_amdgcn_exp2f(fmaf(ds_value<DT>(((const raw*)a.z)[at]), a.c, -m)) * is;
+    const float q = __builtin_amdgcn_exp2f((ds_value<DT>(((const raw*)a.z)[at]) - m) * a.c) * is;
     ((raw*)a.dz)[at] = ds_raw<DT>((q - p) * g);
   }
 }
@@ -475,11 +475,17 @@ __device__ __forceinline__ ds_sum tl_rank(unsigned long long* list, float* left,
   return sum;
 }
 
+// log-sum-exp; of finite logits it stays finite (the type's lowest value over a temperature of 1)
+__device__ __forceinline__ float tl_rest(ds_sum sum, float c) {
+  const float r = (float)(((double)sum.m * (double)c + log2((double)sum.s)) * 0.69314718055994530942);
+  return fabsf(sum.m) < INFINITY ? fminf(fmaxf(r, -3.402823466e38f), 3.402823466e38f) : r;
+}
+
 template <int DT, int THREADS, bool WHOLE>
 __global__ __launch_bounds__(THREADS, 4) void top_logits_kernel(tl_args a) {
   constexpr int CH = ds_type<DT>::CH;
   // Small workgroups: half the list and at most 128 registers, so that four share a CU (1024 rows are then one round of the chip: 1024 x 100003
-  // bf16, 64 kept, 75 us; 90 us with the whole list and as many registers as the compiler likes).
+  // bf16, 64 kept, 78 us; 93 us with the whole list and as many registers as the compiler likes).
   constexpr int CAP = THREADS == TL_SMALL ? TL_CAP / 2 : TL_CAP;
   __shared__ __attribute__((aligned(16))) unsigned long long list[CAP + 2];
   __shared__ float left[CAP];
@@ -594,9 +600,9 @@ __global__ __launch_bounds__(THREADS, 4) void top_logits_kernel(tl_args a) {
   sum = tl_rank<THREADS>(list, left, n, K, a.c, sum, leave);
   if constexpr (!WHOLE)
     for (int i = K + threadIdx.x; i < a.K; i += THREADS) a.cand[(int64_t)blockIdx.x * a.K + i] = 0ull;
-  sum = ds_join<THREADS>(sum, redm, reds);
+  sum = ds_join<THREADS>(sum, a.c, redm, reds);
   if (threadIdx.x == 0) {
-    if constexpr (WHOLE) a.rest[row] = (sum.m + __builtin_amdgcn_logf(sum.s)) * 0.69314718055994530942f;
+    if constexpr (WHOLE) a.rest[row] = tl_rest(sum, a.c);
     else { a.part[2 * blockIdx.x] = sum.m; a.part[2 * blockIdx.x + 1] = sum.s; }
   }
 }
@@ -618,14 +624,14 @@ __global__ __launch_bounds__(TL_THREADS) void top_logits_join_kernel(tl_args a) 
   const int n = count;
   ds_sum sum;
   if (threadIdx.x == 0)
-    for (int i = 0; i < a.segs; ++i) sum.join(a.part[2 * (row * a.segs + i)], a.part[2 * (row * a.segs + i) + 1]);
+    for (int i = 0; i < a.segs; ++i) sum.join(a.part[2 * (row * a.segs + i)], a.part[2 * (row * a.segs + i) + 1], a.c);
   sum = tl_rank<TL_THREADS>(list, left, n, a.K, a.c, sum, [&](int rank, unsigned long long k) {
     const int cls = (int)~(unsigned)k;
     a.indices[row * a.K + rank] = cls;
     ((typename ds_type<DT>::raw*)a.values)[row * a.K + rank] = ((const typename ds_type<DT>::raw*)a.z)[row * a.V + cls];
   });
-  sum = ds_join<TL_THREADS>(sum, redm, reds);
-  if (threadIdx.x == 0) a.rest[row] = (sum.m + __builtin_amdgcn_logf(sum.s)) * 0.69314718055994530942f;
+  sum = ds_join<TL_THREADS>(sum, a.c, redm, reds);
+  if (threadIdx.x == 0) a.rest[row] = tl_rest(sum, a.c);
 }
 
 int ds_es(int dtype) { return dtype == DS_F32 ? 4 : 2; }
@@ -643,7 +649,7 @@ int tl_segments(int64_t R, int V, int K) {
   return (int)(s < 1 ? 1 : s);
 }
 int ds_check(const void* z, const void* values, const void* indices, int64_t R, int32_t V, int32_t K, float tau, int32_t dtype) {
-  if (!z || !values || !indices || R < 1 || V < 1 || K < 1 || dtype < 0 || dtype > 2 || !(tau > 0.f) || !(tau < 3.0e38f)) return OFB_EINVAL;
+  if (!z || !values || !indices || R < 1 || V < 1 || K < 1 || dtype < 0 || dtype > 2 || !(tau > 1e-37f) || !(tau < 3.0e38f)) return OFB_EINVAL;
   if (K > DS_KMAX || K > V || V > (1 << 30) || R >= (1 << 22)) return OFB_ELIMIT;      // (threads of a launch count in 32 bits)
   if (!ofb_aligned16(z)) return OFB_EINVAL;
   return OFB_OK;

@@ -1117,7 +1117,7 @@ def _rows_operand(t):
 def _check_logits(what, z, K, temperature):
     if not isinstance(z, torch.Tensor) or z.dim() != 2 or z.dtype not in hip.DTYPE_CODE:
         raise hip.OfbError(f'{what}: logits must be a (rows, classes) tensor of float32, bfloat16 or float16')
-    if not 0 < float(temperature) < 3e38:
+    if not 1e-37 < float(temperature) < 3e38:
         raise hip.OfbError(f'{what}: temperature must be positive and finite, got {temperature}')
     if not 1 <= K <= min(z.shape[1], 1024):
         raise hip.OfbError(f'{what}: {K} of {z.shape[1]} classes: 1 to 1024 can be stored, at most all')

@@ -1,6 +1,6 @@
 """Distillation from stored top logits by its definition in 64 bits on the CPU, with bounds for the kernels' arithmetic.
 
-Bounds.  An exponential is exp2 of one fma: its argument y log2 e - max is off by 2^-24 of itself (the scale's rounding, 2^-24 of y too) and the result by
+Bounds.  An exponential is exp2 of (y - max) times a rounded scale: its argument is off by 3 x 2^-24 of itself and the result by
 2^-23; with g the largest |y - max| (counted up to 100: beyond, it is 0 in f32) a probability is off by e = (4 g + 8) 2^-24 relative, and the sums over a thread's classes by n 2^-24
 with n = V / 256 + 32.  Twice that for a probability over its sum; the gradient is rounded once to its type (u, or half a subnormal step)."""
 import math

@@ -221,3 +221,51 @@ def test_as_many_rows_as_there_can_be():
     assert torch.equal(values, v[:, :2]) and torch.equal(indices.long(), i[:, :2]) and torch.allclose(rest, v[:, 2], rtol=0, atol=1e-5)
     loss, g = run(z.flip(0), values.flip(0), indices.flip(0), rest.flip(0), 1.0, torch.ones((), device='cuda'), 'sum')
     assert float(loss) <= R * 1e-6 and float(g.abs().max()) <= 1e-5
+
+
+@pytest.mark.parametrize('dtype', list(DT))
+@pytest.mark.parametrize('V', [300, 20001])
+def test_classes_masked_with_the_lowest_value(V, dtype):
+    """a padded vocabulary: the last classes and some others hold the type's lowest value, a stored one among them"""
+    R, K = 5, 12
+    z, values, idx, rest = make(6, R, V, K, DT[dtype])
+    low = torch.finfo(DT[dtype]).min
+    z[:, -V // 5:] = low
+    z[:, ::7] = low
+    z.scatter_(1, idx[:, 1:].long(), 1.5)
+    idx[:, 0] = 7
+    z[:, 7] = low
+    values[:, 0] = values.min() - 4                           # the teacher gives a masked class next to nothing
+    values[2:, 0] = -math.inf                                 # or nothing at all
+    up = torch.ones(R, device='cuda')
+    for r in (rest, None):
+        got = run(z[2:], values[2:], idx[2:], None if r is None else r[2:], 2.0, up[2:])
+        check(got, U.reference(z[2:], values[2:], idx[2:], None if r is None else r[2:], 2.0, up[2:]))
+        loss, g = run(z, values, idx, r, 2.0, up)
+        if dtype == 'f16':                                    # (f16's lowest value is a logit like any other)
+            check((loss, g), U.reference(z, values, idx, r, 2.0, up))
+        else:
+            assert bool((loss[:2] > 1e30).all()) and torch.isfinite(g).all()      # probability where the student has none: beyond any loss
+    t, i, left = ops.top_logits(z, K, 2.0)
+    v, j, w = U.top(z.cpu(), K, 2.0)
+    assert torch.equal(i.cpu(), j) and same(t.cpu(), v) and bool(((left.cpu().double() - w).abs() <= 1e-5 * (1 + w.abs())).all())
+
+
+@pytest.mark.parametrize('dtype', list(DT))
+@pytest.mark.parametrize('low', ['lowest', -1e4])
+def test_rows_of_one_value(low, dtype):
+    """every logit the type's lowest value, or another one, student and teacher: even rows"""
+    R, V, K = 3, 5003, 10
+    low = torch.finfo(DT[dtype]).min if low == 'lowest' else low
+    z = torch.full((R, V), low, dtype=DT[dtype], device='cuda')
+    for tau in (1.0, 2.0, 3.0):
+        t, i, left = ops.top_logits(z, K, tau)
+        assert torch.equal(i.cpu(), torch.arange(K, dtype=torch.int32).expand(R, K)) and bool((t == z[:, :K]).all()) and torch.isfinite(left).all()
+        even = torch.full((R,), math.log(V - K), device='cuda')
+        loss, g = run(z, torch.zeros_like(t), i, even, tau, torch.ones(R, device='cuda'))      # a teacher that is even
+        assert float(loss.abs().max()) <= 1e-5 * tau * tau and float(g.abs().max()) <= 1e-6
+        loss, g = run(z, t, i, None, tau, torch.ones(R, device='cuda'))                        # and one that is even over the ten alone
+        want = torch.full((R, V), 1 / V, dtype=torch.float64)
+        want[:, :K] -= 1 / K
+        assert float((loss.double().cpu() - tau * tau * math.log(V / K)).abs().max()) <= 1e-5 * tau * tau
+        assert bool(((g.double().cpu() - tau * want).abs() <= (torch.finfo(DT[dtype]).eps + 1e-5) * tau * want.abs() + 2.0 ** -24).all())
