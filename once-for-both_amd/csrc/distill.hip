@@ -24,7 +24,7 @@
 #define DS_STATS 8                /* floats kept per row: m_t, kappa, m, 1/s, m_teacher, 1/s_teacher, used, 0 */
 #define TL_CAP 4096               /* candidates of a row or segment that are ranked at once */
 #define TL_THREADS 1024
-#define TL_SMALL 256              /* threads for lists of up to TL_SMALL / 2: 1024 x 100003 bf16, 64 kept: 78 us, 1024 threads 102 us */
+#define TL_SMALL 256              /* threads for lists of up to TL_SMALL / 2 (1024 x 100003 bf16, 64 kept: 90 us, 1024 threads 99 us, all else alike) */
 
 namespace {
 
@@ -485,7 +485,7 @@ template <int DT, int THREADS, bool WHOLE>
 __global__ __launch_bounds__(THREADS, 4) void top_logits_kernel(tl_args a) {
   constexpr int CH = ds_type<DT>::CH;
   // Small workgroups: half the list and at most 128 registers, so that four share a CU (1024 rows are then one round of the chip: 1024 x 100003
-  // bf16, 64 kept, 78 us; 93 us with the whole list and as many registers as the compiler likes).
+  // bf16, 64 kept: 90 us with the whole list and as many registers as the compiler likes, 75 us so; 78 us with today's exponentials).
   constexpr int CAP = THREADS == TL_SMALL ? TL_CAP / 2 : TL_CAP;
   __shared__ __attribute__((aligned(16))) unsigned long long list[CAP + 2];
   __shared__ float left[CAP];
