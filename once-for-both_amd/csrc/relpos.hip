@@ -857,8 +857,9 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && (DT == RP_F32 || FEW) ? 1 :
     if (most > 0.f) frexpf(most, &ex);
     unit = 62 - max(ex, -60) - (7 + 32 - __clz(a.Nk));
     const float mul = __builtin_ldexpf(linv, unit - 32), nd = nD - __builtin_ldexpf(left, e.ed + e.ev - e.es);
+    // (to the end of the last wave's 32 rows, as in the waves' own tests: what a wave has not summed as a whole must be visited)
     auto next = [&](int kb) {
-      while (kb < kb1 && is_whole(kb * KB, KB, qt * RP_TILE) && beyond(kb * KB, KB, qt * RP_TILE, q_last)) ++kb;
+      while (kb < kb1 && is_whole(kb * KB, KB, qt * RP_TILE) && beyond(kb * KB, KB, qt * RP_TILE, q_last | 31)) ++kb;
       return kb;
     };
     int kb = bad ? kb1 : next(0), buf = 0;
