@@ -30,6 +30,10 @@
 #define RP_PE 14                 /* f32's planes, and the backward's f16, hold P 2^14 */
 #define RP_ESMAX 100             /* dS is scaled by 2^-100 .. 2^60 */
 #define RP_NBOUND 256            /* partial maxima of a tensor */
+// A weight is exp2 of the ROUNDED score minus the row's maximum, which is a rounded score: 1 at most, and the same in every kernel.  Tiles of one bias leave
+// the rounding out (one fma: the product plus bias - maximum) only where maximum and bias are at most this, in log2 units: scores are then known to 2^-14,
+// and so is what the two forms differ by.  Beyond, a weight could be exp2 of half the last place of 1e9.
+#define RP_PLAIN 1024.f
 // Keys up to which a workgroup of the f32 forward reads its head's K and V once more for their maxima; a pass of its own over both otherwise.  Both, heads
 // of 64: 128 x 197 keys, 6 heads 68 and 73 us; 32 x 256, 6 heads 26 and 31; 16 x 512, 12 heads 65.5 and 67.5; 8 x 768 75.7 and 76.6; 8 x 1024 111 and 108.
 #define RP_OWN 512
@@ -422,8 +426,9 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 3 : DT == RP_F32 ? 1 : 2)) 
       const int dmax = j0 + KB - 1 - q0 - a.q_offset, dmin = j0 - (q0 + 31) - a.q_offset;
       float bt = 0.f, c_t = 1.f;
       const float wc = rp_uniform(w[RP_PAD + (dmax <= lo ? 0 : width - 1)]);
-      // (a bias that swallows the scores, and a scale that is not positive, take the general form)
-      if (!POS && (dmax <= lo || dmin >= hi) && fabsf(wc) < 1e30f && c_s > 0.f) {
+      // (a large bias, and a scale that is not positive, take the general form)
+      const bool one_bias = !POS && (dmax <= lo || dmin >= hi) && fabsf(wc) <= RP_PLAIN && c_s > 0.f;
+      if (one_bias) {
         bt = wc;
         c_t = c_s;
       } else if constexpr (POS) {
@@ -463,6 +468,14 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 3 : DT == RP_F32 ? 1 : 2)) 
         for (int r = 0; r < 16; ++r) mb = fmaxf(mb, S[t][r]);
       OFB_XOR_STEP(mb, fmaxf, 32)
       const float m_new = fmaxf(m, fmaf(mb, c_t, bt));
+      if (one_bias && __any(fabsf(m_new) > RP_PLAIN)) {        // large scores: rounded, as in the general form
+#pragma unroll
+        for (int t = 0; t < KB / 32; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) S[t][r] = fmaf(S[t][r], c_t, bt);
+        c_t = 1.f;
+        bt = 0.f;
+      }
       if (__any(m_new > m)) {                                  // the running maximum moves rarely after the first tiles
         const float alpha = m_new > -INFINITY ? __builtin_amdgcn_exp2f(m - m_new) : 1.f;
         l *= alpha;
