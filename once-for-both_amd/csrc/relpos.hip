@@ -707,7 +707,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && (DT == RP_F32 || FEW) ? 1 :
     if (POS && threadIdx.x < KB) pk[buf * KB + threadIdx.x] = pk_next;
   };
   if (kb1 > 0) commit(0);
-  __syncthreads();
+  const bool plain = !__syncthreads_or(qok && fabsf(m) > RP_PLAIN);        // (of the workgroup: its waves share the second visit's tiles)
   const int lo = a.lo, width = a.width, hi = lo + width - 1, w_first = rp_lds_base(w), w_last = w_first + 4 * (width - 1), pq4 = 4 * (pq + lo) - w_first;
   // S and dP - D (in dP's scale) of 32 keys
   auto products = [&](const char* kt_, const char* vt_, int t0, float nd, f32x16& S, f32x16& dP) {
@@ -768,9 +768,9 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && (DT == RP_F32 || FEW) ? 1 :
   auto visible = [&](int j0) { return active && j0 < kend && !(a.causal && j0 > q0 + 31 + a.q_offset); };
   auto is_whole = [&](int j0, int n, int first) { return j0 + n <= kend && (!a.causal || j0 + n - 1 <= first + a.q_offset); };
   // the whole tile of keys j0 .. j0 + n - 1 and queries first .. last lies beyond an end: -1, 1 or 0
-  // (a bias that swallows the scores takes the general form, as in the forward)
+  // (large biases and scores take the general form, as in the forward)
   const float w_lo = rp_uniform(w[RP_PAD]), w_hi = rp_uniform(w[RP_PAD + width - 1]);
-  const int below = fabsf(w_lo) < 1e30f ? lo + a.q_offset : -0x7fffffff, above = fabsf(w_hi) < 1e30f ? hi + a.q_offset : 0x7fffffff;
+  const int below = plain && fabsf(w_lo) <= RP_PLAIN ? lo + a.q_offset : -0x7fffffff, above = plain && fabsf(w_hi) <= RP_PLAIN ? hi + a.q_offset : 0x7fffffff;
   auto beyond = [&](int j0, int n, int first, int last) { return POS ? 0 : j0 + n - 1 - first <= below ? -1 : j0 - last >= above ? 1 : 0; };
   float most = 0.f;                                            // the largest |ds| that goes to a bin
   for (int kb = 0; kb < kb1; ++kb) {

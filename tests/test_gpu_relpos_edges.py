@@ -87,3 +87,84 @@ def test_large_scores(size, dtype):
             err = (out.cpu().double().transpose(1, 2) - want).abs()[clear]
             assert torch.isfinite(out).all()
             assert bool((err <= 2 * rounding(q) * want.abs()[clear] + 2.0 ** -38 * float(v.abs().max())).all()), float(err.max())
+
+
+def consistent(q, k, v, dout, scale, got):
+    """What holds for any weights P whose rows sum to 1, if forward and backward use the same ones: |dv| <= sum of |dout|; sum v dv = sum dout out (both are
+    sum P dout v); sum q dq = sum k dk (both are scale sum dS q k); the table's gradients sum to nothing (as a row of dS does).
+
+    Tolerances: P, dS, D (bf16, f16: of an output whose P was rounded) and the results are off by u of the sums of their absolute terms each, and n terms in f32 by n 2^-24; the rows of P sum
+    to 1, so a head's sums of |P dout v| and |dS q k| are at most Nq d max|dout| max|v| and Nq (2 d max|dout| max|v|) d max|q| max|k| scale.  Two sides: twice that."""
+    B, Nq, H, d = q.shape
+    off = 4 * rounding(q) + (k.shape[1] + Nq + d + 64) * 2.0 ** -24
+    x = {n: t.detach().cpu().double().transpose(1, 2) for n, t in (('q', q), ('k', k), ('v', v), ('do', dout), *((m, got[m]) for m in ('out', 'dq', 'dk', 'dv')))}
+    big = {n: float(t.abs().amax()) for n, t in x.items()}
+    assert all(bool(torch.isfinite(t).all()) for t in got.values())
+    assert big['dv'] <= Nq * big['do'] * (1 + off)
+    apart = (x['v'] * x['dv']).sum((2, 3)) - (x['do'] * x['out']).sum((2, 3))
+    assert float(apart.abs().max()) <= 2 * off * Nq * d * big['v'] * big['do'], apart
+    top = 2 * d * big['do'] * big['v']
+    apart = (x['q'] * x['dq']).sum((2, 3)) - (x['k'] * x['dk']).sum((2, 3))
+    assert float(apart.abs().max()) <= 2 * off * Nq * top * scale * d * big['q'] * big['k'], apart
+    assert float(got['dtable'].double().sum(0).abs().max()) <= B * off * Nq * top
+
+
+def check_with_floors(q, k, v, dout, got, want):
+    """... and what is small in absolute terms: f32 holds P to 2^-39 (half a subnormal step of f16 over the 2^14 of its scale) in dv; a pair is rounded down to a bin's unit, 2^-(55 - bits of Nk) of a
+    power of two up to twice the largest |dS| <= 2 d max|dout| max|v|"""
+    B, Nq, H, d = q.shape
+    Nk = k.shape[1]
+    U.check({n: x for n, x in got.items() if n != 'dtable'}, want, tiny=Nq * 2.0 ** -39 * float(dout.abs().max()))
+    unit = 2.0 ** (2 - 55 + Nk.bit_length()) * 2 * d * float(dout.abs().max()) * float(v.abs().max())
+    U.check({'dtable': got['dtable']}, want, tiny=B * Nq * Nk * unit)
+
+
+@pytest.mark.parametrize('dtype', list(DT))
+@pytest.mark.parametrize('size', [1.0, 6.0])
+@pytest.mark.parametrize('bias', BIASES)
+def test_gradients_of_finite_mask_biases(bias, size, dtype):
+    """element by element where every row's maximum lies beside the mask, or the bias leaves its score 32-bit digits: the bounds count a score's rounding, 2^-24 of it, to first order, which is no
+    bound from 2^24 on.  The identities hold everywhere."""
+    for plan, masked in windows():
+        for Nq, Nk, d in ((70, 300, 64), (1, 700, 64), (70, 300, 128), (33, 200, 16)):
+            q, k, v, table, dout = make(Nq + int(size), 2, Nq, Nk, 2, d, DT[dtype], plan)
+            q *= size
+            table[masked] = bias
+            for off in (0, Nk // 2, Nk - Nq, 2000, -2000):
+                kw = dict(q_offset=off, causal=off == Nk // 2)
+                got = step(q, k, v, table, plan, dout, **kw)
+                consistent(q, k, v, dout, d ** -0.5, got)
+                sees = torch.ones(Nq, Nk, dtype=torch.bool) if not kw['causal'] else torch.arange(Nk) <= torch.arange(Nq)[:, None] + off
+                of_mask = sees & (U.bucket_matrix(plan, Nq, Nk, off) == masked % plan.num_buckets)
+                blurred = of_mask.any(1) if bias > 0 else of_mask.any(1) & ~(sees & ~of_mask).any(1)
+                if abs(bias) < 1e6 or not bool(blurred.any()):
+                    check_with_floors(q, k, v, dout, got, U.reference(q, k, v, table, plan, dout=dout, **kw))
+
+
+def check_one_key(q, k, v, dout, best, clear, got, scale=0.125):
+    """each row has one key: P is 1 there and 0 elsewhere, so dv is the sum of those rows' dout (u for the result, 2^-24 a term); the scores' rounding must not show.  (Rows
+    whose best key is not clear add their dout to some keys: those are left out.)"""
+    consistent(q, k, v, dout, scale, got)
+    do, dv = dout.cpu().double().transpose(1, 2), got['dv'].cpu().double().transpose(1, 2)
+    Nk = k.shape[1]
+    hit = torch.zeros(*best.shape[:2], Nk, dtype=torch.bool)
+    want = torch.zeros_like(dv)
+    for b in range(best.shape[0]):
+        for h in range(best.shape[1]):
+            want[b, h].index_add_(0, best[b, h], do[b, h])
+            hit[b, h, best[b, h][clear[b, h]]] = True
+            hit[b, h, best[b, h][~clear[b, h]]] = False
+    err = (dv - want).abs()[hit]
+    tol = 2 * rounding(q) * want.abs()[hit] + best.shape[2] * (rounding(q) + 2.0 ** -24) * float(do.abs().max()) * (~clear).any() + 8 * 2.0 ** -24 * float(do.abs().max())
+    assert bool((err <= tol).all()), float(err.max())
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'f16'])
+@pytest.mark.parametrize('size', [300.0, 3000.0, 1e4])
+def test_gradients_of_large_scores(size, dtype):
+    for name in ('clip0', 'log8', 'step'):
+        plan = PLANS[name]()
+        for Nq, Nk, off, causal in LARGE:
+            (q, k, v, table, dout), best, clear = one_key_each(dtype, Nq, Nk, size, plan, off, causal)
+            got = step(q, k, v, table, plan, dout, q_offset=off, causal=causal)
+            check_one_key(q, k, v, dout, best, clear, got)
