@@ -73,11 +73,12 @@ __device__ __forceinline__ f32x16 rp_mm1(rp_frag a, rp_frag b, f32x16 c) {
   if constexpr (DT == RP_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(rp_bf16x8, a), __builtin_bit_cast(rp_bf16x8, b), c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(ofb_f16x8, a), __builtin_bit_cast(ofb_f16x8, b), c, 0, 0, 0);
 }
-template <int DT, int NP>
+// SWAPPED: the terms in the order of the product whose A and B are this one's B and A, whose sums are then the same to the last bit
+template <int DT, int NP, bool SWAPPED = false>
 __device__ __forceinline__ f32x16 rp_mm(const rp_frag (&a)[NP], const rp_frag (&b)[NP], f32x16 c) {
   if constexpr (NP == 2) {                                   // smallest terms first; the dropped one is below 2^-22 of the product
-    c = rp_mm1<DT>(a[1], b[0], c);
-    c = rp_mm1<DT>(a[0], b[1], c);
+    c = rp_mm1<DT>(a[!SWAPPED], b[SWAPPED], c);
+    c = rp_mm1<DT>(a[SWAPPED], b[!SWAPPED], c);
   }
   return rp_mm1<DT>(a[0], b[0], c);
 }
@@ -949,8 +950,8 @@ __device__ __forceinline__ void rp_tile_ds(const ofb_relpos_args& a, const char*
     rp_frag qa[NP], da[NP];
     rp_rows<DT, DP, KB>(qt_, tr, s, lane, qa);
     rp_rows<DT, DP, KB>(dt_, tr, s, lane, da);
-    S = rp_mm<DT, NP>(qa, kf[s], S);
-    dP = rp_mm<DT, NP>(da, vf[s], dP);
+    S = rp_mm<DT, NP, true>(qa, kf[s], S);                      // the forward's S: its weights are 1 at most whatever the scores' size is
+    dP = rp_mm<DT, NP, true>(da, vf[s], dP);
   }
   const int dmax = j0 + 31 - i0 - a.q_offset, dmin = j0 - (i0 + 31) - a.q_offset;
   const bool cut = a.causal && j0 + 31 > i0 + a.q_offset;

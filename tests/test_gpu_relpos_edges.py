@@ -159,7 +159,7 @@ def check_one_key(q, k, v, dout, best, clear, got, scale=0.125):
     assert bool((err <= tol).all()), float(err.max())
 
 
-@pytest.mark.parametrize('dtype', ['bf16', 'f16'])
+@pytest.mark.parametrize('dtype', list(DT))
 @pytest.mark.parametrize('size', [300.0, 3000.0, 1e4])
 def test_gradients_of_large_scores(size, dtype):
     for name in ('clip0', 'log8', 'step'):
