@@ -12,7 +12,8 @@
 // three products (hformat.h), with exponents from the maxima of the tile (Q, dO, dS) or of the head (K, V; of all heads where a pass of its own
 // finds them).  Scores, softmax statistics, dS and all sums are f32 (the table's gradient sums in 64 bits); P and dS are rounded to the operand
 // type for the second product: bf16 as they are, f16 with dS times a power of two that keeps it below 2^15 (and P times 2^14 for dV), f32 likewise
-// in two f16 planes.  (Exponents of f32 operands end at 2^60: a tensor whose maximum is below 2^-45 is held to 2^-85.)
+// in two f16 planes.  (f32 operands of any size: exponents run from 2^-113, for f32's largest value, to 2^112, where a tensor whose maximum is below 2^-97 is
+// held to 2^-137.  What has to fit f32 is what f32 arithmetic forms too: scores, dP and dS.)
 //
 // Operand conventions (lane l, hh = l >> 5): A[row = l & 31][k = 8 hh + j], B[k = 8 hh + j][col = l & 31], accumulator register r holds
 // row 8 (r >> 2) + 4 hh + (r & 3) of column l & 31.  A reduction may run over its index in any order that both operands share, so an
@@ -28,7 +29,9 @@
 #define RP_PAD 4                 /* entries of w on either side, so that four consecutive differences need one clamp */
 #define RP_WMAX 4096
 #define RP_PE 14                 /* f32's planes, and the backward's f16, hold P 2^14 */
-#define RP_ESMAX 100             /* dS is scaled by 2^-100 .. 2^60 */
+#define RP_EMIN -113             /* exponents of the planes: f32's largest value times 2^-113 is below 2^15 */
+#define RP_EMAX 112              /* ... and 2^-(112 + RP_PE) is still a normal number */
+#define RP_ESMAX 126             /* dS is scaled by 2^RP_EMIN .. 2^126 */
 #define RP_NBOUND 256            /* partial maxima of a tensor */
 // A weight is exp2 of the ROUNDED score minus the row's maximum, which is a rounded score: 1 at most, and the same in every kernel.  Tiles of one bias leave
 // the rounding out (one fma: the product plus bias - maximum) only where maximum and bias are at most this, in log2 units: scores are then known to 2^-14,
@@ -198,6 +201,14 @@ __device__ __forceinline__ void rp_cols(const char* lds, int row0, int ct, int l
 }
 
 struct rp_scales { int eq, ek, ev, ed, es; };
+
+// exponent of the planes of a tensor whose maximum is b: b 2^e in [2^14, 2^15), as far as the exponents go
+__device__ __forceinline__ int rp_exp(float b) {
+  if (!(b > 0.f) || !(b < INFINITY)) return 0;
+  int ex;
+  frexpf(b, &ex);
+  return min(15 - ex, RP_EMAX);
+}
 
 // The workgroup's tile and head.  Neighbouring tiles of a head share an L2 (its keys or queries are streamed by all of them); causal tiles differ in
 // length, so there the longest of all heads come first, and a head stays on one XCD where the number of heads is a multiple of eight.
@@ -378,15 +389,14 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 3 : DT == RP_F32 ? 1 : 2)) 
       a.bound_k[bh] = top[1];
       a.bound_v[bh] = top[2];
     }
-    const int eq = ofb_h_exp(top[0]), ek = ofb_h_exp(top[1]), ev = ofb_h_exp(top[2]);
+    const int eq = rp_exp(top[0]), ek = rp_exp(top[1]), ev = rp_exp(top[2]);
     hq = ofb_h_pow2(eq); hk = ofb_h_pow2(ek); hv = ofb_h_pow2(ev);
-    c_s = c_s * ofb_h_pow2(-eq) * ofb_h_pow2(-ek);
-    c_o = ofb_h_pow2(-ev);
+    c_s = __builtin_ldexpf(c_s, -eq - ek);
+    c_o = ofb_h_pow2(-ev - RP_PE);                             // P's scale is in it too
   }
   // f32: P's planes hold it times 2^14.  (Not by way of the exponent, where a maximum like -1e9 would swallow it; f16 needs no scale here: P is at
   // most 1 and its row's sum at least 1, what falls below the subnormal step 2^-24 is nothing beside f16's own 2^-11.)
   const float p_sc = DT == RP_F32 ? ofb_h_pow2(RP_PE) : 1.f;
-  if constexpr (DT == RP_F32) c_o *= ofb_h_pow2(-RP_PE);
 
   const int pq = POS ? (qok ? a.pos_q[qi] : 0) : qi + a.q_offset;
   rp_frag qf[DP / 16][NP];
@@ -512,7 +522,8 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 3 : DT == RP_F32 ? 1 : 2)) 
   }
   OFB_XOR_STEP(l, ofb_add_, 32)
   if (!qok) return;
-  if constexpr (SPLIT) {                                       // partial sums in units of exp2(m), joined by relpos_join_kernel
+  const float linv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);             // (a NaN stays one)
+  if constexpr (SPLIT) {                                       // the range's own result, joined by relpos_join_kernel
     const int64_t row = ((int64_t)blockIdx.y * a.B * a.H + bh) * a.Nq + qi;
     if (hh == 0) { a.split_ml[2 * row] = m; a.split_ml[2 * row + 1] = l; }
 #pragma unroll
@@ -520,16 +531,14 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 3 : DT == RP_F32 ? 1 : 2)) 
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
         const int ch = 32 * ct + rp_row(r, hh);
-        if (ch < a.d) *reinterpret_cast<f32x4*>(a.split_o + row * a.d + ch) = f32x4{O[ct][r] * c_o, O[ct][r + 1] * c_o, O[ct][r + 2] * c_o, O[ct][r + 3] * c_o};
+        if (ch < a.d) *reinterpret_cast<f32x4*>(a.split_o + row * a.d + ch) = f32x4{O[ct][r] * linv * c_o, O[ct][r + 1] * linv * c_o, O[ct][r + 2] * linv * c_o, O[ct][r + 3] * linv * c_o};
       }
   } else {
-    const float linv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);           // (a NaN stays one)
     if (a.stats && hh == 0) {
       float* st = a.stats + 2 * ((int64_t)bh * a.Nq + qi);
       st[0] = m > -INFINITY ? m : 0.f;
       st[1] = linv;
     }
-    const float f = linv * c_o;
     char* op = (char*)a.out + (b * a.o_sb + qi * a.o_st + head * a.o_sh) * ES;
     float* o32 = a.out32 ? a.out32 + (((int64_t)b * a.Nq + qi) * a.H + head) * a.d : nullptr;
 #pragma unroll
@@ -538,7 +547,7 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 3 : DT == RP_F32 ? 1 : 2)) 
       for (int r = 0; r < 16; r += 4) {
         const int ch = 32 * ct + rp_row(r, hh);
         if (ch < a.d) {
-          const float x0 = O[ct][r] * f, x1 = O[ct][r + 1] * f, x2 = O[ct][r + 2] * f, x3 = O[ct][r + 3] * f;
+          const float x0 = O[ct][r] * linv * c_o, x1 = O[ct][r + 1] * linv * c_o, x2 = O[ct][r + 2] * linv * c_o, x3 = O[ct][r + 3] * linv * c_o;
           rp_store4<DT>(op + ch * ES, x0, x1, x2, x3);
           if (o32) *reinterpret_cast<f32x4*>(o32 + ch) = f32x4{x0, x1, x2, x3};
         }
@@ -565,9 +574,10 @@ __global__ __launch_bounds__(RP_THREADS) void relpos_join_kernel(ofb_relpos_args
   if (a.stats && lane == 0) { a.stats[2 * row] = mu; a.stats[2 * row + 1] = linv; }
   for (int ch = lane * 4; ch < a.d; ch += 256) {
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < splits; ++s)
-      o += *reinterpret_cast<const f32x4*>(a.split_o + (s * rows + row) * a.d + ch) * __builtin_amdgcn_exp2f(a.split_ml[2 * (s * rows + row)] - mu);
-    o *= linv;
+    for (int s = 0; s < splits; ++s) {
+      const float part = a.split_ml[2 * (s * rows + row) + 1] * __builtin_amdgcn_exp2f(a.split_ml[2 * (s * rows + row)] - mu) * linv;      // the range's share of the row
+      o += *reinterpret_cast<const f32x4*>(a.split_o + (s * rows + row) * a.d + ch) * part;
+    }
     rp_store4<DT>((char*)a.out + (b * a.o_sb + qi * a.o_st + head * a.o_sh + ch) * ES, o[0], o[1], o[2], o[3]);
     if (a.out32) *reinterpret_cast<f32x4*>(a.out32 + ((b * a.Nq + qi) * a.H + head) * a.d + ch) = o;
   }
@@ -583,10 +593,10 @@ __device__ __forceinline__ rp_scales rp_all_scales(float (&top)[4], int d, float
   if constexpr (DT != RP_BF16) {
     rp_tops(top, red);
     if constexpr (DT == RP_F32) {
-      e.eq = ofb_h_exp(top[0]);
-      e.ek = ofb_h_exp(top[1]);
-      e.ev = ofb_h_exp(top[2]);
-      e.ed = ofb_h_exp(top[3]);
+      e.eq = rp_exp(top[0]);
+      e.ek = rp_exp(top[1]);
+      e.ev = rp_exp(top[2]);
+      e.ed = rp_exp(top[3]);
     }
     // |dS| <= P (|dP| + |D|) <= 2 d max|dO| max|V| = m 2^ex, m in [0.5, 1): m 2^15 in its scale, as long as that is a power of two that f32 has room for
     // (the factors' exponents apart: their product may leave f32)
@@ -595,7 +605,7 @@ __device__ __forceinline__ rp_scales rp_all_scales(float (&top)[4], int d, float
     if (m > 0.f) {
       int ex;
       frexpf(m, &ex);
-      e.es = max(-RP_ESMAX, min(OFB_H_EMAX, 15 - ex - ev - ed - ec));
+      e.es = max(RP_EMIN, min(RP_ESMAX, 15 - ex - ev - ed - ec));
     }
   }
   return e;
@@ -680,9 +690,8 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && (DT == RP_F32 || FEW) ? 1 :
     a.bound_do[(int64_t)bh * nqt + qt] = top[3];
   }
   const float hq = ofb_h_pow2(e.eq), hk = ofb_h_pow2(e.ek), hv = ofb_h_pow2(e.ev), hd = ofb_h_pow2(e.ed);
-  const float c_s = a.scale * 1.44269504088896340736f * ofb_h_pow2(-e.eq) * ofb_h_pow2(-e.ek);
+  const float c_s = __builtin_ldexpf(a.scale * 1.44269504088896340736f, -e.eq - e.ek);
   const int ek_ = e.es - e.ed - e.ev;                          // dP's accumulators times 2^ek_ are in dS's scale
-  const float c_dq = a.scale * ofb_h_pow2(-e.es) * ofb_h_pow2(-e.ek);
   rp_frag qf[DP / 16][NP], df[DP / 16][NP];
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
@@ -830,7 +839,8 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && (DT == RP_F32 || FEW) ? 1 :
     if (kb + 1 < kb1) commit(buf ^ 1);
     __syncthreads();
   }
-  const float c_out = c_dq * linv;
+  const float c_dq = a.scale * linv;
+  const int e_dq = -e.es - e.ek;                               // (apart from the factor: the two together may leave f32)
   if (qok) {
     char* op = (char*)a.dq + (b * a.dq_sb + qi * a.dq_st + head * a.dq_sh) * ES;
 #pragma unroll
@@ -838,7 +848,8 @@ __global__ __launch_bounds__(RP_THREADS, (DP > 64 && (DT == RP_F32 || FEW) ? 1 :
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
         const int ch = 32 * ct + rp_row(r, hh);
-        if (ch < a.d) rp_store4<DT>(op + ch * ES, dQ[ct][r] * c_out, dQ[ct][r + 1] * c_out, dQ[ct][r + 2] * c_out, dQ[ct][r + 3] * c_out);
+        if (ch < a.d) rp_store4<DT>(op + ch * ES, __builtin_ldexpf(dQ[ct][r] * c_dq, e_dq), __builtin_ldexpf(dQ[ct][r + 1] * c_dq, e_dq),
+                                    __builtin_ldexpf(dQ[ct][r + 2] * c_dq, e_dq), __builtin_ldexpf(dQ[ct][r + 3] * c_dq, e_dq));
       }
   }
   // D came from an output whose P was rounded for the product.  A row of dS sums to zero, so what this row's sum is off by is D's error: the
@@ -1043,10 +1054,10 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 2 : 1)) void relpos_dkv_ker
   rp_bias_vector(a, head, w);
   if (qb0 < qb1) fetch(qb0);
   const float hq = ofb_h_pow2(e.eq), hk = ofb_h_pow2(e.ek), hv = ofb_h_pow2(e.ev), hd = ofb_h_pow2(e.ed);
-  const float c_s = a.scale * 1.44269504088896340736f * ofb_h_pow2(-e.eq) * ofb_h_pow2(-e.ek);
+  const float c_s = __builtin_ldexpf(a.scale * 1.44269504088896340736f, -e.eq - e.ek);
   const float c_x = DT == RP_BF16 ? 1.f : ofb_h_pow2(e.es - e.ed - e.ev - RP_PE);      // dS from rp_tile_ds to the operand's scale
-  const float c_dk = a.scale * ofb_h_pow2(-e.es) * ofb_h_pow2(-e.eq);
-  const float c_dv = DT == RP_BF16 ? 1.f : ofb_h_pow2(-RP_PE) * ofb_h_pow2(-e.ed);
+  const int e_dk = -e.es - e.eq;
+  const float c_dv = DT == RP_BF16 ? 1.f : ofb_h_pow2(-RP_PE - e.ed);
 
   const int j0 = j_first + wv * 32, kj = j0 + (lane & 31);
   const bool active = j0 < kend, kok = kj < kend;
@@ -1118,7 +1129,8 @@ __global__ __launch_bounds__(RP_THREADS, (DP <= 64 ? 2 : 1)) void relpos_dkv_ker
     for (int r = 0; r < 16; r += 4) {
       const int ch = 32 * ct + rp_row(r, hh);
       if (ch < a.d) {
-        rp_store4<DT>(okp + ch * ES, dK[ct][r] * c_dk, dK[ct][r + 1] * c_dk, dK[ct][r + 2] * c_dk, dK[ct][r + 3] * c_dk);
+        rp_store4<DT>(okp + ch * ES, __builtin_ldexpf(dK[ct][r] * a.scale, e_dk), __builtin_ldexpf(dK[ct][r + 1] * a.scale, e_dk),
+                      __builtin_ldexpf(dK[ct][r + 2] * a.scale, e_dk), __builtin_ldexpf(dK[ct][r + 3] * a.scale, e_dk));
         rp_store4<DT>(ovp + ch * ES, dV[ct][r] * c_dv, dV[ct][r + 1] * c_dv, dV[ct][r + 2] * c_dv, dV[ct][r + 3] * c_dv);
       }
     }

@@ -1068,7 +1068,10 @@ def relpos_attention(q, k, v, table, buckets, scale=None, causal=False, key_lens
     causal: a query sees the keys at or before its position; keys behind the last query's are not read.  key_lens (B,) int32: keys from there on are padding - they are not read, and
     their gradients are zero; a length beyond Nk counts as Nk, one below 0 as 0.  A query that sees no key has output and gradients 0.
     Returns (B, Nq, H, d) of q's type.  Differentiable once, in q, k, v and the table; the same inputs give the same bits.  A NaN or infinity makes the rows,
-    and the gradients, that meet it NaN, and the table's gradient of its head."""
+    and the gradients, that meet it NaN, and the table's gradient of its head.
+    float32 tensors may have any finite size as long as scores and dout v^T fit float32.  Their values enter the products with 22 bits, and not finer than 2^-39 of the largest |k| and
+    |v| of the head that a query sees and of the largest |q| and |dout| of a head: one huge key or value lowers what the rows that do not meet it keep.  bfloat16 and float16: the
+    weights and the scores' gradients are rounded to the type once, as operands of the products that follow."""
     call = _RelposCall(q, k, v, table, buckets, scale, causal, key_lens, q_offset)
     if key_lens is not None:
         key_lens = _c(key_lens)

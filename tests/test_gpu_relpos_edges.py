@@ -168,3 +168,37 @@ def test_gradients_of_large_scores(size, dtype):
             (q, k, v, table, dout), best, clear = one_key_each(dtype, Nq, Nk, size, plan, off, causal)
             got = step(q, k, v, table, plan, dout, q_offset=off, causal=causal)
             check_one_key(q, k, v, dout, best, clear, got)
+
+
+# sizes of q, k, v, dout; what f32 arithmetic forms (scores, dP, dS) fits f32 in all of them
+WIDE = [(1.0, 1.0, 1e25, 1.0), (1.0, 1.0, 1.0, 1e25), (1e25, 1e-25, 1.0, 1.0), (1e-30, 1e30, 1e10, 1e-10), (1.0, 1.0, 5e36, 1e-36), (1.0, 1.0, 1e-36, 5e36), (1e-4, 1e4, 7e22, 1.0),
+        (1.0, 1.0, 1e23, 1e-20), (1.0, 1.0, 1e-30, 1.0), (1.0, 1.0, 1.0, 1e-30), (1.0, 1.0, 1e-22, 1e-8), (1e-30, 1e30, 1.0, 1e-28), (1e-28, 1.0, 1.0, 1.0), (1.0, 1e-28, 1.0, 1.0), (1e-20, 1e-20, 1e20, 1e10)]
+
+
+@pytest.mark.parametrize('sizes', WIDE, ids=lambda s: '-'.join(f'{x:g}' for x in s))
+def test_float32_of_any_size(sizes):
+    """the bounds of ordinary sizes, relative to the tensors' maxima.  (In absolute terms: planes whose exponent ends at 2^112 hold their tensor to 2^-137, of which 600 products with
+    factors up to 5 are below 1e-38.)"""
+    plan = PLANS['clip']()
+    for Nq, Nk in ((70, 70), (1, 1500), (200, 600)):
+        q, k, v, table, dout = make(33, 1, Nq, Nk, 1, 64, torch.float32, plan)
+        q, k, v, dout = (x * s for x, s in zip((q, k, v, dout), sizes))
+        got = step(q, k, v, table, plan, dout)
+        U.check(got, U.reference(q, k, v, table, plan, dout=dout), tiny=1e-38)
+        assert bool(got['out'].any()) and bool(got['dv'].any())
+
+
+@pytest.mark.parametrize('largest', [3e38, torch.finfo(torch.float32).max])
+def test_the_largest_float32(largest):
+    """one value at the end of f32, alone in its column and met by some rows; then all values there, whose mean is (in one range of keys and joined from several).  The rows that do not meet it are held to
+    2^-39 of it, like all of a head."""
+    plan = PLANS['clip']()
+    for Nq, Nk, off, causal in ((70, 70, 0, True), (1, 1500, 1499, False), (150, 600, 450, True)):
+        q, k, v, table, dout = make(34, 1, Nq, Nk, 1, 64, torch.float32, plan)
+        v[:, -3], v[:, -3, :, 2] = 0.0, largest
+        kw = dict(q_offset=off, causal=causal)
+        with torch.no_grad():
+            U.check({'out': ops.relpos_attention(q, k, v, table, plan, **kw)}, U.reference(q, k, v, table, plan, **kw))
+        v[:] = 3e38
+        with torch.no_grad():
+            U.check({'out': ops.relpos_attention(q, k, v, table, plan, **kw)}, U.reference(q, k, v, table, plan, **kw))
