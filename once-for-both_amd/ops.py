@@ -7,6 +7,7 @@ import ctypes as C
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import hip
 from .dp import grad_slot
@@ -1059,6 +1060,11 @@ class RelposAttentionPacked(torch.autograd.Function):
         return dqkv, dtable, None, None
 
 
+def _differentiated(*tensors):
+    """whether a call goes through autograd.  Forward mode does too, which refuses it there: a tensor with a tangent need not require a gradient"""
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors) or any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def relpos_attention(q, k, v, table, buckets, scale=None, causal=False, key_lens=None, q_offset=0):
     """softmax(scale q k^T + bias) v with a learned bias of the relative position: bias[b, h, i, j] = table[bucket(position of key j - position of query i), h].
 
@@ -1075,7 +1081,7 @@ def relpos_attention(q, k, v, table, buckets, scale=None, causal=False, key_lens
     call = _RelposCall(q, k, v, table, buckets, scale, causal, key_lens, q_offset)
     if key_lens is not None:
         key_lens = _c(key_lens)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad):
+    if _differentiated(q, k, v, table):
         return RelposAttention.apply(q, k, v, table, key_lens, call)
     return call.forward(_att_operand(q), _att_operand(k), _att_operand(v), _c(table), key_lens, False)[0]
 
@@ -1090,7 +1096,7 @@ def relpos_attention_qkv(qkv, table, buckets, scale=None, causal=False, key_lens
     call = _RelposCall(*qkv.unbind(2), table, buckets, scale, causal, key_lens, 0, bound if qkv.dtype == torch.float32 else None)
     if key_lens is not None:
         key_lens = _c(key_lens)
-    if torch.is_grad_enabled() and (qkv.requires_grad or table.requires_grad):
+    if _differentiated(qkv, table):
         return RelposAttentionPacked.apply(qkv, table, key_lens, call)
     return call.forward(*(_att_operand(t) for t in qkv.unbind(2)), _c(table), key_lens, False)[0]
 

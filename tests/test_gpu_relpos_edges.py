@@ -202,3 +202,24 @@ def test_the_largest_float32(largest):
         v[:] = 3e38
         with torch.no_grad():
             U.check({'out': ops.relpos_attention(q, k, v, table, plan, **kw)}, U.reference(q, k, v, table, plan, **kw))
+
+
+def test_forward_mode_is_refused():
+    """a tangent is never dropped in silence: dual tensors need not require a gradient, with and without gradients enabled"""
+    from torch.autograd import forward_ad
+    plan = PLANS['clip']()
+    q, k, v, table, dout = make(35, 1, 5, 5, 1, 64, torch.float32, plan)
+    qkv = torch.stack([q, k, v], 2)
+    with forward_ad.dual_level():
+        plain = ops.relpos_attention(q, k, v, table, plan)
+        for enabled in (True, False):
+            with torch.set_grad_enabled(enabled):
+                for at in range(4):
+                    ins = [q, k, v, table]
+                    ins[at] = forward_ad.make_dual(ins[at], torch.ones_like(ins[at]))
+                    with pytest.raises(RuntimeError):
+                        ops.relpos_attention(*ins, plan)
+                for ins in ((forward_ad.make_dual(qkv, qkv), table), (qkv, forward_ad.make_dual(table, table))):
+                    with pytest.raises(RuntimeError):
+                        ops.relpos_attention_qkv(*ins, plan)
+    assert torch.equal(plain, ops.relpos_attention(q, k, v, table, plan))
