@@ -6,7 +6,7 @@ positions themselves."""
 import numpy as np
 import torch
 
-from .hip import OfbError
+from .hip import OfbError, raw_stream
 
 MAX_WIDTH = 4096
 _FAR = 1 << 26                         # (four times a difference of two positions and `lo` stays a 32-bit number)
@@ -17,8 +17,8 @@ class RelPosBuckets:
     positions: (positions of the queries, positions of the keys) as integer sequences, for sequences of exactly those lengths - default: key j
     stands at j and query i at i + q_offset.
 
-    One plan serves any number of layers, batches and devices; `to(device)` uploads it ahead of the first call (a call uploads it
-    otherwise, which a captured graph cannot)."""
+    One plan serves any number of layers, batches, devices and streams; `to(device)` uploads it ahead of the first call (a call uploads it
+    otherwise, which a captured graph cannot).  A captured graph reads the upload at every replay: keep the plan as long as the graph."""
 
     def __init__(self, lut, lo, num_buckets=None, positions=None):
         lut = [int(x) for x in (lut.tolist() if isinstance(lut, torch.Tensor) else lut)]
@@ -61,7 +61,7 @@ class RelPosBuckets:
         device = torch.device(device)
         if device.index is None and device.type == 'cuda':
             device = torch.device('cuda', torch.cuda.current_device())
-        got = self._on.get(device)
+        got, raw = self._on.get(device), raw_stream(device)
         if got is None:
             lut = np.asarray(self.lut)
             start = np.cumsum(np.bincount(lut, minlength=self.num_buckets))
@@ -69,10 +69,14 @@ class RelPosBuckets:
             flat = torch.from_numpy(np.concatenate(parts).astype(np.int32)).to(device)
             sizes = [self.width, self.num_buckets + 1, self.width, *(len(p) for p in self.positions or ())]
             parts = list(flat.split(sizes))
-            got = self._on[device] = tuple(parts) if self.positions else (*parts, None, None)
+            got = self._on[device] = (tuple(parts) if self.positions else (*parts, None, None), {raw})
             if device.type == 'cuda':
                 torch.cuda.current_stream(device).synchronize()      # any stream may read the plan from here on
-        return got
+        tensors, streams = got
+        if raw not in streams:                                 # a dropped plan's memory waits for the streams that read it
+            streams.add(raw)
+            tensors[0].record_stream(torch.cuda.current_stream(device))      # (one allocation holds all parts)
+        return tensors
 
     def to(self, device):
         self.on(device)

@@ -223,3 +223,23 @@ def test_forward_mode_is_refused():
                     with pytest.raises(RuntimeError):
                         ops.relpos_attention_qkv(*ins, plan)
     assert torch.equal(plain, ops.relpos_attention(q, k, v, table, plan))
+
+
+def test_a_plan_that_is_dropped_while_another_stream_reads_it():
+    """its memory is not handed out before that stream is done.  (What asks for memory meanwhile writes zeros: buckets like any other.)"""
+    side = torch.cuda.Stream()
+    q, k, v, table, dout = make(7, 2, 60, 60, 2, 64, torch.bfloat16, RelPosBuckets.clipped(30))
+    want = ops.relpos_attention(q, k, v, table, RelPosBuckets.clipped(30))
+    for _ in range(3):
+        plan = RelPosBuckets.clipped(30).to('cuda')
+        words = sum(t.numel() for t in plan.on('cuda') if t is not None)
+        ops.relpos_attention(q, k, v, table, plan)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            got = ops.relpos_attention(q, k, v, table, plan)
+        del plan
+        taken = [torch.zeros(words, dtype=torch.int32, device='cuda') for _ in range(64)]
+        side.synchronize()
+        assert torch.equal(got, want)
+        del taken

@@ -145,3 +145,26 @@ def test_bias_tables_are_not_decayed():
     by_id = {id(p): n for n, p in m.named_parameters()}
     kept = {by_id[id(p)] for g in param_groups_lrd(m, no_weight_decay_list=m.no_weight_decay()) if g['weight_decay'] == 0 for p in g['params']}
     assert set(tables) <= kept
+
+
+def test_a_plan_is_kept_for_the_streams_that_read_it(monkeypatch):
+    """every stream that a call of the plan runs on is made known to the allocator once, for the memory of all its parts"""
+    from ofb_amd import relpos
+    device, current, known, syncs = torch.device('cuda', 0), [7], [], []
+
+    class Stream:
+        synchronize = staticmethod(lambda: syncs.append(current[0]))
+
+    monkeypatch.setattr(relpos, 'raw_stream', lambda d: current[0])
+    monkeypatch.setattr(torch.cuda, 'current_stream', lambda d=None: Stream)
+    monkeypatch.setattr(torch.Tensor, 'to', lambda self, d: self)
+    monkeypatch.setattr(torch.Tensor, 'record_stream', lambda self, s: known.append((current[0], self.untyped_storage().data_ptr())))
+    for plan in (RelPosBuckets.grid(2, 3), RelPosBuckets.clipped(4)):
+        known.clear(), syncs.clear()
+        parts = plan.on(device)
+        memory = {t.untyped_storage().data_ptr() for t in parts if t is not None}
+        assert syncs == [7] and not known and len(memory) == 1
+        for current[0] in (7, 8, 8, 9, 7, 8):
+            assert plan.on(device) is parts
+        assert known == [(8, *memory), (9, *memory)] and syncs == [7]
+        current[0] = 7
