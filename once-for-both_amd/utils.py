@@ -267,6 +267,7 @@ def init_distributed_mode(args):
     args.distributed = True
     torch.cuda.set_device(args.gpu)
     args.dist_backend = 'nccl'
+    hip.ensure_side_stream(torch.device('cuda', args.gpu))     # before RCCL's streams exist (hardware-queue mapping)
     print('| distributed init (rank {}): {}'.format(args.rank, args.dist_url), flush=True)
     torch.distributed.init_process_group(backend=args.dist_backend, init_method=args.dist_url, world_size=args.world_size,
                                          rank=args.rank)

@@ -83,3 +83,19 @@ def test_loss_scaler_stand_in_and_rank_helpers():
     finally:
         os.environ.update(saved)
     assert a.distributed is False
+
+
+def test_the_side_stream_comes_before_the_process_group(monkeypatch):
+    """a side stream created after RCCL's streams can share the main stream's hardware queue"""
+    from ofb_amd import hip, utils
+    did = []
+    monkeypatch.setenv('RANK', '3'), monkeypatch.setenv('WORLD_SIZE', '8'), monkeypatch.setenv('LOCAL_RANK', '2')
+    monkeypatch.setattr(torch.cuda, 'set_device', lambda d: did.append(('device', d)))
+    monkeypatch.setattr(hip, 'ensure_side_stream', lambda d: did.append(('side stream', d.index)))
+    monkeypatch.setattr(torch.distributed, 'init_process_group', lambda **kw: did.append(('group', kw['rank'])))
+    monkeypatch.setattr(torch.distributed, 'barrier', lambda: did.append(('barrier',)))
+    monkeypatch.setattr(utils, 'setup_for_distributed', lambda master: did.append(('print', master)))
+    a = types.SimpleNamespace(gpu=None, dist_url='env://')
+    utils.init_distributed_mode(a)
+    assert did == [('device', 2), ('side stream', 2), ('group', 3), ('barrier',), ('print', False)]
+    assert (a.rank, a.world_size, a.gpu, a.distributed) == (3, 8, 2, True)
