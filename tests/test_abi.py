@@ -42,3 +42,26 @@ def test_product_never_imports_oracle():
             if f.endswith('.py'):
                 src = open(os.path.join(dp, f)).read()
                 assert 'oracle' not in src.replace('no oracle', ''), f'{f} mentions the oracle'
+
+
+def test_build_compiles_again_when_asked(monkeypatch):
+    """a process does not repeat what it has just compiled, unless `force` says so"""
+    import __graft_entry__ as entry
+    compiled = []
+
+    class Compiler:
+        def __init__(self, cmd):
+            compiled.append(cmd[-3])
+
+        def wait(self):
+            return 0
+
+    monkeypatch.setattr(entry.subprocess, 'Popen', Compiler)
+    monkeypatch.setattr(entry.subprocess, 'check_call', lambda cmd: None)
+    monkeypatch.setattr(entry, '_built', [None])
+    entry.build()
+    sources = len(compiled)
+    entry.build()
+    assert sources > 5 and len(compiled) == sources
+    entry.build(force=True)
+    assert len(compiled) == 2 * sources
