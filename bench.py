@@ -308,7 +308,7 @@ def main():
     ap.add_argument('--no-cpu-baseline', action='store_true')
     ap.add_argument('--no-prof', action='store_true', help='skip per-kernel HIP-event timing')
     ap.add_argument('--prof-all', action='store_true', help='bracket every tagged kernel family in the sampled steps (default: the GEMM only)')
-    ap.add_argument('--graph', action='store_true', help='search mode: capture the whole step (with N > 1: incl. the RCCL exchange) into a hipGraph and replay it '
+    ap.add_argument('--graph', action='store_true', help='search mode: capture the whole step (one rank: a captured RCCL exchange is refused) into a hipGraph and replay it '
                     '(engine.GraphedStep); for launch-bound sizes (small batches); the sampled profile steps stay eager')
     ap.add_argument('--force-dp', action='store_true', help='exercise the DP bucket path even with one rank (debug)')
     ap.add_argument('--pruned', action='store_true', help='search mode: time the search step of a model that compress() has already cut '
@@ -431,7 +431,7 @@ def main():
         step()
     eager_step = step
     if use_graph:
-        gstep = engine.GraphedStep(eager_step, (opt_p, opt_a, opt_d), reducer=reducer)   # with a reducer the RCCL exchange is captured too
+        gstep = engine.GraphedStep(eager_step, (opt_p, opt_a, opt_d), reducer=reducer)   # (refuses a reducer that exchanges)
         gstep.capture()                                      # two more eager steps on the capture stream, then the capture
         step = gstep
     for _ in range(args.warmup):

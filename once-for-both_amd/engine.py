@@ -90,11 +90,12 @@ class GraphedStep:
     (allocator / workspaces warm); it may use the side stream (it is forked from and joined into the capturing stream).  The AdamW
     instances passed in read their learning rate and bias corrections from device memory inside the graph (optim.AdamW.begin_capture)
     and are refreshed before every replay; random draws (DropPath, patch masking) come from torch's graph-safe generator.
-    With a data-parallel reducer (pass it as `reducer`): the bucketed RCCL all-reduces of the step are captured with it (RCCL
-    collectives are stream-ordered kernels; every rank captures and replays the same sequence) - the launch-bound sizes keep the
-    graph's gain when a second rank exists.  Not across compress() (shapes and buckets change: capture again)."""
+    Not across compress() (shapes change: capture again).  Not with a reducer that exchanges gradients (pass it as `reducer`): captured RCCL
+    all-reduces have aborted the process, in the process group's watchdog thread, and the cause is not shown - such a step runs eagerly."""
 
     def __init__(self, fn, optimizers, reducer=None, side_stream=False):
+        if reducer is not None and (reducer.world > 1 or reducer.force_collective):
+            raise NotImplementedError('GraphedStep: a captured RCCL exchange has aborted the process for a reason that is not known: run the step of a data-parallel job eagerly')
         self.fn, self.opts = fn, [o for o in optimizers if o is not None]
         self.reducer, self.side_stream = reducer, side_stream
         self.graph, self.out, self.k, self._keep = None, None, 0, None

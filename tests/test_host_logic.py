@@ -182,3 +182,14 @@ def test_distillation_loss_soft_and_hard_match_reference_expressions():
         assert torch.allclose(got, base(out, labels) * 0.7 + d * 0.3, atol=1e-6)
     with pytest.raises(ValueError):
         DistillationLoss(base, teacher, 'soft', 0.3, 2.0)(x, out, labels)
+
+
+def test_a_captured_gradient_exchange_is_refused():
+    """it has aborted the process, and why is not known; a reducer of one rank exchanges nothing"""
+    from types import SimpleNamespace
+    from ofb_amd import engine
+    for world, force in ((2, False), (1, True)):
+        with pytest.raises(NotImplementedError):
+            engine.GraphedStep(lambda: None, [], reducer=SimpleNamespace(world=world, force_collective=force))
+    engine.GraphedStep(lambda: None, [], reducer=SimpleNamespace(world=1, force_collective=False))
+    engine.GraphedStep(lambda: None, [])
