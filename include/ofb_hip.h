@@ -240,7 +240,7 @@ int ofb_attention_bwd(const float* qkv, const float* out, const float* lse, cons
                       int32_t N, int32_t H, int32_t dh, float scale, const float* qkv_bound, const float* dout_bound,
                       float* dqkv_amax, void* stream);
 /* The same with the maximum left as ONE WORD PER WORKGROUP: wg_amax[B * H] (required) is plainly written - no atomic max, and nothing to
- * zero ahead of the launch (ofb_attention_bwd enqueues a 4-byte memset node for its scalar); hand the vector to ofb_to_hformat_colsum_nb */
+ * zero ahead of the launch (ofb_attention_bwd clears its scalar with a fill kernel); hand the vector to ofb_to_hformat_colsum_nb */
 int ofb_attention_bwd_wgmax(const float* qkv, const float* out, const float* lse, const float* dout, float* dqkv, int32_t B,
                             int32_t N, int32_t H, int32_t dh, float scale, const float* qkv_bound, const float* dout_bound,
                             float* wg_amax, void* stream);

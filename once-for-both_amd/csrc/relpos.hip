@@ -13,7 +13,11 @@
 // finds them).  Scores, softmax statistics, dS and all sums are f32 (the table's gradient sums in 64 bits); P and dS are rounded to the operand
 // type for the second product: bf16 as they are, f16 with dS times a power of two that keeps it below 2^15 (and P times 2^14 for dV), f32 likewise
 // in two f16 planes.  (f32 operands of any size: exponents run from 2^-113, for f32's largest value, to 2^112, where a tensor whose maximum is below 2^-97 is
-// held to 2^-137.  What has to fit f32 is what f32 arithmetic forms too: scores, dP and dS.)
+// held to 2^-137.  What has to fit f32 is what f32 arithmetic forms too: scores, dP and dS.  A value keeps 22 bits, and no less than 2^-39 of the maximum behind its
+// exponent: one huge key or value lowers what the rows that do not meet it keep.)
+// bf16 / f16: P and dS as one term, because their rounding is of the size of the operands' own, and the result's: errors against 64 bits are 1.2 to 1.45 times those of one rounding at
+// the end (bf16: 0.0021 / 0.0017 for out, 0.0024 / 0.0017 for the gradients; f16: 0.00029 / 0.00021).  As two terms (value and remainder) they are those of one rounding, and the kernels run
+// one product more for each: 6007 tokens bf16, train, 1064 and 1286 us; 16 x 512 181 and 198; 4 x 1025 causal f16 187 and 205; one token over caches 94 and 101.
 //
 // Operand conventions (lane l, hh = l >> 5): A[row = l & 31][k = 8 hh + j], B[k = 8 hh + j][col = l & 31], accumulator register r holds
 // row 8 (r >> 2) + 4 hh + (r & 3) of column l & 31.  A reduction may run over its index in any order that both operands share, so an

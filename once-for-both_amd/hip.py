@@ -794,7 +794,7 @@ def attention_fwd_h(qkv, out, outP, lse, B, N, H, dh, scale, qkv_bound=None):
 def attention_bwd(qkv, out, lse, dout, dqkv, B, N, H, dh, scale, qkv_bound=None, dout_bound=None, dqkv_amax=None, wg_amax=None):
     """qkv_bound: the bound the forward used; dout_bound: device scalar >= max |dout|; dqkv_amax: device scalar that receives
     max |dqkv| (the bound for its H-format copy); wg_amax [B * H] instead: one word per workgroup, written without atomics and without
-    a memset node ahead of the launch - to_hformat(..., colsum_out=..., bound=wg_amax) reduces the vector itself"""
+    a fill kernel ahead of the launch - to_hformat(..., colsum_out=..., bound=wg_amax) reduces the vector itself"""
     _check_lse(lse, B, N, H)
     qkv_bound = qkv_bound if qkv_bound is not None else amax(qkv)
     dout_bound = dout_bound if dout_bound is not None else amax(dout)
