@@ -1061,8 +1061,11 @@ class RelposAttentionPacked(torch.autograd.Function):
 
 
 def _differentiated(*tensors):
-    """whether a call goes through autograd.  Forward mode does too, which refuses it there: a tensor with a tangent need not require a gradient"""
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors) or any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    """whether a call goes through autograd.  Forward mode does too, which refuses it there: a tensor with a tangent need not require a gradient.
+    (Outside of a dual level, 3.6 us of host time for four tensors, none is asked.)"""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def relpos_attention(q, k, v, table, buckets, scale=None, causal=False, key_lens=None, q_offset=0):
@@ -1077,7 +1080,8 @@ def relpos_attention(q, k, v, table, buckets, scale=None, causal=False, key_lens
     and the gradients, that meet it NaN, and the table's gradient of its head.
     float32 tensors may have any finite size as long as scores and dout v^T fit float32.  Their values enter the products with 22 bits, and not finer than 2^-39 of the largest |k| and
     |v| of the head that a query sees and of the largest |q| and |dout| of a head: one huge key or value lowers what the rows that do not meet it keep.  bfloat16 and float16: the
-    weights and the scores' gradients are rounded to the type once, as operands of the products that follow."""
+    weights and the scores' gradients are rounded to the type once, as operands of the products that follow; |v| times the number of keys has to fit float32.
+    Forward-mode differentiation is refused."""
     call = _RelposCall(q, k, v, table, buckets, scale, causal, key_lens, q_offset)
     if key_lens is not None:
         key_lens = _c(key_lens)
